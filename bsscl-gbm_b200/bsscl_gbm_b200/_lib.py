@@ -35,7 +35,9 @@ EXPORTS = (
     "gbm_predict_upload_raw", "gbm_predict_raw", "gbm_test_peer_wait", "gbm_upload_labels_mc",
     "gbm_round_mc", "gbm_get_F_mc", "gbm_get_grad_mc", "gbm_upload_targets", "gbm_round_reg",
     "gbm_check_model", "gbm_sampler_create_device", "gbm_predict_upload_u16", "gbm_round_mc_sampled",
-    "gbm_round_reg_sampled",
+    "gbm_round_reg_sampled", "gbm_softmax_xent", "gbm_softmax_xent_grad", "gbm_softmax_xent_workspace",
+    "gbm_leaf_linear", "gbm_leaf_linear_grad", "gbm_leaf_linear_workspace", "gbm_grad_clip_plan_bytes",
+    "gbm_grad_clip_plan", "gbm_grad_clip", "gbm_grad_clip_workspace", "gbm_ops_status",
 )
 
 
@@ -167,6 +169,23 @@ def lib():
     L.gbm_predict_noalloc.argtypes = [P, i64, i32, P, P, P, P, P, P, i32, i32, f64, f64, P, P, P,
                                       C.c_char_p, i32]
     L.gbm_check_model.argtypes = [C.POINTER(GbmPacked), i32, C.c_char_p, i32]
+    L.gbm_softmax_xent.argtypes = [P, i64, P, i64, i32, i64, i64, i64, P, P, P, P, i64, P, C.c_char_p, i32]
+    L.gbm_softmax_xent_grad.argtypes = [P, i64, P, i64, i32, i64, i64, i64, P, P, P, P, i64, P, i64, P, i64, P,
+                                        C.c_char_p, i32]
+    L.gbm_softmax_xent_workspace.argtypes = [i64, i64, i64, i32]
+    L.gbm_softmax_xent_workspace.restype = i64
+    L.gbm_leaf_linear.argtypes = [P, i64, P, P, i32, i64, i32, i64, i64, P, i64, i32, P, i64, P, C.c_char_p, i32]
+    L.gbm_leaf_linear_grad.argtypes = [P, i64, P, P, P, i64, i32, i64, i32, i64, i64, P, i64, i32, P, P, i64, P,
+                                       C.c_char_p, i32]
+    L.gbm_leaf_linear_workspace.argtypes = [i64, i32, i64, i64, i32]
+    L.gbm_leaf_linear_workspace.restype = i64
+    L.gbm_grad_clip_plan_bytes.argtypes = [P, i32]
+    L.gbm_grad_clip_plan_bytes.restype = i64
+    L.gbm_grad_clip_plan.argtypes = [P, P, P, P, i32, P, i64, C.c_char_p, i32]
+    L.gbm_grad_clip.argtypes = [P, P, f64, P, P, i64, P, C.c_char_p, i32]
+    L.gbm_grad_clip_workspace.argtypes = [P]
+    L.gbm_grad_clip_workspace.restype = i64
+    L.gbm_ops_status.argtypes = [P, C.c_char_p, i32]
     _lib = L
     return L
 

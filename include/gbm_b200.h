@@ -373,6 +373,113 @@ int gbm_predict_noalloc(const uint8_t *xbin_dev, int64_t n, int32_t p, const int
                         int32_t n_nodes, double learning_rate, double base_score, double *F_dev,
                         double *proba_dev, void *stream, char *errbuf, int32_t errlen);
 
+/* ---- device operators for leaf-wise linear models ----------------------- */
+
+/* A training step of a linear softmax model whose rows the trees have routed
+ * into leaves: products grouped by leaf, softmax cross entropy over many
+ * classes, and clipping of the gradients.  No reference counterpart: the
+ * reference's leaves hold constants, and its multi-class loss (E:2989-3008)
+ * keeps F for every row and class.
+ *
+ * Every call takes device pointers the caller owns (inputs, outputs and
+ * workspace), runs on `stream` (a cudaStream_t, NULL = the default stream)
+ * of the current device, allocates nothing, waits for nothing and can be
+ * captured into a CUDA graph.  Calls that overlap need workspaces of their
+ * own.  Outputs must not overlap inputs or one another unless a call says
+ * so.  `errbuf` (optional, `errlen` bytes) receives a message.  A null
+ * pointer, a size out of range, a row stride below its row, a pointer not
+ * aligned to its elements or a workspace that is too small is GBM_ERR_ARG, a
+ * type that a call does not take GBM_ERR_UNSUPPORTED; nothing is launched
+ * then. */
+enum {
+    GBM_TYPE_F32 = 0,
+    GBM_TYPE_BF16 = 2,
+    GBM_TYPE_F16 = 3
+};
+
+/* Softmax cross entropy of a linear head over v classes, without keeping the
+ * logits.  x [n][d] (row stride ldx elements) and w [v][d] (row stride ldw)
+ * in `dtype` (GBM_TYPE_BF16 or GBM_TYPE_F16); l_ik = x_i . w_k is summed in
+ * 32 bits.  lse [n] f32 gets log sum_k exp l_ik, and loss [n] f32 gets
+ * lse_i - l_i,target_i.  A row whose target is outside 0..v-1 is ignored: its loss is 0
+ * (its lse is still computed).  n >= 0, d and v >= 1, each below 2^31 - 512.
+ * ws: gbm_softmax_xent_workspace(n, d, v, 0) bytes, 256-byte aligned. */
+int gbm_softmax_xent(const void *x, int64_t ldx, const void *w, int64_t ldw, int32_t dtype, int64_t n,
+                     int64_t d, int64_t v, const int64_t *target, float *loss, float *lse, void *ws,
+                     int64_t ws_bytes, void *stream, char *errbuf, int32_t errlen);
+
+/* The gradients of sum_i grad_loss_i loss_i: with
+ * G_ik = grad_loss_i (exp(l_ik - lse_i) - [k = target_i]), dx = G w [n][d] and
+ * dw = G^T x [v][d] (row strides lddx, lddw), in `dtype`.  Either may be
+ * NULL.  An ignored row adds nothing to dw, whatever its features hold, and
+ * its dx is 0.  lse is gbm_softmax_xent's; grad_loss [n] f32.  G is made a piece of
+ * classes at a time and rounded to `dtype` for the products (to half
+ * precision times a power of two that follows the largest |grad_loss|, so
+ * that small probabilities keep their bits); the products are summed in 32
+ * bits.  ws: gbm_softmax_xent_workspace(n, d, v, 1) bytes, 256-byte aligned. */
+int gbm_softmax_xent_grad(const void *x, int64_t ldx, const void *w, int64_t ldw, int32_t dtype, int64_t n,
+                          int64_t d, int64_t v, const int64_t *target, const float *lse,
+                          const float *grad_loss, void *dx, int64_t lddx, void *dw, int64_t lddw, void *ws,
+                          int64_t ws_bytes, void *stream, char *errbuf, int32_t errlen);
+
+/* Workspace of the two calls above in bytes (grad 0: the loss, 1: the
+ * gradients); -1 when a size is out of range. */
+int64_t gbm_softmax_xent_workspace(int64_t n, int64_t d, int64_t v, int32_t grad);
+
+/* Products grouped by leaf.  The rows of x [t][din] (row stride ldx) lie leaf
+ * after leaf: leaf g has the rows offsets[g] .. offsets[g+1]-1 (offsets
+ * [groups+1] int32 on the device, non-decreasing, within 0..t; a leaf may
+ * have none), and y_r = w_g x_r with w [groups][dout][din] contiguous.  y
+ * [t][dout] has row stride ldy.  x, w and y in `dtype` (GBM_TYPE_BF16 or
+ * GBM_TYPE_F16), sums in 32 bits.  Rows before the first leaf and behind the
+ * last one are set to 0 when zero_rest is not 0, else left as they were.
+ * Offsets that break the rule are clamped into 0..t and a leaf with a
+ * negative row count has no rows, so no access leaves the arrays.  t >= 0,
+ * groups, din and dout >= 1, groups below 65536, the others below 2^31 - 512.
+ * ws: gbm_leaf_linear_workspace(t, groups, din, dout, 0) bytes. */
+int gbm_leaf_linear(const void *x, int64_t ldx, const void *w, const int32_t *offsets, int32_t dtype,
+                    int64_t t, int32_t groups, int64_t din, int64_t dout, void *y, int64_t ldy,
+                    int32_t zero_rest, void *ws, int64_t ws_bytes, void *stream, char *errbuf,
+                    int32_t errlen);
+
+/* Its gradients: dx_r = w_g^T dy_r [t][din] (row stride lddx, rows outside
+ * the leaves as zero_rest says) and dw_g = sum over leaf g's rows of
+ * dy_r x_r^T [groups][dout][din] contiguous (0 for a leaf without rows).
+ * dx or dw may be NULL; w is read for dx only, x for dw only (either may be
+ * NULL otherwise).  ws: gbm_leaf_linear_workspace(t, groups, din, dout, 1). */
+int gbm_leaf_linear_grad(const void *x, int64_t ldx, const void *w, const int32_t *offsets, const void *dy,
+                         int64_t lddy, int32_t dtype, int64_t t, int32_t groups, int64_t din, int64_t dout,
+                         void *dx, int64_t lddx, int32_t zero_rest, void *dw, void *ws, int64_t ws_bytes,
+                         void *stream, char *errbuf, int32_t errlen);
+int64_t gbm_leaf_linear_workspace(int64_t t, int32_t groups, int64_t din, int64_t dout, int32_t grad);
+
+/* The global 2-norm of many gradients, and clipping.  A plan describes the
+ * gradients: src[i] and dst[i] (device addresses, contiguous; dst[i] may be
+ * src[i], no other overlap), sizes[i] >= 0 elements of dtypes[i]
+ * (GBM_TYPE_F32, _BF16 or _F16).  gbm_grad_clip_plan checks them on the host
+ * and writes the plan into plan_host (gbm_grad_clip_plan_bytes bytes); the
+ * caller copies it to plan_dev (16-byte aligned) once and keeps both as long
+ * as the buffers stay.  Overlapping buffers are GBM_ERR_ARG. */
+int64_t gbm_grad_clip_plan_bytes(const int64_t *sizes, int32_t n);
+int gbm_grad_clip_plan(const void *const *src, void *const *dst, const int64_t *sizes, const int32_t *dtypes,
+                       int32_t n, void *plan_host, int64_t plan_bytes, char *errbuf, int32_t errlen);
+
+/* norm (f32, device) = sqrt of the sum of all squares (summed in 64 bits,
+ * the same at every call), and dst = src * min(1, max_norm / (norm + 1e-6)),
+ * the factor computed in 64 bits and rounded to 32.  A norm that is not
+ * finite goes through the same formula (an infinite one makes finite entries
+ * 0, NaN makes all NaN).  ws: gbm_grad_clip_workspace(plan_host) bytes,
+ * 16-byte aligned. */
+int gbm_grad_clip(const void *plan_host, const void *plan_dev, double max_norm, float *norm, void *ws,
+                  int64_t ws_bytes, void *stream, char *errbuf, int32_t errlen);
+int64_t gbm_grad_clip_workspace(const void *plan_host);
+
+/* Waits for `stream` and tells whether a bounded wait inside one of the
+ * operators ran out on the current device since the last time it was asked
+ * (GBM_ERR_TIMEOUT: their outputs are not valid); also the first
+ * asynchronous error (GBM_ERR_CUDA). */
+int gbm_ops_status(void *stream, char *errbuf, int32_t errlen);
+
 /* Synchronise the context's stream; returns the first asynchronous error
  * (no reference counterpart). */
 int gbm_sync(gbm_ctx *ctx);
