@@ -172,12 +172,12 @@ def lib():
     L.gbm_softmax_xent.argtypes = [P, i64, P, i64, i32, i64, i64, i64, P, P, P, P, i64, P, C.c_char_p, i32]
     L.gbm_softmax_xent_grad.argtypes = [P, i64, P, i64, i32, i64, i64, i64, P, P, P, P, i64, P, i64, P, i64, P,
                                         C.c_char_p, i32]
-    L.gbm_softmax_xent_workspace.argtypes = [i64, i64, i64, i32]
+    L.gbm_softmax_xent_workspace.argtypes = [i64, i64, i64, i32, i32]
     L.gbm_softmax_xent_workspace.restype = i64
     L.gbm_leaf_linear.argtypes = [P, i64, P, P, i32, i64, i32, i64, i64, P, i64, i32, P, i64, P, C.c_char_p, i32]
     L.gbm_leaf_linear_grad.argtypes = [P, i64, P, P, P, i64, i32, i64, i32, i64, i64, P, i64, i32, P, P, i64, P,
                                        C.c_char_p, i32]
-    L.gbm_leaf_linear_workspace.argtypes = [i64, i32, i64, i64, i32]
+    L.gbm_leaf_linear_workspace.argtypes = [i64, i32, i64, i64, i32, i32]
     L.gbm_leaf_linear_workspace.restype = i64
     L.gbm_grad_clip_plan_bytes.argtypes = [P, i32]
     L.gbm_grad_clip_plan_bytes.restype = i64

@@ -88,6 +88,11 @@ def _vector(a, name, dtype, n, like):
         raise ValueError(f"{name} must be contiguous")
 
 
+def _in_place(*operands):
+    """1 where every operand's rows start on 16-byte boundaries."""
+    return int(all(a.data_ptr() % 16 == 0 and ld % 8 == 0 for a, ld in operands))
+
+
 def _workspace(size, like):
     if size < 0:
         raise ValueError("a size is out of range")
@@ -109,7 +114,7 @@ def softmax_xent(x, w, target):
     _vector(target, "target", t.int64, n, x)
     loss = t.empty(n, dtype=t.float32, device=x.device)
     lse = t.empty(n, dtype=t.float32, device=x.device)
-    size = lib().gbm_softmax_xent_workspace(n, d, v, 0)
+    size = lib().gbm_softmax_xent_workspace(n, d, v, 0, _in_place((x, ldx), (w, ldw)))
     ws = _workspace(size, x)
     _call("gbm_softmax_xent", x.device, x.data_ptr(), ldx, w.data_ptr(), ldw, _types()[x.dtype], n, d, v,
           target.data_ptr(), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size)
@@ -132,7 +137,7 @@ def softmax_xent_grad(x, w, target, lse, grad_loss, want_dx=True, want_dw=True):
         raise ValueError("neither dx nor dw is wanted")
     dx = t.empty(n, d, dtype=x.dtype, device=x.device) if want_dx else None
     dw = t.empty(v, d, dtype=x.dtype, device=x.device) if want_dw else None
-    size = lib().gbm_softmax_xent_workspace(n, d, v, 1)
+    size = lib().gbm_softmax_xent_workspace(n, d, v, 1, _in_place((x, ldx), (w, ldw)))
     ws = _workspace(size, x)
     if n == 0 and not want_dw:
         return dx, dw
@@ -176,7 +181,7 @@ def leaf_linear(x, w, offsets, out=None):
     y, ldy, rest = _output(out, n, dout, x, "out")
     if n == 0:
         return y
-    size = lib().gbm_leaf_linear_workspace(n, e, din, dout, 0)
+    size = lib().gbm_leaf_linear_workspace(n, e, din, dout, 0, _in_place((x, ldx), (w, din)))
     ws = _workspace(size, x)
     _call("gbm_leaf_linear", x.device, x.data_ptr(), ldx, w.data_ptr(), offsets.data_ptr(), _types()[x.dtype], n, e,
           din, dout, y.data_ptr(), ldy, rest, ws.data_ptr(), size)
@@ -201,7 +206,7 @@ def leaf_linear_grad(x, w, offsets, dy, want_dx=True, want_dw=True):
     dw = t.empty(e, dout, din, dtype=x.dtype, device=x.device) if want_dw else None
     if n == 0 and not want_dw:
         return dx, dw
-    size = lib().gbm_leaf_linear_workspace(n, e, din, dout, 1)
+    size = lib().gbm_leaf_linear_workspace(n, e, din, dout, 1, _in_place((x, ldx), (w, din), (dy, lddy)))
     ws = _workspace(size, x)
     _call("gbm_leaf_linear_grad", x.device, x.data_ptr(), ldx, w.data_ptr(), offsets.data_ptr(), dy.data_ptr(), lddy,
           _types()[x.dtype], n, e, din, dout, dx.data_ptr() if want_dx and n else None, din, 1,

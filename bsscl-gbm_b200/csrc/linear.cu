@@ -6,14 +6,17 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/gbm_b200.h"
+#include "linear_tc.cuh"
 
 namespace {
 
@@ -42,156 +45,520 @@ template <> __device__ __forceinline__ __half from_f(float v) { return __float2h
 template <> __device__ __forceinline__ float from_f(float v) { return v; }
 
 // ---------------------------------------------------------------------------
-// a plain tiled product: c(m, n) = sum_k a(m, k) b(n, k) in 32 bits
+// launches
 // ---------------------------------------------------------------------------
 
-// One operand: element (i, k) at p[i * si + k * sk].
-template <class T> struct Mat {
-    const T *p;
-    int64_t si, sk;
+int sm_count() {
+    static std::atomic<int> cached[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev >= 0 && dev < 64 && cached[dev].load()) return cached[dev].load();
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev >= 0 && dev < 64) cached[dev].store(n);
+    return n;
+}
+
+// A matrix the tensor cores read: rows of `inner` contiguous values, `ld` from
+// one to the next, `batch` matrices of `rows` rows.  box: rows a copy brings.
+struct View {
+    const void *p;
+    int64_t inner, rows, ld;
+    int64_t batch = 1;
 };
 
-// 64 x 64 tile of 256 threads, 4 x 4 products a thread, 16 values of k a
-// step.  epi(m, n, sum) is called for every m < M, n < N.
-template <class TA, class TB, class Epi>
-__device__ void mm_tile(int64_t m0, int64_t n0, int64_t M, int64_t N, int64_t K, Mat<TA> a, Mat<TB> b, Epi epi) {
-    __shared__ float sa[16][68], sb[16][68];
-    const int tid = threadIdx.x, tm = tid / 16, tn = tid % 16;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < K; k0 += 16) {
-        for (int e = tid; e < 64 * 16; e += 256) {
-            // the thread index runs along the operand's contiguous direction
-            int ia = a.sk == 1 ? e / 16 : e % 64, ka = a.sk == 1 ? e % 16 : e / 64;
-            int ib = b.sk == 1 ? e / 16 : e % 64, kb = b.sk == 1 ? e % 16 : e / 64;
-            sa[ka][ia] = (m0 + ia < M && k0 + ka < K) ? to_f(a.p[(m0 + ia) * a.si + (k0 + ka) * a.sk]) : 0.f;
-            sb[kb][ib] = (n0 + ib < N && k0 + kb < K) ? to_f(b.p[(n0 + ib) * b.si + (k0 + kb) * b.sk]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] += sa[k][tm * 4 + i] * sb[k][tn * 4 + j];
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            int64_t m = m0 + tm * 4 + i, n = n0 + tn * 4 + j;
-            if (m < M && n < N) epi(m, n, acc[i][j]);
-        }
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                              const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static std::atomic<EncodeFn> cached;
+    EncodeFn f = cached.load();
+    if (f) return f;
+    void *q = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+        return nullptr;
+    f = reinterpret_cast<EncodeFn>(q);
+    cached.store(f);
+    return f;
 }
+
+struct Err {
+    int code = GBM_OK;
+    const char *what = "";
+    bool bad() const { return code != GBM_OK; }
+};
+
+// The tensor map of boxes of 64 values by `box` rows (128-byte swizzle).
+Err encode(CUtensorMap *map, const View &v, bool bf16, int box) {
+    EncodeFn f = encode_fn();
+    if (!f) return {GBM_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled"};
+    cuuint64_t dims[3] = {(cuuint64_t)v.inner, (cuuint64_t)v.rows, (cuuint64_t)v.batch};
+    cuuint64_t strides[2] = {(cuuint64_t)v.ld * 2, (cuuint64_t)(v.batch > 1 ? v.ld * v.rows * 2 : v.ld * 2)};
+    cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1}, steps[3] = {1, 1, 1};
+    CUresult r = f(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(v.p), dims, strides, boxes,
+                   steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return {GBM_ERR_CUDA, "cuTensorMapEncodeTiled refused an operand"};
+    return {};
+}
+
+// One launch of the frame: `units` tiles at most, a cluster of two CTAs for each, at most one CTA an SM.
+template <class Op> Err launch(const View &a, const View &b, const Op &op, bool bf16, int64_t units, cudaStream_t st) {
+    using S = tc::Shape<Op::kBN>;
+    if (units <= 0) return {};
+    CUtensorMap ma, mb;
+    Err e = encode(&ma, a, bf16, Op::kAMN ? 64 : 128);
+    if (!e.bad()) e = encode(&mb, b, bf16, Op::kBMN ? 64 : Op::kBN / 2);
+    if (e.bad()) return e;
+    static std::atomic<uint64_t> ready;     // devices whose limit for this kernel is set
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return {GBM_ERR_CUDA, "no current CUDA device"};
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(ready.load() & bit)) {
+        if (cudaFuncSetAttribute(tc::k_tc<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
+            return {GBM_ERR_CUDA, "the device does not have the kernel's shared memory"};
+        ready.fetch_or(bit);
+    }
+    const int64_t clusters = std::min<int64_t>(units, sm_count() / 2);
+    if (clusters < 1) return {GBM_ERR_CUDA, "no SMs"};
+    tc::k_tc<Op><<<(unsigned)(2 * clusters), tc::kThreads, S::kSmem, st>>>(ma, mb, op, tc::make_idesc(bf16, Op::kAMN, Op::kBMN, Op::kBN));
+    if (cudaError_t c = cudaGetLastError(); c != cudaSuccess) return {GBM_ERR_CUDA, cudaGetErrorString(c)};
+    return {};
+}
+
+// Whether TMA can read the rows in place: 16-byte boundaries.
+bool tma_rows(const void *p, int64_t ld) { return aligned(p, 16) && ld % 8 == 0; }
+
+// Rows of 16-bit values to rows on 16-byte boundaries, zeros behind the last
+// column; a row whose target is ignored becomes zeros where `target` is given.
+__global__ void __launch_bounds__(256) k_pack(const uint16_t *__restrict__ src, int64_t ld, int64_t rows, int64_t cols, uint16_t *__restrict__ dst,
+                                              int64_t ldp, bool vec, const int64_t *__restrict__ target, int64_t v) {
+    const int64_t per = ldp / 8, total = rows * per;
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const int64_t r = i / per, c = (i - r * per) * 8;
+        uint4 q = make_uint4(0, 0, 0, 0);
+        bool has = true;
+        if (target) {
+            const int64_t y = target[r];
+            has = y >= 0 && y < v;
+        }
+        if (has) {
+            const uint16_t *p = src + r * ld + c;
+            if (vec && c + 8 <= cols) {
+                q = *(const uint4 *)p;
+            } else {
+                uint32_t h[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) h[j] = c + j < cols ? p[j] : 0;
+                q = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+            }
+        }
+        *(uint4 *)(dst + r * ldp + c) = q;
+    }
+}
+
+void pack(const void *src, int64_t ld, int64_t rows, int64_t cols, void *dst, int64_t ldp, const int64_t *target, int64_t v, cudaStream_t st) {
+    const int64_t blocks = std::min<int64_t>((rows * (ldp / 8) + 255) / 256, sm_count() * 16LL);
+    if (blocks > 0)
+        k_pack<<<(unsigned)blocks, 256, 0, st>>>((const uint16_t *)src, ld, rows, cols, (uint16_t *)dst, ldp, tma_rows(src, ld), target, v);
+}
+
+// `v` itself, or its packed copy at `room`.
+View readable(View v, void *room, cudaStream_t st) {
+    if (tma_rows(v.p, v.ld)) return v;
+    const int64_t ldp = round_up(v.inner, 8);
+    pack(v.p, v.ld, v.rows * v.batch, v.inner, room, ldp, nullptr, 0, st);
+    v.p = room;
+    v.ld = ldp;
+    return v;
+}
+
+// ---------------------------------------------------------------------------
+// tiles
+// ---------------------------------------------------------------------------
+
+// The tiles of one dense product, 8 tiles of m beside one another before the
+// next tile of n, so that the 74 tiles worked on at a time share their
+// operands in L2; `splits` parts of the k axis one behind the other.
+struct Dense {
+    int64_t m, n;      // extents of the result
+    int nkb;           // stages of the whole k axis
+    int splits;        // parts of the k axis
+    int kb;            // where B's k axis starts
+    __host__ __device__ int64_t mt() const { return (m + 255) / 256; }
+    template <int BN> __host__ __device__ int64_t nt() const { return (n + BN - 1) / BN; }
+    template <int BN> __host__ __device__ int64_t units() const { return mt() * nt<BN>() * splits; }
+};
+
+template <int BN> struct DenseIter {
+    int64_t at, step;
+    template <class Op> __device__ DenseIter(const Op &, int cid, int ncl) : at(cid), step(ncl) {}
+    template <class Op> __device__ bool next(const Op &op, tc::Tile &t) {
+        const Dense &g = op.dense;
+        const int64_t mt = g.mt(), nt = g.nt<BN>(), tiles = mt * nt;
+        if (at >= tiles * g.splits) return false;
+        const int64_t part = at / tiles, i = at - part * tiles;
+        const int64_t block = i / (8 * nt), rest = i - block * 8 * nt, wide = min((int64_t)8, mt - block * 8);
+        const int64_t tn = rest / wide, tm = block * 8 + (rest - tn * wide);
+        const int per = (g.nkb + g.splits - 1) / g.splits, k0 = min((int)part * per, g.nkb);
+        t.m0 = t.am = (int)(tm * 256);
+        t.n0 = t.bn = (int)(tn * BN);
+        t.mend = (int)min(g.m, tm * 256 + 256);
+        t.nend = (int)min(g.n, tn * BN + BN);
+        t.ka = k0 * tc::kBK;
+        t.kb = g.kb + t.ka;
+        t.nkb = min(per, g.nkb - k0);
+        t.az = t.bz = 0;
+        t.tail = 0;
+        t.aux = (int)part;
+        at += step;
+        return true;
+    }
+};
 
 // ---------------------------------------------------------------------------
 // softmax cross entropy
 // ---------------------------------------------------------------------------
 
-template <class T>
-__global__ void __launch_bounds__(256) k_xent_logits(const T *x, int64_t ldx, const T *w, int64_t ldw, int64_t n,
-                                                     int64_t d, int64_t pc, float *l) {
-    mm_tile(blockIdx.y * 64LL, blockIdx.x * 64LL, n, pc, d, Mat<T>{x, ldx, 1}, Mat<T>{w, ldw, 1},
-            [=](int64_t m, int64_t k, float v) { l[m * pc + k] = v; });
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-// The running maximum and sum of a row over one more piece of its logits:
-// with m' = max(m, max l), s' = s exp(m - m') + sum exp(l - m').
-__global__ void __launch_bounds__(256) k_xent_fold(const float *l, int64_t pc, int64_t c0, int64_t v,
-                                                   const int64_t *target, float *stat_m, float *stat_s,
-                                                   float *loss, float *lse, bool first, bool last) {
-    const int64_t i = blockIdx.x;
-    const float *row = l + i * pc;
-    __shared__ float red[8];
-    float m = -INFINITY;
-    for (int64_t k = threadIdx.x; k < pc; k += 256) m = fmaxf(m, row[k]);
+// (m, s) stands for the sum s exp(m) of exponentials.  With no finite m yet
+// the shift is 0, so that s stays 0 (or NaN, if a NaN is among them).
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x), shift = m == -INFINITY ? 0.f : m;
+    return make_float2(m, a.y * ex2((a.x - shift) * kLog2e) + b.y * ex2((b.x - shift) * kLog2e));
+}
+
+// x w^T, of which each tile leaves the maximum and the sum of exponentials of
+// its 256 classes for each row (part [128 classes][row]), and the target's
+// logit.  One lane of the epilogue has one row, so no exchange between lanes
+// is needed.
+struct XentStats {
+    static constexpr int kBN = 256;
+    static constexpr bool kAMN = false, kBMN = false, kTail = false;
+    using Iter = DenseIter<kBN>;
+    Dense dense;
+    const int64_t *target;
+    float2 *part;
+    float *ly;
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+        const int row = t.m0 + p.row, c0 = p.half * 128, left = t.nend - t.n0 - c0;    // columns of this half that exist
+        const bool in = row < t.mend;
+        const int64_t y = in ? target[row] : -1;
+        const int64_t off = y - t.n0 - c0;
+        const int yc = off >= 0 && off < min(128, left) ? (int)off : -1;
+        float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+            float v[32];
+            tc::tmem_ld32(addr + c, v);
+            tc::tmem_wait(v);
+            if (c == 96) release();
+            if (__any_sync(~0u, yc >= c && yc < c + 32)) {
+                float z = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; i++) z = yc == c + i ? v[i] : z;
+                if (yc >= c && yc < c + 32) ly[row] = z;
+            }
+            if (c + 32 > left) {
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (c + i >= left) v[i] = -INFINITY;
+            }
+            float top[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) top[i] = fmaxf(fmaxf(v[i], v[i + 4]), fmaxf(v[i + 8], v[i + 12]));
+#pragma unroll
+            for (int i = 0; i < 4; i++) top[i] = fmaxf(fmaxf(top[i], fmaxf(v[i + 16], v[i + 20])), fmaxf(v[i + 24], v[i + 28]));
+            const float mc = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
+            const float shift = mc == -INFINITY ? 0.f : mc, z = shift * kLog2e;
+            float e[4] = {s * ex2((m - shift) * kLog2e), 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 32; i++) e[i & 3] += ex2(fmaf(v[i], kLog2e, -z));
+            s = (e[0] + e[1]) + (e[2] + e[3]);
+            m = mc;
+        }
+        if (in) part[((int64_t)(t.n0 / kBN) * 2 + p.half) * dense.m + row] = make_float2(m, s);
+    }
+};
+
+// lse and loss from the tiles' parts: 8 rows a block, 32 threads a row.
+__global__ void __launch_bounds__(256) k_xent_join(const float2 *__restrict__ part, int64_t n, int64_t nt, int64_t v, const int64_t *__restrict__ target,
+                                                   const float *__restrict__ ly, float *__restrict__ loss, float *__restrict__ lse) {
+    __shared__ float2 sh[32][9];
+    const int r = threadIdx.x % 8, q = threadIdx.x / 8;
+    const int64_t row = blockIdx.x * 8LL + r;
+    float2 a = make_float2(-INFINITY, 0.f);
+    if (row < n)
+        for (int64_t k = q; k < nt; k += 32) a = join(a, part[k * n + row]);
+    sh[q][r] = a;
+    __syncthreads();
+    for (int o = 16; o; o >>= 1) {
+        if (q < o) sh[q][r] = join(sh[q][r], sh[q + o][r]);
+        __syncthreads();
+    }
+    if (q || row >= n) return;
+    a = sh[0][r];
+    const float z = a.x == -INFINITY ? logf(a.y) : a.x + logf(a.y);
+    const int64_t y = target[row];
+    lse[row] = z;
+    loss[row] = y >= 0 && y < v ? z - ly[row] : 0.f;
+}
+
+// The power of two that takes the largest |grad_loss| of the rows that count
+// to at most 2^14, half precision's range (scale[0], its inverse in scale[1]).
+__global__ void __launch_bounds__(1024) k_xent_scale(const float *__restrict__ grad_loss, const int64_t *__restrict__ target, int64_t n, int64_t v,
+                                                     float *scale) {
+    __shared__ float red[32];
+    float m = 0.f;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        const int64_t y = target[i];
+        if (y >= 0 && y < v) m = fmaxf(m, fabsf(grad_loss[i]));
+    }
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
     __syncthreads();
-    for (int k = 0; k < 8; k++) m = fmaxf(m, red[k]);
-    float m0 = first ? -INFINITY : stat_m[i];
-    m = fmaxf(m, m0);
-    float s = 0.f;
-    for (int64_t k = threadIdx.x; k < pc; k += 256) s += m == -INFINITY ? (isnan(row[k]) ? row[k] : 0.f) : __expf(row[k] - m);
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = s;
-    __syncthreads();
     if (threadIdx.x) return;
-    s = 0.f;
-    for (int k = 0; k < 8; k++) s += red[k];
-    if (!first && m0 != -INFINITY) s += stat_s[i] * __expf(m0 - m);
-    else if (!first) s += stat_s[i];
-    stat_m[i] = m;
-    stat_s[i] = s;
-    const int64_t y = target[i];
-    if (first) loss[i] = 0.f;
-    if (y >= c0 && y < c0 + pc && y < v) loss[i] = row[y - c0];
-    if (last) {
-        float z = m + logf(s);
-        lse[i] = z;
-        loss[i] = (y >= 0 && y < v) ? z - loss[i] : 0.f;
+    for (int k = 1; k < 32; k++) m = fmaxf(m, red[k]);
+    int e = 0;
+    if (m > 0.f && m < INFINITY) e = min(max(14 - (ilogbf(m) + 1), -100), 100);
+    scale[0] = ldexpf(1.f, e);
+    scale[1] = ldexpf(1.f, -e);
+}
+
+// One piece of G: the logits once more, G = c (exp(l - lse) - [k = target])
+// times the scale, rounded to the products' type.
+template <class T> struct XentG {
+    static constexpr int kBN = 256;
+    static constexpr bool kAMN = false, kBMN = false, kTail = false;
+    using Iter = DenseIter<kBN>;
+    Dense dense;
+    int64_t c0, v;      // the piece's first class; classes in all
+    const int64_t *target;
+    const float *lse, *grad_loss, *scale;
+    T *g;
+    int64_t ldg;
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+        const int row = t.m0 + p.row, h0 = p.half * 128;
+        int64_t y = -1;
+        float c = 0.f, z = 0.f;
+        if (row < t.mend) {
+            y = target[row];
+            if (y >= 0 && y < v) {
+                c = grad_loss[row] * (scale ? *scale : 1.f);
+                z = lse[row] * kLog2e;
+            }
+        }
+        const bool has = y >= 0 && y < v, all = __all_sync(~0u, has);
+        const int64_t off = y - c0 - t.n0 - h0;
+        const int yc = has && off >= 0 && off < 128 ? (int)off : -1;
+        const int row0 = t.m0 + p.row - p.lane;
+        tc::store_tile<T, 128>(
+            p, addr, g + (int64_t)row0 * ldg + t.n0 + h0, ldg, t.mend - row0, t.nend - t.n0 - h0, true, false,
+            [&](float (&x)[32], int col) {
+                const bool here = __any_sync(~0u, yc >= col && yc < col + 32);
+#pragma unroll
+                for (int i = 0; i < 32; i++) x[i] = c * ex2(fmaf(x[i], kLog2e, -z));
+                if (here) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (yc == col + i) x[i] -= c;
+                }
+                if (!all) {    // whatever an ignored row's features hold
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = has ? x[i] : 0.f;
+                }
+            },
+            release);
+    }
+};
+
+// C = A B with B's n axis contiguous: G w (A K-major), G^T x (A's m axis
+// contiguous too).  The result is rounded and stored when one launch makes all
+// of it (acc null); else its f32 sums go to acc [split][m][ldacc], on top of
+// what an earlier piece left there (add).
+template <class T, bool AMN> struct Product {
+    static constexpr int kBN = 256;
+    static constexpr bool kAMN = AMN, kBMN = true, kTail = false;
+    using Iter = DenseIter<kBN>;
+    Dense dense;
+    const int64_t *target;     // rows whose target is ignored are 0 (null: none)
+    int64_t v;
+    const float *scale;        // scale[1] takes G's scale back (null: 1)
+    T *out;
+    int64_t ld;
+    bool vec;
+    float *acc;
+    int64_t ldacc;
+    bool add;
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+        const int row = t.m0 + p.row, row0 = row - p.lane, h0 = p.half * 128, cols = t.nend - t.n0 - h0;
+        if (!acc) {
+            float c = scale ? scale[1] : 1.f;
+            bool has = true;
+            if (target && row < t.mend) {
+                const int64_t y = target[row];
+                has = y >= 0 && y < v;
+            }
+            tc::store_tile<T, 128>(
+                p, addr, out + (int64_t)row0 * ld + t.n0 + h0, ld, t.mend - row0, cols, vec, t.nkb == 0,
+                [&](float (&x)[32], int) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = has ? x[i] * c : 0.f;
+                },
+                release);
+            return;
+        }
+        float *q = acc + ((int64_t)t.aux * dense.m + row) * ldacc + t.n0 + h0;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+            float x[32];
+            if (t.nkb) {
+                tc::tmem_ld32(addr + c, x);
+                tc::tmem_wait(x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i++) x[i] = 0.f;
+            }
+            if (c == 96) release();
+            if (row < t.mend && c < cols) {     // ldacc is a multiple of 64: whole groups of 32 fit
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    float4 w = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                    float4 *d = (float4 *)(q + c) + i;
+                    if (add) {
+                        const float4 o = *d;
+                        w.x += o.x, w.y += o.y, w.z += o.z, w.w += o.w;
+                    }
+                    *d = w;
+                }
+            }
+        }
+    }
+};
+
+// out = the splits' sums, scaled back and rounded; ignored rows 0.
+template <class T>
+__global__ void __launch_bounds__(256) k_sum_splits(const float *__restrict__ acc, int64_t ldacc, int64_t m, int64_t n, int splits,
+                                                    const float *__restrict__ scale, const int64_t *__restrict__ target, int64_t v, T *__restrict__ out,
+                                                    int64_t ld) {
+    const int64_t per = (n + 3) / 4, total = m * per;
+    const float c = scale ? scale[1] : 1.f;
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const int64_t r = i / per, k = (i - r * per) * 4;
+        float4 s = *(const float4 *)(acc + r * ldacc + k);
+        for (int q = 1; q < splits; q++) {
+            const float4 o = *(const float4 *)(acc + (q * m + r) * ldacc + k);
+            s.x += o.x, s.y += o.y, s.z += o.z, s.w += o.w;
+        }
+        bool has = true;
+        if (target) {
+            const int64_t y = target[r];
+            has = y >= 0 && y < v;
+        }
+        const float x[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (k + j < n) out[r * ld + k + j] = from_f<T>(has ? x[j] * c : 0.f);
     }
 }
 
-__global__ void __launch_bounds__(256) k_xent_g(float *l, int64_t pc, int64_t c0, int64_t v, const int64_t *target,
-                                                const float *lse, const float *grad_loss) {
-    const int64_t i = blockIdx.x, y = target[i];
-    float *row = l + i * pc;
-    const bool has = y >= 0 && y < v;
-    const float z = lse[i], c = has ? grad_loss[i] : 0.f;
-    for (int64_t k = threadIdx.x; k < pc; k += 256)
-        row[k] = has ? c * (__expf(row[k] - z) - (c0 + k == y ? 1.f : 0.f)) : 0.f;
-}
-
 template <class T>
-__global__ void __launch_bounds__(256) k_xent_dx(const float *g, int64_t pc, const T *w, int64_t ldw, int64_t n,
-                                                 int64_t d, float *acc, T *dx, int64_t lddx, bool first, bool last,
-                                                 const int64_t *target, int64_t v) {
-    mm_tile(blockIdx.y * 64LL, blockIdx.x * 64LL, n, d, pc, Mat<float>{g, pc, 1}, Mat<T>{w, 1, ldw},
-            [=](int64_t m, int64_t k, float s) {
-                if (!first) s += acc[m * d + k];
-                if (last)
-                    dx[m * lddx + k] = from_f<T>(target[m] >= 0 && target[m] < v ? s : 0.f);
-                else
-                    acc[m * d + k] = s;
-            });
+Err sum_splits(const float *acc, int64_t ldacc, int64_t m, int64_t n, int splits, const float *scale, const int64_t *target, int64_t v, T *out,
+               int64_t ld, cudaStream_t st) {
+    const int64_t blocks = std::min<int64_t>((m * ((n + 3) / 4) + 255) / 256, sm_count() * 16LL);
+    k_sum_splits<T><<<(unsigned)blocks, 256, 0, st>>>(acc, ldacc, m, n, splits, scale, target, v, out, ld);
+    return {};
 }
 
-// x with the ignored rows as zeros
-template <class T> __global__ void k_xent_rows(const T *x, int64_t ldx, int64_t d, const int64_t *target, int64_t v, T *out) {
-    const int64_t i = blockIdx.x;
-    const bool has = target[i] >= 0 && target[i] < v;
-    for (int64_t k = threadIdx.x; k < d; k += blockDim.x) out[i * d + k] = has ? x[i * ldx + k] : from_f<T>(0.f);
+// Parts of the k axis for a product of `tiles` tiles and `nkb` stages: as many
+// as make the longest chain of stages one cluster works through shortest,
+// counting about 8 stages' time for a tile's start and end and the time the
+// f32 sums take to be written and read again (65536 x 8 bytes a tile: about a
+// sixth of a stage's 0.27 us spread over 74 clusters).
+int choose_splits(int64_t tiles, int64_t nkb) {
+    constexpr int64_t kClusters = 74;      // 148 SMs; fixed, so that sizes alone set the workspace
+    int best = 1;
+    double least = 1e300;
+    for (int s = 1; s <= 32 && s <= nkb; s++) {
+        const int64_t waves = (tiles * s + kClusters - 1) / kClusters;
+        const double t = (double)waves * ((nkb + s - 1) / s + 8) + (s > 1 ? 10.0 + tiles * s * 0.3 : 0.0);
+        if (t < least * 0.98) least = t, best = s;
+    }
+    return best;
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) k_xent_dw(const float *g, int64_t pc, const T *x, int64_t n, int64_t d, T *dw,
-                                                 int64_t lddw) {
-    mm_tile(blockIdx.y * 64LL, blockIdx.x * 64LL, pc, d, n, Mat<float>{g, 1, pc}, Mat<T>{x, 1, d},
-            [=](int64_t m, int64_t k, float s) { dw[m * lddw + k] = from_f<T>(s); });
-}
+// How the gradient's work is cut: pieces of classes whose G takes at most
+// 256 MB, and splits of both products' k axes.
+struct XentPlan {
+    int64_t dp;        // features in packed rows
+    int64_t pc;        // classes of a piece, a multiple of 256 unless there is one piece
+    int64_t ldg;       // row stride of G
+    int64_t ldacc;
+    int pieces, sx, sw;
+    XentPlan(int64_t n, int64_t d, int64_t v) {
+        dp = round_up(d, 8);
+        constexpr int64_t kMost = 256 << 20;
+        pieces = (int)std::min<int64_t>((n * v * 2 + kMost - 1) / kMost, (v + 255) / 256);
+        pieces = std::max(pieces, 1);
+        pc = pieces > 1 ? std::min(v, round_up((v + pieces - 1) / pieces, 256)) : v;
+        pieces = (int)((v + pc - 1) / pc);
+        ldg = round_up(pc, 64);
+        ldacc = round_up(d, 64);
+        const int64_t mt = (n + 255) / 256, vt = (pc + 255) / 256, dt = (d + 255) / 256;
+        sx = choose_splits(mt * dt, (pc + 63) / 64);
+        sw = choose_splits(vt * dt, (n + 63) / 64);
+    }
+    bool dx_acc() const { return pieces > 1 || sx > 1; }
+};
 
-// classes of one piece: its logits stay under 64 MB
-int64_t xent_piece(int64_t n, int64_t v) {
-    return std::min(v, std::max<int64_t>(64, (int64_t)(16 << 20) / std::max<int64_t>(n, 1) / 64 * 64));
-}
+struct Room {
+    char *at, *base;
+    explicit Room(void *p) : at((char *)p), base((char *)p) {}
+    template <class T> T *take(int64_t count) {
+        char *r = at;
+        at += round_up(count * (int64_t)sizeof(T), 256);
+        return (T *)r;
+    }
+    int64_t bytes() const { return at - base; }
+};
 
-struct XentWs {
-    float *l, *m, *s, *acc;
-    void *x;
+struct XentLoss {
+    uint16_t *x, *w;
+    float2 *part;
+    float *ly;
     int64_t bytes;
-    XentWs(void *ws, int64_t n, int64_t d, int64_t v, bool grad) {
-        char *p = static_cast<char *>(ws), *at = p;
-        auto take = [&](int64_t b) {
-            char *r = at;
-            at += round_up(b, 256);
-            return r;
-        };
-        l = (float *)take(n * xent_piece(n, v) * 4);
-        m = (float *)take(n * 4);
-        s = (float *)take(n * 4);
-        acc = (float *)take(grad ? n * d * 4 : 0);
-        x = take(grad ? n * d * 2 : 0);
-        bytes = at - p;
+    XentLoss(void *ws, int64_t n, int64_t d, int64_t v, bool in_place) {
+        Room r(ws);
+        const int64_t dp = round_up(d, 8);
+        x = r.take<uint16_t>(in_place ? 0 : n * dp);
+        w = r.take<uint16_t>(in_place ? 0 : v * dp);
+        part = r.take<float2>((v + 255) / 256 * 2 * n);
+        ly = r.take<float>(n);
+        bytes = r.bytes();
+    }
+};
+
+struct XentGrad {
+    uint16_t *x, *w, *g;
+    float *accx, *accw, *scale;
+    int64_t bytes;
+    XentGrad(void *ws, int64_t n, int64_t d, int64_t v, bool in_place) {
+        Room r(ws);
+        const XentPlan pl(n, d, v);
+        scale = r.take<float>(2);
+        x = r.take<uint16_t>(n * pl.dp);
+        w = r.take<uint16_t>(in_place ? 0 : v * pl.dp);
+        g = r.take<uint16_t>(n * pl.ldg);
+        accx = r.take<float>(pl.dx_acc() ? pl.sx * n * pl.ldacc : 0);
+        accw = r.take<float>(pl.sw > 1 ? pl.sw * pl.pc * pl.ldacc : 0);
+        bytes = r.bytes();
     }
 };
 
@@ -199,37 +566,57 @@ bool sizes_ok(int64_t n, int64_t d, int64_t v) {
     return n >= 0 && n <= kMaxDim && d >= 1 && d <= kMaxDim && v >= 1 && v <= kMaxDim;
 }
 
-dim3 tiles(int64_t m, int64_t n) { return dim3((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64)); }
-
-template <class T>
-void xent_forward(const T *x, int64_t ldx, const T *w, int64_t ldw, int64_t n, int64_t d, int64_t v,
-                  const int64_t *target, float *loss, float *lse, void *ws, cudaStream_t st) {
-    XentWs q(ws, n, d, v, false);
-    const int64_t step = xent_piece(n, v);
-    for (int64_t c = 0; c < v; c += step) {
-        int64_t pc = std::min(step, v - c);
-        k_xent_logits<T><<<tiles(n, pc), 256, 0, st>>>(x, ldx, w + c * ldw, ldw, n, d, pc, q.l);
-        k_xent_fold<<<(unsigned)n, 256, 0, st>>>(q.l, pc, c, v, target, q.m, q.s, loss, lse, c == 0, c + pc == v);
-    }
+Err xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, bool bf16, int64_t n, int64_t d, int64_t v, const int64_t *target, float *loss,
+                 float *lse, void *ws, cudaStream_t st) {
+    XentLoss q(ws, n, d, v, tma_rows(x, ldx) && tma_rows(w, ldw));
+    const View a = readable({x, d, n, ldx}, q.x, st), b = readable({w, d, v, ldw}, q.w, st);
+    XentStats op{{n, v, (int)((d + 63) / 64), 1, 0}, target, q.part, q.ly};
+    Err e = launch(a, b, op, bf16, op.dense.units<256>(), st);
+    if (e.bad()) return e;
+    k_xent_join<<<(unsigned)((n + 7) / 8), 256, 0, st>>>(q.part, n, (v + 255) / 256 * 2, v, target, q.ly, loss, lse);
+    return {};
 }
 
 template <class T>
-void xent_backward(const T *x, int64_t ldx, const T *w, int64_t ldw, int64_t n, int64_t d, int64_t v,
-                   const int64_t *target, const float *lse, const float *grad_loss, T *dx, int64_t lddx, T *dw,
-                   int64_t lddw, void *ws, cudaStream_t st) {
-    XentWs q(ws, n, d, v, true);
-    T *xr = static_cast<T *>(q.x);
-    k_xent_rows<T><<<(unsigned)n, 128, 0, st>>>(x, ldx, d, target, v, xr);
-    const int64_t step = xent_piece(n, v);
-    for (int64_t c = 0; c < v; c += step) {
-        int64_t pc = std::min(step, v - c);
-        k_xent_logits<T><<<tiles(n, pc), 256, 0, st>>>(x, ldx, w + c * ldw, ldw, n, d, pc, q.l);
-        k_xent_g<<<(unsigned)n, 256, 0, st>>>(q.l, pc, c, v, target, lse, grad_loss);
-        if (dx)
-            k_xent_dx<T><<<tiles(n, d), 256, 0, st>>>(q.l, pc, w + c * ldw, ldw, n, d, q.acc, dx, lddx, c == 0,
-                                                      c + pc == v, target, v);
-        if (dw) k_xent_dw<T><<<tiles(pc, d), 256, 0, st>>>(q.l, pc, xr, n, d, dw + c * lddw, lddw);
+Err xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t n, int64_t d, int64_t v, const int64_t *target, const float *lse,
+                  const float *grad_loss, T *dx, int64_t lddx, T *dw, int64_t lddw, void *ws, cudaStream_t st) {
+    constexpr bool bf16 = sizeof(T) && std::is_same<T, __nv_bfloat16>::value;
+    const XentPlan pl(n, d, v);
+    XentGrad q(ws, n, d, v, tma_rows(x, ldx) && tma_rows(w, ldw));
+    // rows that count, zeros in the others': an ignored row's features must not reach dw
+    pack(x, ldx, n, d, q.x, pl.dp, target, v, st);
+    const View xs{q.x, d, n, pl.dp}, wv = readable({w, d, v, ldw}, q.w, st);
+    const float *scale = nullptr;
+    if (!bf16) {
+        k_xent_scale<<<1, 1024, 0, st>>>(grad_loss, target, n, v, q.scale);
+        scale = q.scale;
     }
+    T *g = (T *)q.g;
+    for (int64_t c = 0; c < v; c += pl.pc) {
+        const int64_t pc = std::min(pl.pc, v - c);
+        View wp = wv;
+        wp.p = (const char *)wv.p + c * wv.ld * 2;
+        wp.rows = pc;
+        XentG<T> og{{n, pc, (int)((d + 63) / 64), 1, 0}, c, v, target, lse, grad_loss, scale, g, pl.ldg};
+        Err e = launch(xs, wp, og, bf16, og.dense.template units<256>(), st);
+        if (e.bad()) return e;
+        const View gv{g, pc, n, pl.ldg};
+        if (dx) {
+            const bool acc = pl.dx_acc();
+            Product<T, false> op{{n, d, (int)((pc + 63) / 64), pl.sx, 0}, target, v, scale, dx, lddx, tma_rows(dx, lddx), acc ? q.accx : nullptr, pl.ldacc, c > 0};
+            e = launch(gv, wp, op, bf16, op.dense.template units<256>(), st);
+            if (e.bad()) return e;
+        }
+        if (dw) {
+            T *o = dw + c * lddw;
+            Product<T, true> op{{pc, d, (int)((n + 63) / 64), pl.sw, 0}, nullptr, 0, scale, o, lddw, tma_rows(o, lddw), pl.sw > 1 ? q.accw : nullptr, pl.ldacc, false};
+            e = launch(gv, xs, op, bf16, op.dense.template units<256>(), st);
+            if (!e.bad() && pl.sw > 1) e = sum_splits<T>(q.accw, pl.ldacc, pc, d, pl.sw, scale, nullptr, 0, o, lddw, st);
+            if (e.bad()) return e;
+        }
+    }
+    if (dx && pl.dx_acc()) return sum_splits<T>(q.accx, pl.ldacc, n, d, pl.sx, scale, target, v, dx, lddx, st);
+    return {};
 }
 
 // ---------------------------------------------------------------------------
@@ -237,39 +624,157 @@ void xent_backward(const T *x, int64_t ldx, const T *w, int64_t ldw, int64_t n, 
 // ---------------------------------------------------------------------------
 
 // Rows [lo, hi) of leaf g, clamped so that no access leaves the arrays.
-__device__ __forceinline__ void leaf_rows(const int32_t *off, int32_t g, int64_t t, int64_t &lo, int64_t &hi) {
-    lo = min(max((int64_t)off[g], (int64_t)0), t);
-    hi = max(min((int64_t)off[g + 1], t), lo);
+__device__ __forceinline__ void leaf_rows(const int32_t *off, int32_t g, int64_t t, int &lo, int &hi) {
+    lo = (int)min(max((int64_t)off[g], (int64_t)0), t);
+    hi = (int)max(min((int64_t)off[g + 1], t), (int64_t)lo);
 }
 
-// y = x w^T (TRANS 0) or dx = dy w (TRANS 1): one leaf per blockIdx.y, its
-// row tiles taken in turn.
-template <class T, int TRANS>
-__global__ void __launch_bounds__(256) k_leaf_rows(const T *x, int64_t ldx, const T *w, const int32_t *off, int64_t t,
-                                                   int64_t K, int64_t N, T *y, int64_t ldy) {
-    int64_t lo, hi;
-    leaf_rows(off, blockIdx.y, t, lo, hi);
-    const T *wg = w + (int64_t)blockIdx.y * K * N;
-    Mat<T> b = TRANS ? Mat<T>{wg, 1, N} : Mat<T>{wg, K, 1};
-    for (int64_t r = blockIdx.z * 64LL; r < hi - lo; r += gridDim.z * 64LL)
-        mm_tile(r, blockIdx.x * 64LL, hi - lo, N, K, Mat<T>{x + lo * ldx, ldx, 1}, b,
-                [=](int64_t m, int64_t n, float s) { y[(lo + m) * ldy + n] = from_f<T>(s); });
-}
+struct Leaves {
+    const int32_t *off;
+    int64_t t;
+    int32_t groups;
+    int64_t n;          // columns of the result
+    int nkb;
+};
 
-template <class T>
-__global__ void __launch_bounds__(256) k_leaf_dw(const T *x, int64_t ldx, const T *dy, int64_t lddy, const int32_t *off,
-                                                 int64_t t, int64_t din, int64_t dout, T *dw) {
-    int64_t lo, hi;
-    leaf_rows(off, blockIdx.z, t, lo, hi);
-    T *out = dw + (int64_t)blockIdx.z * dout * din;
-    for (int64_t m0 = blockIdx.y * 64LL; m0 < dout; m0 += gridDim.y * 64LL)
-        mm_tile(m0, blockIdx.x * 64LL, dout, din, hi - lo, Mat<T>{dy + lo * lddy, 1, lddy},
-                Mat<T>{x + lo * ldx, 1, ldx}, [=](int64_t m, int64_t n, float s) { out[m * din + n] = from_f<T>(s); });
-}
+// The 256 x BN tiles of all leaves' rows, leaf after leaf.  A warp looks
+// through 32 leaves at a time: each lane counts one leaf's row tiles.
+template <int BN> struct LeafIter {
+    int64_t at, step, base, total, upto;    // tiles before these 32 leaves, in them, in them up to this lane's
+    int first, lo, hi;
+    int64_t nt;
+    template <class Op> __device__ LeafIter(const Op &op, int cid, int ncl) : at(cid), step(ncl), base(0), first(0) {
+        nt = (op.leaves.n + BN - 1) / BN;
+        look(op);
+    }
+    template <class Op> __device__ void look(const Op &op) {
+        const int lane = threadIdx.x % 32, g = first + lane;
+        lo = hi = 0;
+        if (g < op.leaves.groups) leaf_rows(op.leaves.off, g, op.leaves.t, lo, hi);
+        upto = (int64_t)((hi - lo + 255) / 256) * nt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(~0u, upto, o);
+            if (lane >= o) upto += u;
+        }
+        total = __shfl_sync(~0u, upto, 31);
+    }
+    template <class Op> __device__ bool next(const Op &op, tc::Tile &t) {
+        while (at >= base + total) {
+            base += total;
+            first += 32;
+            if (first >= op.leaves.groups) return false;
+            look(op);
+        }
+        const int64_t rel = at - base;
+        const int l = __ffs(__ballot_sync(~0u, upto > rel)) - 1;
+        const int a = __shfl_sync(~0u, lo, l), b = __shfl_sync(~0u, hi, l);
+        const int64_t end = __shfl_sync(~0u, upto, l), rt = (b - a + 255) / 256, i = rel - (end - rt * nt);
+        // 8 row tiles beside one another, as in Dense
+        const int64_t block = i / (8 * nt), rest = i - block * 8 * nt, wide = min((int64_t)8, rt - block * 8);
+        const int64_t tn = rest / wide, tm = block * 8 + (rest - tn * wide);
+        t.m0 = t.am = a + (int)tm * 256;
+        t.n0 = t.bn = (int)(tn * BN);
+        t.mend = min(b, t.m0 + 256);
+        t.nend = (int)min(op.leaves.n, tn * BN + BN);
+        t.ka = t.kb = 0;
+        t.nkb = op.leaves.nkb;
+        t.az = 0;
+        t.bz = first + l;
+        t.tail = 0;
+        t.aux = 0;
+        at += step;
+        return true;
+    }
+};
+
+// y = x w^T (B K-major) or dx = dy w (B's n axis contiguous), leaf by leaf.
+// Rows behind a leaf's last one belong to the next leaf: they are
+// computed with this leaf's weights and not stored.
+template <class T, bool BMN> struct LeafRows {
+    static constexpr int kBN = 256;
+    static constexpr bool kAMN = false, kBMN = BMN, kTail = false;
+    using Iter = LeafIter<kBN>;
+    Leaves leaves;
+    T *out;
+    int64_t ld;
+    bool vec;
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+        const int row0 = t.m0 + p.row - p.lane, h0 = p.half * 128;
+        tc::store_tile<T, 128>(p, addr, out + (int64_t)row0 * ld + t.n0 + h0, ld, t.mend - row0, t.nend - t.n0 - h0, vec, false, [](float (&)[32], int) {}, release);
+    }
+};
+
+// dw: one 256 x 256 tile of one leaf (and one part of its rows) a unit; the k
+// axis is the leaf's rows.
+struct LeafDwIter {
+    int64_t at, step;
+    template <class Op> __device__ LeafDwIter(const Op &, int cid, int ncl) : at(cid), step(ncl) {}
+    template <class Op> __device__ bool next(const Op &op, tc::Tile &t) {
+        const int64_t mt = (op.dout + 255) / 256, nt = (op.din + 255) / 256, per = mt * nt * op.splits;
+        if (at >= per * op.groups) return false;
+        const int g = (int)(at / per), i = (int)(at - g * per), part = (int)(i / (mt * nt)), tile = (int)(i - part * (mt * nt));
+        const int tm = (int)(tile / nt), tn = (int)(tile - tm * nt);
+        int lo, hi;
+        leaf_rows(op.off, g, op.t, lo, hi);
+        const int nkb = (hi - lo + 63) / 64, each = (nkb + op.splits - 1) / op.splits, k0 = min(part * each, nkb), k1 = min(k0 + each, nkb);
+        t.m0 = t.am = tm * 256;
+        t.n0 = t.bn = tn * 256;
+        t.mend = (int)min(op.dout, (int64_t)t.m0 + 256);
+        t.nend = (int)min(op.din, (int64_t)t.n0 + 256);
+        t.ka = t.kb = lo + k0 * 64;
+        t.nkb = k1 - k0;
+        t.az = t.bz = 0;
+        // behind the last row of all TMA fills zeros
+        t.tail = k1 == nkb && hi < op.t ? (hi - lo) % 64 : 0;
+        t.aux = part * op.groups + g;
+        at += step;
+        return true;
+    }
+};
+
+template <class T> struct LeafDw {
+    static constexpr int kBN = 256;
+    static constexpr bool kAMN = true, kBMN = true, kTail = true;
+    using Iter = LeafDwIter;
+    const int32_t *off;
+    int64_t t, din, dout;
+    int32_t groups;
+    int splits;
+    T *out;
+    bool vec;
+    float *acc;         // [split][groups * dout][ldacc] where there are several
+    int64_t ldacc;
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+        const int row = t.m0 + p.row, row0 = row - p.lane, h0 = p.half * 128, cols = t.nend - t.n0 - h0;
+        if (!acc) {
+            tc::store_tile<T, 128>(p, addr, out + ((int64_t)t.aux * dout + row0) * din + t.n0 + h0, din, t.mend - row0, cols, vec, t.nkb == 0,
+                                   [](float (&)[32], int) {}, release);
+            return;
+        }
+        float *q = acc + ((int64_t)t.aux * dout + row) * ldacc + t.n0 + h0;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+            float x[32];
+            if (t.nkb) {
+                tc::tmem_ld32(addr + c, x);
+                tc::tmem_wait(x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i++) x[i] = 0.f;
+            }
+            if (c == 96) release();
+            if (row < t.mend && c < cols) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) ((float4 *)(q + c))[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            }
+        }
+    }
+};
 
 // The rows before the first leaf and behind the last one as zeros.
 template <class T> __global__ void k_leaf_rest(const int32_t *off, int32_t groups, int64_t t, int64_t cols, T *y, int64_t ldy) {
-    int64_t lo = min(max((int64_t)off[0], (int64_t)0), t), hi = max(min((int64_t)off[groups], t), lo);
+    const int64_t lo = min(max((int64_t)off[0], (int64_t)0), t), hi = max(min((int64_t)off[groups], t), lo);
     const int64_t rest = lo + (t - hi);
     for (int64_t r = blockIdx.x; r < rest; r += gridDim.x) {
         T *row = y + (r < lo ? r : hi + r - lo) * ldy;
@@ -277,17 +782,71 @@ template <class T> __global__ void k_leaf_rest(const int32_t *off, int32_t group
     }
 }
 
-unsigned row_blocks(int64_t t) { return (unsigned)std::min<int64_t>(64, std::max<int64_t>(1, t / 64)); }
+int leaf_splits(int64_t t, int32_t groups, int64_t din, int64_t dout) {
+    return choose_splits((int64_t)groups * ((din + 255) / 256) * ((dout + 255) / 256), (t / groups + 63) / 64);
+}
+
+struct LeafWs {
+    uint16_t *x, *w, *dy;
+    float *acc;
+    int64_t ldacc, bytes;
+    LeafWs(void *ws, int64_t t, int32_t groups, int64_t din, int64_t dout, bool grad, bool in_place) {
+        Room r(ws);
+        const int64_t ip = round_up(din, 8), op = round_up(dout, 8);
+        x = r.take<uint16_t>(in_place ? 0 : t * ip);
+        w = r.take<uint16_t>(in_place ? 0 : groups * dout * ip);
+        dy = r.take<uint16_t>(in_place || !grad ? 0 : t * op);
+        ldacc = round_up(din, 64);
+        const int s = grad ? leaf_splits(t, groups, din, dout) : 1;
+        acc = r.take<float>(s > 1 ? s * groups * dout * ldacc : 0);
+        bytes = r.bytes();
+    }
+};
+
+// Tiles of a grouped product at most: each leaf may end in a part of one.
+int64_t leaf_units(int64_t t, int32_t groups, int64_t n) { return ((t + 255) / 256 + groups) * ((n + 255) / 256); }
+
+template <class T, bool BMN>
+Err leaf_rows_launch(const View &a, const View &w, const int32_t *off, int64_t t, int32_t groups, int64_t k, int64_t n, T *y, int64_t ldy, bool zero_rest,
+                     cudaStream_t st) {
+    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    LeafRows<T, BMN> op{{off, t, groups, n, (int)((k + 63) / 64)}, y, ldy, tma_rows(y, ldy)};
+    Err e = launch(a, w, op, bf16, leaf_units(t, groups, n), st);
+    if (!e.bad() && zero_rest) k_leaf_rest<T><<<(unsigned)std::min<int64_t>(t, sm_count()), 256, 0, st>>>(off, groups, t, n, y, ldy);
+    return e;
+}
 
 template <class T>
-void leaf_rows_launch(const T *x, int64_t ldx, const T *w, const int32_t *off, int64_t t, int32_t groups, int64_t K,
-                      int64_t N, bool trans, T *y, int64_t ldy, bool zero_rest, cudaStream_t st) {
-    dim3 grid((unsigned)((N + 63) / 64), (unsigned)groups, row_blocks(t));
-    if (trans)
-        k_leaf_rows<T, 1><<<grid, 256, 0, st>>>(x, ldx, w, off, t, K, N, y, ldy);
-    else
-        k_leaf_rows<T, 0><<<grid, 256, 0, st>>>(x, ldx, w, off, t, K, N, y, ldy);
-    if (zero_rest) k_leaf_rest<T><<<256, 256, 0, st>>>(off, groups, t, N, y, ldy);
+Err leaf_forward(const void *x, int64_t ldx, const void *w, const int32_t *off, int64_t t, int32_t groups, int64_t din, int64_t dout, T *y, int64_t ldy,
+                 bool zero_rest, void *ws, cudaStream_t st) {
+    LeafWs q(ws, t, groups, din, dout, false, tma_rows(x, ldx) && tma_rows(w, din));
+    const View a = readable({x, din, t, ldx}, q.x, st), b = readable({w, din, dout, din, groups}, q.w, st);
+    return leaf_rows_launch<T, false>(a, b, off, t, groups, din, dout, y, ldy, zero_rest, st);
+}
+
+template <class T>
+Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off, const void *dy, int64_t lddy, int64_t t, int32_t groups, int64_t din,
+                  int64_t dout, T *dx, int64_t lddx, bool zero_rest, T *dw, void *ws, cudaStream_t st) {
+    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    const bool in_place = (!dw || tma_rows(x, ldx)) && (!dx || tma_rows(w, din)) && tma_rows(dy, lddy);
+    LeafWs q(ws, t, groups, din, dout, true, in_place);
+    if (!t) {
+        if (dw && cudaMemsetAsync(dw, 0, (size_t)groups * dout * din * 2, st) != cudaSuccess) return {GBM_ERR_CUDA, "cudaMemsetAsync"};
+        return {};
+    }
+    const View g = readable({dy, dout, t, lddy}, q.dy, st);
+    if (dx) {
+        const View b = readable({w, din, dout, din, groups}, q.w, st);
+        Err e = leaf_rows_launch<T, true>(g, b, off, t, groups, dout, din, dx, lddx, zero_rest, st);
+        if (e.bad()) return e;
+    }
+    if (!dw) return {};
+    const View a = readable({x, din, t, ldx}, q.x, st);
+    const int s = leaf_splits(t, groups, din, dout);
+    LeafDw<T> op{off, t, din, dout, groups, s, dw, tma_rows(dw, din), s > 1 ? q.acc : nullptr, q.ldacc};
+    Err e = launch(g, a, op, bf16, (int64_t)groups * s * ((din + 255) / 256) * ((dout + 255) / 256), st);
+    if (!e.bad() && s > 1) e = sum_splits<T>(q.acc, q.ldacc, groups * dout, din, s, nullptr, nullptr, 0, dw, din, st);
+    return e;
 }
 
 // ---------------------------------------------------------------------------
@@ -379,9 +938,9 @@ int type_size(int32_t t) { return t == GBM_TYPE_F32 ? 4 : t == GBM_TYPE_BF16 || 
 
 extern "C" {
 
-int64_t gbm_softmax_xent_workspace(int64_t n, int64_t d, int64_t v, int32_t grad) {
+int64_t gbm_softmax_xent_workspace(int64_t n, int64_t d, int64_t v, int32_t grad, int32_t in_place) {
     if (!sizes_ok(n, d, v)) return -1;
-    return XentWs(nullptr, n, d, v, grad != 0).bytes;
+    return grad ? XentGrad(nullptr, n, d, v, in_place != 0).bytes : XentLoss(nullptr, n, d, v, in_place != 0).bytes;
 }
 
 static int xent_check(const char *what, const void *x, int64_t ldx, const void *w, int64_t ldw, int32_t dtype,
@@ -398,7 +957,7 @@ static int xent_check(const char *what, const void *x, int64_t ldx, const void *
                     (long long)ldx, (long long)ldw, (long long)d);
     if (!aligned(x, 2) || !aligned(w, 2) || !aligned(target, 8) || !aligned(ws, 256))
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: a pointer is not aligned to its elements (workspace: 256 bytes)", what);
-    const int64_t need = gbm_softmax_xent_workspace(n, d, v, grad);
+    const int64_t need = gbm_softmax_xent_workspace(n, d, v, grad, tma_rows(x, ldx) && tma_rows(w, ldw));
     if (need && (!ws || ws_bytes < need))
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes,
                     (long long)need);
@@ -413,11 +972,8 @@ int gbm_softmax_xent(const void *x, int64_t ldx, const void *w, int64_t ldw, int
     if (n && (!loss || !lse || !aligned(loss, 4) || !aligned(lse, 4)))
         return fail(errbuf, errlen, GBM_ERR_ARG, "gbm_softmax_xent: loss or lse is null or not aligned");
     if (!n) return GBM_OK;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == GBM_TYPE_BF16)
-        xent_forward((const __nv_bfloat16 *)x, ldx, (const __nv_bfloat16 *)w, ldw, n, d, v, target, loss, lse, ws, st);
-    else
-        xent_forward((const __half *)x, ldx, (const __half *)w, ldw, n, d, v, target, loss, lse, ws, st);
+    Err e = xent_forward(x, ldx, w, ldw, dtype == GBM_TYPE_BF16, n, d, v, target, loss, lse, ws, static_cast<cudaStream_t>(stream));
+    if (e.bad()) return fail(errbuf, errlen, e.code, "gbm_softmax_xent: %s", e.what);
     return finish("gbm_softmax_xent", errbuf, errlen);
 }
 
@@ -438,29 +994,27 @@ int gbm_softmax_xent_grad(const void *x, int64_t ldx, const void *w, int64_t ldw
         if (dw && cudaMemset2DAsync(dw, lddw * 2, 0, d * 2, v, st) != cudaSuccess) return finish(what, errbuf, errlen);
         return GBM_OK;
     }
-    if (dtype == GBM_TYPE_BF16)
-        xent_backward((const __nv_bfloat16 *)x, ldx, (const __nv_bfloat16 *)w, ldw, n, d, v, target, lse, grad_loss,
-                      (__nv_bfloat16 *)dx, lddx, (__nv_bfloat16 *)dw, lddw, ws, st);
-    else
-        xent_backward((const __half *)x, ldx, (const __half *)w, ldw, n, d, v, target, lse, grad_loss, (__half *)dx,
-                      lddx, (__half *)dw, lddw, ws, st);
+    Err e = dtype == GBM_TYPE_BF16
+                ? xent_backward(x, ldx, w, ldw, n, d, v, target, lse, grad_loss, (__nv_bfloat16 *)dx, lddx, (__nv_bfloat16 *)dw, lddw, ws, st)
+                : xent_backward(x, ldx, w, ldw, n, d, v, target, lse, grad_loss, (__half *)dx, lddx, (__half *)dw, lddw, ws, st);
+    if (e.bad()) return fail(errbuf, errlen, e.code, "%s: %s", what, e.what);
     return finish(what, errbuf, errlen);
 }
 
-int64_t gbm_leaf_linear_workspace(int64_t t, int32_t groups, int64_t din, int64_t dout, int32_t grad) {
+int64_t gbm_leaf_linear_workspace(int64_t t, int32_t groups, int64_t din, int64_t dout, int32_t grad, int32_t in_place) {
     if (!sizes_ok(t, din, dout) || groups < 1 || groups >= 65536) return -1;
-    return 0;
+    return LeafWs(nullptr, t, groups, din, dout, grad != 0, in_place != 0).bytes;
 }
 
 static int leaf_check(const char *what, const int32_t *offsets, int32_t dtype, int64_t t, int32_t groups, int64_t din,
-                      int64_t dout, const void *ws, int64_t ws_bytes, int32_t grad, char *errbuf, int32_t errlen) {
+                      int64_t dout, bool in_place, const void *ws, int64_t ws_bytes, int32_t grad, char *errbuf, int32_t errlen) {
     if (dtype != GBM_TYPE_BF16 && dtype != GBM_TYPE_F16)
         return fail(errbuf, errlen, GBM_ERR_UNSUPPORTED, "%s: type %d is neither bf16 nor f16", what, dtype);
     if (!sizes_ok(t, din, dout) || groups < 1 || groups >= 65536)
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: sizes t=%lld groups=%d din=%lld dout=%lld out of range", what,
                     (long long)t, groups, (long long)din, (long long)dout);
     if (!offsets || !aligned(offsets, 4)) return fail(errbuf, errlen, GBM_ERR_ARG, "%s: offsets null or not aligned", what);
-    const int64_t need = gbm_leaf_linear_workspace(t, groups, din, dout, grad);
+    const int64_t need = gbm_leaf_linear_workspace(t, groups, din, dout, grad, in_place);
     if (need && (!ws || ws_bytes < need || !aligned(ws, 256)))
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: workspace of %lld bytes, %lld needed (256-byte aligned)", what,
                     (long long)ws_bytes, (long long)need);
@@ -471,19 +1025,17 @@ int gbm_leaf_linear(const void *x, int64_t ldx, const void *w, const int32_t *of
                     int32_t groups, int64_t din, int64_t dout, void *y, int64_t ldy, int32_t zero_rest, void *ws,
                     int64_t ws_bytes, void *stream, char *errbuf, int32_t errlen) {
     const char *what = "gbm_leaf_linear";
-    int rc = leaf_check(what, offsets, dtype, t, groups, din, dout, ws, ws_bytes, 0, errbuf, errlen);
+    int rc = leaf_check(what, offsets, dtype, t, groups, din, dout, tma_rows(x, ldx) && tma_rows(w, din), ws, ws_bytes, 0, errbuf,
+                        errlen);
     if (rc != GBM_OK) return rc;
     if (!w || (t && (!x || !y)) || !aligned(x, 2) || !aligned(w, 2) || !aligned(y, 2))
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: null or unaligned pointer", what);
     if (ldx < din || ldy < dout) return fail(errbuf, errlen, GBM_ERR_ARG, "%s: row stride below its row", what);
     if (!t) return GBM_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == GBM_TYPE_BF16)
-        leaf_rows_launch((const __nv_bfloat16 *)x, ldx, (const __nv_bfloat16 *)w, offsets, t, groups, din, dout, false,
-                         (__nv_bfloat16 *)y, ldy, zero_rest != 0, st);
-    else
-        leaf_rows_launch((const __half *)x, ldx, (const __half *)w, offsets, t, groups, din, dout, false, (__half *)y,
-                         ldy, zero_rest != 0, st);
+    Err e = dtype == GBM_TYPE_BF16 ? leaf_forward(x, ldx, w, offsets, t, groups, din, dout, (__nv_bfloat16 *)y, ldy, zero_rest != 0, ws, st)
+                                   : leaf_forward(x, ldx, w, offsets, t, groups, din, dout, (__half *)y, ldy, zero_rest != 0, ws, st);
+    if (e.bad()) return fail(errbuf, errlen, e.code, "%s: %s", what, e.what);
     return finish(what, errbuf, errlen);
 }
 
@@ -492,7 +1044,8 @@ int gbm_leaf_linear_grad(const void *x, int64_t ldx, const void *w, const int32_
                          int64_t lddx, int32_t zero_rest, void *dw, void *ws, int64_t ws_bytes, void *stream,
                          char *errbuf, int32_t errlen) {
     const char *what = "gbm_leaf_linear_grad";
-    int rc = leaf_check(what, offsets, dtype, t, groups, din, dout, ws, ws_bytes, 1, errbuf, errlen);
+    int rc = leaf_check(what, offsets, dtype, t, groups, din, dout,
+                        (!dw || tma_rows(x, ldx)) && (!dx || tma_rows(w, din)) && tma_rows(dy, lddy), ws, ws_bytes, 1, errbuf, errlen);
     if (rc != GBM_OK) return rc;
     if (!dx && !dw) return fail(errbuf, errlen, GBM_ERR_ARG, "%s: neither dx nor dw", what);
     if ((t && !dy) || (dx && !w) || (t && dw && !x) || !aligned(x, 2) || !aligned(w, 2) || !aligned(dy, 2) ||
@@ -501,20 +1054,10 @@ int gbm_leaf_linear_grad(const void *x, int64_t ldx, const void *w, const int32_
     if (lddy < dout || (dw && ldx < din) || (dx && lddx < din))
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: row stride below its row", what);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    auto go = [&](auto tag) {
-        using T = decltype(tag);
-        if (dx && t)
-            leaf_rows_launch((const T *)dy, lddy, (const T *)w, offsets, t, groups, dout, din, true, (T *)dx, lddx,
-                             zero_rest != 0, st);
-        if (dw) {
-            dim3 grid((unsigned)((din + 63) / 64), (unsigned)std::min<int64_t>(65535, (dout + 63) / 64), (unsigned)groups);
-            k_leaf_dw<T><<<grid, 256, 0, st>>>((const T *)x, ldx, (const T *)dy, lddy, offsets, t, din, dout, (T *)dw);
-        }
-    };
-    if (dtype == GBM_TYPE_BF16)
-        go(__nv_bfloat16{});
-    else
-        go(__half{});
+    Err e = dtype == GBM_TYPE_BF16 ? leaf_backward(x, ldx, w, offsets, dy, lddy, t, groups, din, dout, (__nv_bfloat16 *)dx, lddx, zero_rest != 0,
+                                                   (__nv_bfloat16 *)dw, ws, st)
+                                   : leaf_backward(x, ldx, w, offsets, dy, lddy, t, groups, din, dout, (__half *)dx, lddx, zero_rest != 0, (__half *)dw, ws, st);
+    if (e.bad()) return fail(errbuf, errlen, e.code, "%s: %s", what, e.what);
     return finish(what, errbuf, errlen);
 }
 
@@ -606,8 +1149,19 @@ int gbm_grad_clip(const void *plan_host, const void *plan_dev, double max_norm, 
 }
 
 int gbm_ops_status(void *stream, char *errbuf, int32_t errlen) {
-    cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    void *flag = nullptr;
+    int late = 0;
+    cudaError_t e = cudaGetSymbolAddress(&flag, tc::g_ops_timeout);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(&late, flag, sizeof late, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess && late) {
+        e = cudaMemsetAsync(flag, 0, sizeof late, st);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    }
     if (e != cudaSuccess) return fail(errbuf, errlen, GBM_ERR_CUDA, "gbm_ops_status: %s", cudaGetErrorString(e));
+    if (late) return fail(errbuf, errlen, GBM_ERR_TIMEOUT, "gbm_ops_status: a wait inside an operator ran out; its outputs are not valid");
     return GBM_OK;
 }
 

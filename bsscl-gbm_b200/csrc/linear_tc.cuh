@@ -1,0 +1,452 @@
+// Matrix products on the fifth-generation tensor cores: one persistent kernel
+// frame for the operators of linear.cu, which differ in how a tile is found
+// (Op::Iter) and in what happens to its sums (Op::epilogue).
+//
+// A cluster of two CTAs works on one 256 x BN tile.  Each CTA keeps 128 rows
+// of A and BN/2 rows of B in shared memory, 64 values of k a stage, fetched
+// by TMA with the 128-byte swizzle; one tcgen05.mma of the pair reads both
+// halves, so each SM fetches half of B: 32 KB a stage at BN = 256, 64 bytes a
+// clock and SM against the 512 clocks of the stage's products.  The sums lie
+// in tensor memory (128 lanes x BN columns in each CTA), twice, so that one
+// tile's epilogue runs under the next one's products.
+//
+// Warp 0 fetches, warp 1 of the leading CTA issues the products, warps 2..9
+// run the epilogue (warp w reads the tensor memory lanes 32 (w % 4) .. +31,
+// warps 2..5 the tile's left columns, warps 6..9 its right ones).
+//
+// Every wait is bounded: when one runs out, the kernel notes it in
+// g_ops_timeout, all roles leave their loops, the copies in flight get time
+// to land, tensor memory is freed and the kernel returns.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace tc {
+
+constexpr int kThreads = 320;
+constexpr int kEpiWarps = 8;
+constexpr int kBK = 64;                       // values of k a stage: 128 bytes
+constexpr int kABytes = 128 * kBK * 2;        // A of one CTA and stage
+constexpr int kStaging = kEpiWarps * 4096;    // 32 rows x 128 bytes a warp
+constexpr long long kWaitClocks = 4000000000ll;   // about 2 s
+
+static __device__ int g_ops_timeout;
+
+template <int BN> struct Shape {
+    static constexpr int kBBytes = BN / 2 * kBK * 2;
+    static constexpr int kStage = kABytes + kBBytes;
+    static constexpr int kStages = (227 * 1024 - kStaging - 2048) / kStage > 8 ? 8 : (227 * 1024 - kStaging - 2048) / kStage;
+    static constexpr int kSmem = kStages * kStage + kStaging + 2048;   // 1024 of alignment, 1024 of barriers and exchange
+};
+
+// ---- shared memory, barriers ------------------------------------------------
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// arrive on the same barrier of the cluster's CTA `rank`
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
+    asm volatile(
+        "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n"
+        " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}" ::"r"(bar), "r"(rank)
+        : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.b32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok;
+}
+// Waits for the phase of this parity; false when the wait ran out here or in another warp of the CTA.
+// Called by whole warps, whose lanes all get the same answer.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead) {
+    bool ok = mbar_try(bar, parity);
+    if (__all_sync(~0u, ok)) return true;
+    const long long t0 = clock64();
+    for (uint32_t i = 1; !ok; i++) {
+        ok = mbar_try(bar, parity);
+        if ((i & 31) == 0 && !ok) {
+            if (*dead) break;
+            if (clock64() - t0 > kWaitClocks) {
+                *dead = 1;
+                g_ops_timeout = 1;
+                break;
+            }
+        }
+    }
+    return __all_sync(~0u, ok);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ---- TMA --------------------------------------------------------------------
+
+// A 3-D tile into this CTA's shared memory, its bytes counted on the leading CTA's barrier.
+__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar & 0xFEFFFFFFu), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+// The same, counted on this CTA's own barrier.
+__device__ __forceinline__ void tma_own(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
+        "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// ---- tcgen05 ----------------------------------------------------------------
+
+// Shared memory descriptor, 128-byte swizzle.  K-major: rows of 128 bytes (64
+// k), groups of 8 rows 1024 bytes apart.  MN-major: rows of 64 values of
+// m (or n), one row a k, groups of 8 k 1024 bytes apart, the next 64 values
+// of m one box of 64 k (8192 bytes) further on.
+template <bool MN> __device__ __forceinline__ uint64_t make_desc(uint32_t addr) {
+    constexpr uint64_t lead = MN ? (8192 >> 4) : 1, stride = 1024 >> 4;
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | lead << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
+}
+// 16 values of k further on, in units of 16 bytes
+template <bool MN> constexpr uint64_t kKStep = MN ? (2048 >> 4) : (32 >> 4);
+
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b),
+        "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+// Arrive on this barrier of both CTAs once all products issued so far are done.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                 : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes: lane l gets row l.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float *v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(addr));
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+// Waits for the loads; ties the registers to it so that none is read before.
+__device__ __forceinline__ void tmem_wait(float *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) asm volatile("" : "+f"(v[i]));
+}
+
+// kind::f16: sums in f32; A and B bf16 (1) or f16 (0); M = 256, N = BN
+inline uint32_t make_idesc(bool bf16, bool a_mn, bool b_mn, int bn) {
+    return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 |
+           (uint32_t)(bn >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
+}
+
+// ---- the frame --------------------------------------------------------------
+
+// One unit of work: C[m0 .. mend) x [n0 .. nend) (256 x BN at most) over
+// nkb stages from k0.  ka/kb_: where the k axis starts in A and B (they
+// differ where B is one piece of a longer axis).  tail: rows of k that count
+// in the last stage where the operands go on behind the k axis' end (0: the
+// maps end there, TMA fills zeros).
+struct Tile {
+    int m0, n0, mend, nend;
+    int am, bn;       // first row of A's m axis and B's n axis in their maps
+    int ka, kb;
+    int nkb;
+    int az, bz;       // batch coordinates
+    int tail;
+    int aux;
+};
+
+// What one epilogue warp knows of its place.
+struct Place {
+    int sub, half, lane, rank;
+    int row;             // row of the tile (0..255) of this lane
+    uint8_t *staging;    // 4096 bytes of this warp's own
+};
+
+template <class Op>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Op op, const uint32_t idesc) {
+    constexpr int BN = Op::kBN;
+    using S = Shape<BN>;
+    constexpr int kCols = 2 * BN < 32 ? 32 : 2 * BN;    // tensor memory columns: a power of two
+    extern __shared__ uint8_t raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *staging = base + S::kStages * S::kStage;
+    uint64_t *bars = (uint64_t *)(staging + kStaging);
+    const uint32_t stages = smem_u32(base);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, tfull = empty + 8 * S::kStages, tempty = tfull + 16,
+                   tailbar = tempty + 16, fixed = tailbar + 8;
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * S::kStages + 6);
+    volatile int *dead = (volatile int *)(tmem_slot + 1);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = cluster_rank();
+    const int cid = blockIdx.x / 2, ncl = gridDim.x / 2;
+
+    if (warp == 0 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+        for (int s = 0; s < S::kStages; s++) {
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(tfull + 8 * s, 1);
+            mbar_init(tempty + 8 * s, 2 * kEpiWarps);
+        }
+        mbar_init(tailbar, 1);
+        mbar_init(fixed, 2);
+        *dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        fence_before();
+    }
+    __syncthreads();
+    cluster_sync();
+    fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+
+    if (warp == 0) {
+        // ---- fetch
+        int s = 0;
+        uint32_t ph = 0, tail_ph = 0;
+        typename Op::Iter it(op, cid, ncl);
+        Tile t;
+        bool ok = true;
+        while (ok && it.next(op, t)) {
+            for (int k = 0; k < t.nkb; k++) {
+                if (!mbar_wait(empty + 8 * s, ph ^ 1, dead)) {
+                    ok = false;
+                    break;
+                }
+                const bool tail = Op::kTail && t.tail && k == t.nkb - 1;
+                const uint32_t a = stages + s * S::kStage, b = a + kABytes;
+                if (lane == 0) {
+                    const uint32_t bar = tail ? tailbar : full + 8 * s;
+                    if (tail) {
+                        mbar_expect(tailbar, S::kStage);
+                        if (rank == 0) mbar_arrive(full + 8 * s);
+                    } else if (rank == 0) {
+                        mbar_expect(full + 8 * s, 2 * S::kStage);
+                    }
+                    auto load = [&](uint32_t dst, const CUtensorMap *m, int x, int y, int z) {
+                        if (tail)
+                            tma_own(dst, m, bar, x, y, z);
+                        else
+                            tma_pair(dst, m, bar, x, y, z);
+                    };
+                    const int am = t.am + (int)rank * 128, ka = t.ka + k * kBK;
+                    if (Op::kAMN) {
+                        load(a, &map_a, am, ka, t.az);
+                        load(a + 8192, &map_a, am + 64, ka, t.az);
+                    } else {
+                        load(a, &map_a, ka, am, t.az);
+                    }
+                    const int bn = t.bn + (int)rank * (BN / 2), kb = t.kb + k * kBK;
+                    if (Op::kBMN) {
+#pragma unroll
+                        for (int j = 0; j < BN / 2; j += 64) load(b + j * 128, &map_b, bn + j, kb, t.bz);
+                    } else {
+                        load(b, &map_b, kb, bn, t.bz);
+                    }
+                }
+                if (tail) {
+                    // rows of k behind the axis' end belong to the next leaf: zeros in their place
+                    if (!mbar_wait(tailbar, tail_ph, dead)) {
+                        ok = false;
+                        break;
+                    }
+                    tail_ph ^= 1;
+                    uint8_t *st = base + s * S::kStage;
+                    for (int box = 0; box < S::kStage / 8192; box++)
+                        for (int i = t.tail * 8 + lane; i < 64 * 8; i += 32) *(uint4 *)(st + box * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_at(fixed, 0);
+                }
+                __syncwarp();
+                if (++s == S::kStages) s = 0, ph ^= 1;
+            }
+        }
+    } else if (warp == 1) {
+        // ---- products
+        if (rank == 0) {
+            int s = 0, n = 0;
+            uint32_t ph = 0, fixed_ph = 0;
+            typename Op::Iter it(op, cid, ncl);
+            Tile t;
+            bool ok = true;
+            while (ok && it.next(op, t)) {
+                const int buf = n & 1;
+                if (!mbar_wait(tempty + 8 * buf, ((n >> 1) & 1) ^ 1, dead)) break;
+                n++;
+                fence_after();
+                const uint32_t d = tmem + buf * BN;
+                for (int k = 0; k < t.nkb; k++) {
+                    if (!mbar_wait(full + 8 * s, ph, dead)) {
+                        ok = false;
+                        break;
+                    }
+                    if (Op::kTail && t.tail && k == t.nkb - 1) {
+                        if (!mbar_wait(fixed, fixed_ph, dead)) {
+                            ok = false;
+                            break;
+                        }
+                        fixed_ph ^= 1;
+                    }
+                    fence_after();
+                    if (lane == 0) {
+                        const uint32_t a = stages + s * S::kStage, b = a + kABytes;
+                        uint64_t da = make_desc<Op::kAMN>(a), db = make_desc<Op::kBMN>(b);
+#pragma unroll
+                        for (int j = 0; j < kBK / 16; j++) {
+                            mma_pair(d, da, db, idesc, k > 0 || j > 0);
+                            da += kKStep<Op::kAMN>;
+                            db += kKStep<Op::kBMN>;
+                        }
+                        commit_pair(empty + 8 * s);
+                    }
+                    __syncwarp();
+                    if (++s == S::kStages) s = 0, ph ^= 1;
+                }
+                if (ok && lane == 0) commit_pair(tfull + 8 * buf);
+                __syncwarp();
+            }
+        }
+    } else {
+        // ---- epilogue
+        Place p;
+        p.sub = warp % 4;
+        p.half = (warp - 2) / 4;
+        p.lane = lane;
+        p.rank = (int)rank;
+        p.row = (int)rank * 128 + p.sub * 32 + lane;
+        p.staging = staging + (warp - 2) * 4096;
+        int n = 0;
+        typename Op::Iter it(op, cid, ncl);
+        Tile t;
+        while (it.next(op, t)) {
+            const int buf = n & 1;
+            if (!mbar_wait(tfull + 8 * buf, (n >> 1) & 1, dead)) break;
+            n++;
+            fence_after();
+            op.epilogue(t, p, tmem + buf * BN + ((uint32_t)(p.sub * 32) << 16) + p.half * (BN / 2), [&] {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(tempty + 8 * buf, 0);
+            });
+        }
+    }
+    __syncwarp();
+    if (*dead)
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);    // copies in flight land meanwhile
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+}
+
+// ---- epilogues --------------------------------------------------------------
+
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+
+// The sums of this warp's 32 rows, COLS columns from `addr` on, through f(v,
+// col) (32 columns at a time, col from the tile's first), rounded to T and
+// stored at out[(row0 + r) * ld + col0 + c] for r < rows, c < cols: 64 columns
+// at a time pass through the warp's staging memory, so that eight lanes store
+// one row's 128 bytes.  vec: rows start on 16-byte boundaries.  release()
+// hands the tensor memory back once it is read.
+template <class T, int COLS, class F, class R>
+__device__ __forceinline__ void store_tile(const Place &p, uint32_t addr, T *out, int64_t ld, int rows, int cols, bool vec, bool zero, F f, R release) {
+    static_assert(COLS % 32 == 0, "");
+    constexpr int kStep = COLS < 64 ? 32 : 64;      // columns a pass
+    constexpr int kChunks = kStep / 8;              // 16-byte pieces of a row
+#pragma unroll 1
+    for (int c = 0; c < COLS; c += kStep) {
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < kStep; h += 32) {
+            float v[32];
+            if (zero) {
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = 0.f;
+            } else {
+                tmem_ld32(addr + c + h, v);
+                tmem_wait(v);
+            }
+            f(v, c + h);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint4 q;
+                q.x = pack2<T>(v[8 * i], v[8 * i + 1]);
+                q.y = pack2<T>(v[8 * i + 2], v[8 * i + 3]);
+                q.z = pack2<T>(v[8 * i + 4], v[8 * i + 5]);
+                q.w = pack2<T>(v[8 * i + 6], v[8 * i + 7]);
+                *(uint4 *)(p.staging + p.lane * 128 + (((h / 8 + i) ^ (p.lane & 7)) * 16)) = q;
+            }
+        }
+        if (c + kStep >= COLS) release();
+        __syncwarp();
+        if (c < cols) {
+#pragma unroll
+            for (int i = 0; i < kChunks; i++) {
+                const int r = i * (32 / kChunks) + p.lane / kChunks, ch = p.lane % kChunks, col = c + ch * 8;
+                const uint4 q = *(const uint4 *)(p.staging + r * 128 + ((ch ^ (r & 7)) * 16));
+                if (r >= rows || col >= cols) continue;
+                T *dst = out + (int64_t)r * ld + col;
+                if (vec && col + 8 <= cols) {
+                    *(uint4 *)dst = q;
+                } else {
+                    const T *e = reinterpret_cast<const T *>(&q);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (col + j < cols) dst[j] = e[j];
+                }
+            }
+        }
+    }
+}
+
+}  // namespace tc

@@ -403,7 +403,7 @@ enum {
  * 32 bits.  lse [n] f32 gets log sum_k exp l_ik, and loss [n] f32 gets
  * lse_i - l_i,target_i.  A row whose target is outside 0..v-1 is ignored: its loss is 0
  * (its lse is still computed).  n >= 0, d and v >= 1, each below 2^31 - 512.
- * ws: gbm_softmax_xent_workspace(n, d, v, 0) bytes, 256-byte aligned. */
+ * ws: gbm_softmax_xent_workspace(n, d, v, 0, in_place) bytes, 256-byte aligned. */
 int gbm_softmax_xent(const void *x, int64_t ldx, const void *w, int64_t ldw, int32_t dtype, int64_t n,
                      int64_t d, int64_t v, const int64_t *target, float *loss, float *lse, void *ws,
                      int64_t ws_bytes, void *stream, char *errbuf, int32_t errlen);
@@ -416,15 +416,17 @@ int gbm_softmax_xent(const void *x, int64_t ldx, const void *w, int64_t ldw, int
  * classes at a time and rounded to `dtype` for the products (to half
  * precision times a power of two that follows the largest |grad_loss|, so
  * that small probabilities keep their bits); the products are summed in 32
- * bits.  ws: gbm_softmax_xent_workspace(n, d, v, 1) bytes, 256-byte aligned. */
+ * bits.  ws: gbm_softmax_xent_workspace(n, d, v, 1, in_place) bytes, 256-byte aligned. */
 int gbm_softmax_xent_grad(const void *x, int64_t ldx, const void *w, int64_t ldw, int32_t dtype, int64_t n,
                           int64_t d, int64_t v, const int64_t *target, const float *lse,
                           const float *grad_loss, void *dx, int64_t lddx, void *dw, int64_t lddw, void *ws,
                           int64_t ws_bytes, void *stream, char *errbuf, int32_t errlen);
 
 /* Workspace of the two calls above in bytes (grad 0: the loss, 1: the
- * gradients); -1 when a size is out of range. */
-int64_t gbm_softmax_xent_workspace(int64_t n, int64_t d, int64_t v, int32_t grad);
+ * gradients); -1 when a size is out of range.  in_place 1: the rows of x and
+ * w all start on 16-byte boundaries (pointers and row strides), so that they are
+ * read where they lie; 0 counts the room for copies that do. */
+int64_t gbm_softmax_xent_workspace(int64_t n, int64_t d, int64_t v, int32_t grad, int32_t in_place);
 
 /* Products grouped by leaf.  The rows of x [t][din] (row stride ldx) lie leaf
  * after leaf: leaf g has the rows offsets[g] .. offsets[g+1]-1 (offsets
@@ -436,7 +438,8 @@ int64_t gbm_softmax_xent_workspace(int64_t n, int64_t d, int64_t v, int32_t grad
  * Offsets that break the rule are clamped into 0..t and a leaf with a
  * negative row count has no rows, so no access leaves the arrays.  t >= 0,
  * groups, din and dout >= 1, groups below 65536, the others below 2^31 - 512.
- * ws: gbm_leaf_linear_workspace(t, groups, din, dout, 0) bytes. */
+ * ws: gbm_leaf_linear_workspace(t, groups, din, dout, 0, in_place) bytes,
+ * 256-byte aligned. */
 int gbm_leaf_linear(const void *x, int64_t ldx, const void *w, const int32_t *offsets, int32_t dtype,
                     int64_t t, int32_t groups, int64_t din, int64_t dout, void *y, int64_t ldy,
                     int32_t zero_rest, void *ws, int64_t ws_bytes, void *stream, char *errbuf,
@@ -446,12 +449,16 @@ int gbm_leaf_linear(const void *x, int64_t ldx, const void *w, const int32_t *of
  * the leaves as zero_rest says) and dw_g = sum over leaf g's rows of
  * dy_r x_r^T [groups][dout][din] contiguous (0 for a leaf without rows).
  * dx or dw may be NULL; w is read for dx only, x for dw only (either may be
- * NULL otherwise).  ws: gbm_leaf_linear_workspace(t, groups, din, dout, 1). */
+ * NULL otherwise).  ws: gbm_leaf_linear_workspace(t, groups, din,
+ * dout, 1, in_place) bytes, 256-byte aligned. */
 int gbm_leaf_linear_grad(const void *x, int64_t ldx, const void *w, const int32_t *offsets, const void *dy,
                          int64_t lddy, int32_t dtype, int64_t t, int32_t groups, int64_t din, int64_t dout,
                          void *dx, int64_t lddx, int32_t zero_rest, void *dw, void *ws, int64_t ws_bytes,
                          void *stream, char *errbuf, int32_t errlen);
-int64_t gbm_leaf_linear_workspace(int64_t t, int32_t groups, int64_t din, int64_t dout, int32_t grad);
+/* Workspace of the two calls above in bytes; -1 when a size is out of range.
+ * in_place 1: the rows of every operand that is read (x, w; dy too for the
+ * gradients) start on 16-byte boundaries. */
+int64_t gbm_leaf_linear_workspace(int64_t t, int32_t groups, int64_t din, int64_t dout, int32_t grad, int32_t in_place);
 
 /* The global 2-norm of many gradients, and clipping.  A plan describes the
  * gradients: src[i] and dst[i] (device addresses, contiguous; dst[i] may be

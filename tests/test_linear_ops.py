@@ -546,7 +546,7 @@ def _rc(f, *a):
 
 
 def test_xent_refusals(L):
-    need = L.gbm_softmax_xent_workspace(10, 16, 20, 0)
+    need = L.gbm_softmax_xent_workspace(10, 16, 20, 0, 1)
     good = [PTR, 16, PTR, 16, BF16, 10, 16, 20, PTR, PTR, PTR, PTR, need]
     for at, value, rc, word in ((0, None, ARG, "null"), (1, 15, ARG, "stride"), (2, None, ARG, "null"), (3, 8, ARG, "stride"),
                                 (4, F32, UNSUPPORTED, "type"), (4, 9, UNSUPPORTED, "type"), (5, -1, ARG, "sizes"), (6, 0, ARG, "sizes"),
@@ -558,7 +558,7 @@ def test_xent_refusals(L):
         got, msg = _rc(L.gbm_softmax_xent, *a)
         assert got == rc and word in msg and "gbm_softmax_xent" in msg, (at, value, got, msg)
     assert _rc(L.gbm_softmax_xent, None, 16, PTR, 16, BF16, 0, 16, 20, None, None, None, PTR, 1 << 30)[0] == OK   # no rows
-    need = L.gbm_softmax_xent_workspace(10, 16, 20, 1)
+    need = L.gbm_softmax_xent_workspace(10, 16, 20, 1, 1)
     good = [PTR, 16, PTR, 16, F16, 10, 16, 20, PTR, PTR, PTR, PTR, 16, PTR, 16, PTR, need]
     for at, value, rc, word in ((9, None, ARG, "null"), (10, None, ARG, "null"), (12, 15, ARG, "stride"), (14, 15, ARG, "stride"),
                                 (11, PTR + 1, ARG, "unaligned"), (16, need - 1, ARG, "workspace"), (4, 1, UNSUPPORTED, "type")):
@@ -569,11 +569,11 @@ def test_xent_refusals(L):
     a = list(good)
     a[11] = a[13] = None
     assert _rc(L.gbm_softmax_xent_grad, *a)[0] == ARG
-    assert L.gbm_softmax_xent_workspace(-1, 1, 1, 0) == -1 and L.gbm_softmax_xent_workspace(1, 1, 1 << 31, 1) == -1
+    assert L.gbm_softmax_xent_workspace(-1, 1, 1, 0, 0) == -1 and L.gbm_softmax_xent_workspace(1, 1, 1 << 31, 1, 1) == -1
 
 
 def test_leaf_refusals(L):
-    need = max(L.gbm_leaf_linear_workspace(10, 3, 16, 24, g) for g in (0, 1))
+    need = max(L.gbm_leaf_linear_workspace(10, 3, 16, 24, g, 0) for g in (0, 1))
     good = [PTR, 16, PTR, PTR, BF16, 10, 3, 16, 24, PTR, 24, 1, PTR, need]
     for at, value, rc in ((0, None, ARG), (1, 15, ARG), (2, None, ARG), (3, None, ARG), (4, F32, UNSUPPORTED), (5, -1, ARG), (6, 0, ARG),
                           (6, 65536, ARG), (7, 0, ARG), (8, 0, ARG), (9, None, ARG), (10, 23, ARG), (9, PTR + 1, ARG), (3, PTR + 2, ARG)):
