@@ -209,7 +209,7 @@ k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensor
     const uint32_t stages = smem_u32(base);
     const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, tfull = empty + 8 * S::kStages, tempty = tfull + 16,
                    tailbar = tempty + 16, fixed = tailbar + 8;
-    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * S::kStages + 6);
+    uint32_t *tmem_slot = (uint32_t *)(bars + 3 * S::kStages + 5);
     volatile int *dead = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cluster_rank();
@@ -221,13 +221,14 @@ k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensor
         for (int s = 0; s < S::kStages; s++) {
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
+            // one a stage: a CTA ahead of the other by a whole short tile must not count for both
+            mbar_init(fixed + 8 * s, 2);
         }
         for (int s = 0; s < 2; s++) {
             mbar_init(tfull + 8 * s, 1);
             mbar_init(tempty + 8 * s, 2 * kEpiWarps);
         }
         mbar_init(tailbar, 1);
-        mbar_init(fixed, 2);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -297,7 +298,7 @@ k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensor
                         for (int i = t.tail * 8 + lane; i < 64 * 8; i += 32) *(uint4 *)(st + box * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_at(fixed, 0);
+                    if (lane == 0) mbar_arrive_at(fixed + 8 * s, 0);
                 }
                 __syncwarp();
                 if (++s == S::kStages) s = 0, ph ^= 1;
@@ -323,11 +324,11 @@ k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensor
                         break;
                     }
                     if (Op::kTail && t.tail && k == t.nkb - 1) {
-                        if (!mbar_wait(fixed, fixed_ph, dead)) {
+                        if (!mbar_wait(fixed + 8 * s, fixed_ph >> s & 1, dead)) {
                             ok = false;
                             break;
                         }
-                        fixed_ph ^= 1;
+                        fixed_ph ^= 1u << s;
                     }
                     fence_after();
                     if (lane == 0) {

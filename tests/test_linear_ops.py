@@ -243,7 +243,8 @@ def _check_leaf(x, w, off, dy, t_rows=None):
     return y, dx, dw
 
 
-LEAF = [([1], 1, 1), ([1], 8, 8), ([0, 3, 0], 30, 20), ([5, 0, 64, 1], 64, 64), ([63, 65, 127, 129], 100, 61),
+# many short leaves: one stage of rows a tile, each with its tail, many tiles a cluster
+LEAF = [([3, 1, 7, 63, 2, 65] * 40, 264, 520), ([1], 1, 1), ([1], 8, 8), ([0, 3, 0], 30, 20), ([5, 0, 64, 1], 64, 64), ([63, 65, 127, 129], 100, 61),
         ([0, 0, 0], 16, 24), ([256, 255, 257, 1, 0, 2], 128, 256), ([700], 264, 136), ([1] * 40, 72, 300),
         ([33, 0, 500, 7], 1000, 50), ([64] * 8, 256, 512), ([3, 1000, 0, 20], 40, 520)]
 
