@@ -1,6 +1,7 @@
 // Device operators for leaf-wise linear models: the softmax cross entropy of
 // a linear head with its gradients, products grouped by leaf with theirs, and
 // the global norm of many gradients with clipping.  See include/gbm_b200.h.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -106,6 +107,7 @@ Err encode(CUtensorMap *map, const View &v, bool bf16, int box) {
 template <class Op> Err launch(const View &a, const View &b, const Op &op, bool bf16, int64_t units, cudaStream_t st) {
     using S = tc::Shape<Op::kBN>;
     if (units <= 0) return {};
+    if (units > INT_MAX - 1024) return {GBM_ERR_ARG, "more than 2^31 tiles"};
     CUtensorMap ma, mb;
     Err e = encode(&ma, a, bf16, Op::kAMN ? 64 : 128);
     if (!e.bad()) e = encode(&mb, b, bf16, Op::kBMN ? 64 : Op::kBN / 2);
@@ -181,33 +183,37 @@ View readable(View v, void *room, cudaStream_t st) {
 // next tile of n, so that the 74 tiles worked on at a time share their
 // operands in L2; `splits` parts of the k axis one behind the other.
 struct Dense {
-    int64_t m, n;      // extents of the result
+    int m, n;          // extents of the result
     int nkb;           // stages of the whole k axis
     int splits;        // parts of the k axis
-    int kb;            // where B's k axis starts
-    __host__ __device__ int64_t mt() const { return (m + 255) / 256; }
-    template <int BN> __host__ __device__ int64_t nt() const { return (n + BN - 1) / BN; }
-    template <int BN> __host__ __device__ int64_t units() const { return mt() * nt<BN>() * splits; }
+    int mt, nt;        // tiles
+    int per;           // stages of a part
+    static constexpr int kBN = 256;
+    Dense(int64_t m_, int64_t n_, int64_t k, int splits_)
+        : m((int)m_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK)), splits(splits_), mt((int)((m_ + 255) / 256)), nt((int)((n_ + kBN - 1) / kBN)),
+          per((nkb + splits_ - 1) / splits_) {}
+    int64_t units() const { return (int64_t)mt * nt * splits; }
 };
 
-template <int BN> struct DenseIter {
-    int64_t at, step;
+// A tile's place is found in 32 bits (64-bit divisions between two tiles held
+// the products up by some 1000 clocks); launch() refuses more units.
+struct DenseIter {
+    uint32_t at, step;
     template <class Op> __device__ DenseIter(const Op &, int cid, int ncl) : at(cid), step(ncl) {}
     template <class Op> __device__ bool next(const Op &op, tc::Tile &t) {
         const Dense &g = op.dense;
-        const int64_t mt = g.mt(), nt = g.nt<BN>(), tiles = mt * nt;
+        const uint32_t tiles = g.mt * g.nt;
         if (at >= tiles * g.splits) return false;
-        const int64_t part = at / tiles, i = at - part * tiles;
-        const int64_t block = i / (8 * nt), rest = i - block * 8 * nt, wide = min((int64_t)8, mt - block * 8);
-        const int64_t tn = rest / wide, tm = block * 8 + (rest - tn * wide);
-        const int per = (g.nkb + g.splits - 1) / g.splits, k0 = min((int)part * per, g.nkb);
+        const uint32_t part = g.splits > 1 ? at / tiles : 0, i = at - part * tiles;
+        const uint32_t band = 8 * g.nt, block = i / band, rest = i - block * band, wide = min(8u, g.mt - block * 8);
+        const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
+        const int k0 = min((int)part * g.per, g.nkb);
         t.m0 = t.am = (int)(tm * 256);
-        t.n0 = t.bn = (int)(tn * BN);
-        t.mend = (int)min(g.m, tm * 256 + 256);
-        t.nend = (int)min(g.n, tn * BN + BN);
-        t.ka = k0 * tc::kBK;
-        t.kb = g.kb + t.ka;
-        t.nkb = min(per, g.nkb - k0);
+        t.n0 = t.bn = (int)(tn * Dense::kBN);
+        t.mend = min(g.m - t.m0, 256) + t.m0;
+        t.nend = min(g.n - t.n0, Dense::kBN) + t.n0;
+        t.ka = t.kb = k0 * tc::kBK;
+        t.nkb = min(g.per, g.nkb - k0);
         t.az = t.bz = 0;
         t.tail = 0;
         t.aux = (int)part;
@@ -242,7 +248,7 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 struct XentStats {
     static constexpr int kBN = 256;
     static constexpr bool kAMN = false, kBMN = false, kTail = false;
-    using Iter = DenseIter<kBN>;
+    using Iter = DenseIter;
     Dense dense;
     const int64_t *target;
     float2 *part;
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(1024) k_xent_scale(const float *__restrict__ g
 template <class T> struct XentG {
     static constexpr int kBN = 256;
     static constexpr bool kAMN = false, kBMN = false, kTail = false;
-    using Iter = DenseIter<kBN>;
+    using Iter = DenseIter;
     Dense dense;
     int64_t c0, v;      // the piece's first class; classes in all
     const int64_t *target;
@@ -386,7 +392,7 @@ template <class T> struct XentG {
 template <class T, bool AMN> struct Product {
     static constexpr int kBN = 256;
     static constexpr bool kAMN = AMN, kBMN = true, kTail = false;
-    using Iter = DenseIter<kBN>;
+    using Iter = DenseIter;
     Dense dense;
     const int64_t *target;     // rows whose target is ignored are 0 (null: none)
     int64_t v;
@@ -570,8 +576,8 @@ Err xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, bool bf
                  float *lse, void *ws, cudaStream_t st) {
     XentLoss q(ws, n, d, v, tma_rows(x, ldx) && tma_rows(w, ldw));
     const View a = readable({x, d, n, ldx}, q.x, st), b = readable({w, d, v, ldw}, q.w, st);
-    XentStats op{{n, v, (int)((d + 63) / 64), 1, 0}, target, q.part, q.ly};
-    Err e = launch(a, b, op, bf16, op.dense.units<256>(), st);
+    XentStats op{Dense(n, v, d, 1), target, q.part, q.ly};
+    Err e = launch(a, b, op, bf16, op.dense.units(), st);
     if (e.bad()) return e;
     k_xent_join<<<(unsigned)((n + 7) / 8), 256, 0, st>>>(q.part, n, (v + 255) / 256 * 2, v, target, q.ly, loss, lse);
     return {};
@@ -597,20 +603,20 @@ Err xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_
         View wp = wv;
         wp.p = (const char *)wv.p + c * wv.ld * 2;
         wp.rows = pc;
-        XentG<T> og{{n, pc, (int)((d + 63) / 64), 1, 0}, c, v, target, lse, grad_loss, scale, g, pl.ldg};
-        Err e = launch(xs, wp, og, bf16, og.dense.template units<256>(), st);
+        XentG<T> og{Dense(n, pc, d, 1), c, v, target, lse, grad_loss, scale, g, pl.ldg};
+        Err e = launch(xs, wp, og, bf16, og.dense.units(), st);
         if (e.bad()) return e;
         const View gv{g, pc, n, pl.ldg};
         if (dx) {
             const bool acc = pl.dx_acc();
-            Product<T, false> op{{n, d, (int)((pc + 63) / 64), pl.sx, 0}, target, v, scale, dx, lddx, tma_rows(dx, lddx), acc ? q.accx : nullptr, pl.ldacc, c > 0};
-            e = launch(gv, wp, op, bf16, op.dense.template units<256>(), st);
+            Product<T, false> op{Dense(n, d, pc, pl.sx), target, v, scale, dx, lddx, tma_rows(dx, lddx), acc ? q.accx : nullptr, pl.ldacc, c > 0};
+            e = launch(gv, wp, op, bf16, op.dense.units(), st);
             if (e.bad()) return e;
         }
         if (dw) {
             T *o = dw + c * lddw;
-            Product<T, true> op{{pc, d, (int)((n + 63) / 64), pl.sw, 0}, nullptr, 0, scale, o, lddw, tma_rows(o, lddw), pl.sw > 1 ? q.accw : nullptr, pl.ldacc, false};
-            e = launch(gv, xs, op, bf16, op.dense.template units<256>(), st);
+            Product<T, true> op{Dense(pc, d, n, pl.sw), nullptr, 0, scale, o, lddw, tma_rows(o, lddw), pl.sw > 1 ? q.accw : nullptr, pl.ldacc, false};
+            e = launch(gv, xs, op, bf16, op.dense.units(), st);
             if (!e.bad() && pl.sw > 1) e = sum_splits<T>(q.accw, pl.ldacc, pc, d, pl.sw, scale, nullptr, 0, o, lddw, st);
             if (e.bad()) return e;
         }
@@ -633,28 +639,28 @@ struct Leaves {
     const int32_t *off;
     int64_t t;
     int32_t groups;
-    int64_t n;          // columns of the result
-    int nkb;
+    int n;              // columns of the result
+    int nkb, nt;
+    Leaves(const int32_t *off_, int64_t t_, int32_t groups_, int64_t k, int64_t n_)
+        : off(off_), t(t_), groups(groups_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK)), nt((int)((n_ + 255) / 256)) {}
+    // tiles at most: each leaf may end in a part of one
+    int64_t units() const { return ((t + 255) / 256 + groups) * nt; }
 };
 
-// The 256 x BN tiles of all leaves' rows, leaf after leaf.  A warp looks
-// through 32 leaves at a time: each lane counts one leaf's row tiles.
-template <int BN> struct LeafIter {
-    int64_t at, step, base, total, upto;    // tiles before these 32 leaves, in them, in them up to this lane's
+// The 256 x 256 tiles of all leaves' rows, leaf after leaf.  A warp looks
+// through 32 leaves at a time: each lane counts one leaf's tiles.
+struct LeafIter {
+    uint32_t at, step, base, total, upto;    // tiles before these 32 leaves, in them, in them up to this lane's
     int first, lo, hi;
-    int64_t nt;
-    template <class Op> __device__ LeafIter(const Op &op, int cid, int ncl) : at(cid), step(ncl), base(0), first(0) {
-        nt = (op.leaves.n + BN - 1) / BN;
-        look(op);
-    }
+    template <class Op> __device__ LeafIter(const Op &op, int cid, int ncl) : at(cid), step(ncl), base(0), first(0) { look(op); }
     template <class Op> __device__ void look(const Op &op) {
         const int lane = threadIdx.x % 32, g = first + lane;
         lo = hi = 0;
         if (g < op.leaves.groups) leaf_rows(op.leaves.off, g, op.leaves.t, lo, hi);
-        upto = (int64_t)((hi - lo + 255) / 256) * nt;
+        upto = (uint32_t)((hi - lo + 255) / 256) * op.leaves.nt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(~0u, upto, o);
+            const uint32_t u = __shfl_up_sync(~0u, upto, o);
             if (lane >= o) upto += u;
         }
         total = __shfl_sync(~0u, upto, 31);
@@ -666,17 +672,17 @@ template <int BN> struct LeafIter {
             if (first >= op.leaves.groups) return false;
             look(op);
         }
-        const int64_t rel = at - base;
+        const uint32_t rel = at - base, nt = op.leaves.nt;
         const int l = __ffs(__ballot_sync(~0u, upto > rel)) - 1;
         const int a = __shfl_sync(~0u, lo, l), b = __shfl_sync(~0u, hi, l);
-        const int64_t end = __shfl_sync(~0u, upto, l), rt = (b - a + 255) / 256, i = rel - (end - rt * nt);
+        const uint32_t end = __shfl_sync(~0u, upto, l), rt = (b - a + 255) / 256, i = rel - (end - rt * nt);
         // 8 row tiles beside one another, as in Dense
-        const int64_t block = i / (8 * nt), rest = i - block * 8 * nt, wide = min((int64_t)8, rt - block * 8);
-        const int64_t tn = rest / wide, tm = block * 8 + (rest - tn * wide);
+        const uint32_t band = 8 * nt, block = i / band, rest = i - block * band, wide = min(8u, rt - block * 8);
+        const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
         t.m0 = t.am = a + (int)tm * 256;
-        t.n0 = t.bn = (int)(tn * BN);
-        t.mend = min(b, t.m0 + 256);
-        t.nend = (int)min(op.leaves.n, tn * BN + BN);
+        t.n0 = t.bn = (int)(tn * 256);
+        t.mend = min(b - t.m0, 256) + t.m0;
+        t.nend = min(op.leaves.n - t.n0, 256) + t.n0;
         t.ka = t.kb = 0;
         t.nkb = op.leaves.nkb;
         t.az = 0;
@@ -694,7 +700,7 @@ template <int BN> struct LeafIter {
 template <class T, bool BMN> struct LeafRows {
     static constexpr int kBN = 256;
     static constexpr bool kAMN = false, kBMN = BMN, kTail = false;
-    using Iter = LeafIter<kBN>;
+    using Iter = LeafIter;
     Leaves leaves;
     T *out;
     int64_t ld;
@@ -708,26 +714,26 @@ template <class T, bool BMN> struct LeafRows {
 // dw: one 256 x 256 tile of one leaf (and one part of its rows) a unit; the k
 // axis is the leaf's rows.
 struct LeafDwIter {
-    int64_t at, step;
+    uint32_t at, step;
     template <class Op> __device__ LeafDwIter(const Op &, int cid, int ncl) : at(cid), step(ncl) {}
     template <class Op> __device__ bool next(const Op &op, tc::Tile &t) {
-        const int64_t mt = (op.dout + 255) / 256, nt = (op.din + 255) / 256, per = mt * nt * op.splits;
+        const uint32_t tiles = op.mt * op.nt, per = tiles * op.splits;
         if (at >= per * op.groups) return false;
-        const int g = (int)(at / per), i = (int)(at - g * per), part = (int)(i / (mt * nt)), tile = (int)(i - part * (mt * nt));
-        const int tm = (int)(tile / nt), tn = (int)(tile - tm * nt);
+        const uint32_t g = at / per, i = at - g * per, part = op.splits > 1 ? i / tiles : 0, tile = i - part * tiles, tm = tile / op.nt, tn = tile - tm * op.nt;
         int lo, hi;
         leaf_rows(op.off, g, op.t, lo, hi);
-        const int nkb = (hi - lo + 63) / 64, each = (nkb + op.splits - 1) / op.splits, k0 = min(part * each, nkb), k1 = min(k0 + each, nkb);
-        t.m0 = t.am = tm * 256;
-        t.n0 = t.bn = tn * 256;
-        t.mend = (int)min(op.dout, (int64_t)t.m0 + 256);
-        t.nend = (int)min(op.din, (int64_t)t.n0 + 256);
+        const int nkb = (hi - lo + 63) / 64, each = op.splits > 1 ? (nkb + op.splits - 1) / op.splits : nkb, k0 = min((int)part * each, nkb),
+                  k1 = min(k0 + each, nkb);
+        t.m0 = t.am = (int)tm * 256;
+        t.n0 = t.bn = (int)tn * 256;
+        t.mend = min((int)op.dout - t.m0, 256) + t.m0;
+        t.nend = min((int)op.din - t.n0, 256) + t.n0;
         t.ka = t.kb = lo + k0 * 64;
         t.nkb = k1 - k0;
         t.az = t.bz = 0;
         // behind the last row of all TMA fills zeros
         t.tail = k1 == nkb && hi < op.t ? (hi - lo) % 64 : 0;
-        t.aux = part * op.groups + g;
+        t.aux = (int)(part * op.groups + g);
         at += step;
         return true;
     }
@@ -740,7 +746,7 @@ template <class T> struct LeafDw {
     const int32_t *off;
     int64_t t, din, dout;
     int32_t groups;
-    int splits;
+    int splits, mt, nt;
     T *out;
     bool vec;
     float *acc;         // [split][groups * dout][ldacc] where there are several
@@ -803,15 +809,12 @@ struct LeafWs {
     }
 };
 
-// Tiles of a grouped product at most: each leaf may end in a part of one.
-int64_t leaf_units(int64_t t, int32_t groups, int64_t n) { return ((t + 255) / 256 + groups) * ((n + 255) / 256); }
-
 template <class T, bool BMN>
 Err leaf_rows_launch(const View &a, const View &w, const int32_t *off, int64_t t, int32_t groups, int64_t k, int64_t n, T *y, int64_t ldy, bool zero_rest,
                      cudaStream_t st) {
     constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    LeafRows<T, BMN> op{{off, t, groups, n, (int)((k + 63) / 64)}, y, ldy, tma_rows(y, ldy)};
-    Err e = launch(a, w, op, bf16, leaf_units(t, groups, n), st);
+    LeafRows<T, BMN> op{Leaves(off, t, groups, k, n), y, ldy, tma_rows(y, ldy)};
+    Err e = launch(a, w, op, bf16, op.leaves.units(), st);
     if (!e.bad() && zero_rest) k_leaf_rest<T><<<(unsigned)std::min<int64_t>(t, sm_count()), 256, 0, st>>>(off, groups, t, n, y, ldy);
     return e;
 }
@@ -843,8 +846,9 @@ Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off,
     if (!dw) return {};
     const View a = readable({x, din, t, ldx}, q.x, st);
     const int s = leaf_splits(t, groups, din, dout);
-    LeafDw<T> op{off, t, din, dout, groups, s, dw, tma_rows(dw, din), s > 1 ? q.acc : nullptr, q.ldacc};
-    Err e = launch(g, a, op, bf16, (int64_t)groups * s * ((din + 255) / 256) * ((dout + 255) / 256), st);
+    const int mt = (int)((dout + 255) / 256), nt = (int)((din + 255) / 256);
+    LeafDw<T> op{off, t, din, dout, groups, s, mt, nt, dw, tma_rows(dw, din), s > 1 ? q.acc : nullptr, q.ldacc};
+    Err e = launch(g, a, op, bf16, (int64_t)groups * s * mt * nt, st);
     if (!e.bad() && s > 1) e = sum_splits<T>(q.acc, q.ldacc, groups * dout, din, s, nullptr, nullptr, 0, dw, din, st);
     return e;
 }
@@ -853,8 +857,12 @@ Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off,
 // norm and clipping
 // ---------------------------------------------------------------------------
 
+// One cooperative launch: every block sums the squares of its items, the grid
+// meets once, every block adds up all blocks' sums in the same order and
+// scales its items, the last one first, while L2 still holds them.  Bound by
+// memory: two reads and a write of what L2 does not keep.
 constexpr uint64_t kClipMagic = 0x47424d434c495031ull;
-constexpr int64_t kClipChunk = 1 << 16;   // elements of one work item
+constexpr int kClipBlocks = 4;     // blocks of 256 threads an SM
 
 struct ClipItem {
     const void *src;
@@ -868,62 +876,131 @@ struct ClipPlan {
     // ClipItem[items] follow
 };
 
-template <class T> __device__ double sum_sq(const T *p, int n) {
-    double s = 0;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        double v = to_f(p[i]);
-        s += v * v;
+// Elements of one item: some 16 items a block where there is that much, so
+// that the blocks' shares differ little, within 2048 .. 16384 (a thread's 8
+// and 64 elements).
+int64_t clip_chunk(int64_t total) { return std::min<int64_t>(16384, std::max<int64_t>(2048, round_up(total / (148 * kClipBlocks * 16), 2048))); }
+
+template <class T> __device__ __forceinline__ void square_add(uint4 q, double *s) {
+    const T *e = reinterpret_cast<const T *>(&q);
+#pragma unroll
+    for (int k = 0; k < (int)(16 / sizeof(T)); k++) {
+        const double v = to_f(e[k]);
+        s[k & 3] = fma(v, v, s[k & 3]);
     }
+}
+
+// elements before the first 16-byte boundary
+template <class T> __device__ __forceinline__ int head_of(const T *p, int n) {
+    return min(n, (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T));
+}
+
+template <class T> __device__ void sum_sq(const T *p, int n, double *s) {
+    constexpr int kVec = 16 / sizeof(T);
+    const int head = head_of(p, n), nv = (n - head) / kVec, tid = threadIdx.x;
+    if (tid < head) {
+        const double v = to_f(p[tid]);
+        s[0] = fma(v, v, s[0]);
+    }
+    const int rest = head + nv * kVec + tid;
+    if (rest < n) {
+        const double v = to_f(p[rest]);
+        s[1] = fma(v, v, s[1]);
+    }
+    const uint4 *q = (const uint4 *)(p + head);
+    int i = tid;
+    for (; i + 768 < nv; i += 1024) {
+        uint4 a[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) a[k] = __ldg(q + i + 256 * k);
+#pragma unroll
+        for (int k = 0; k < 4; k++) square_add<T>(a[k], s);
+    }
+    for (; i < nv; i += 256) square_add<T>(__ldg(q + i), s);
+}
+
+template <class T> __device__ __forceinline__ uint4 scaled(uint4 q, float c) {
+    T *e = reinterpret_cast<T *>(&q);
+#pragma unroll
+    for (int k = 0; k < (int)(16 / sizeof(T)); k++) e[k] = from_f<T>(to_f(e[k]) * c);
+    return q;
+}
+
+// p and q may be the same: no load goes through the read-only path here
+template <class T> __device__ void scale_to(const T *p, T *q, int n, float c) {
+    constexpr int kVec = 16 / sizeof(T);
+    const int tid = threadIdx.x;
+    if ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15) {
+#pragma unroll 8
+        for (int i = tid; i < n; i += 256) q[i] = from_f<T>(to_f(p[i]) * c);
+        return;
+    }
+    const int head = head_of(p, n), nv = (n - head) / kVec;
+    if (tid < head) q[tid] = from_f<T>(to_f(p[tid]) * c);
+    const int rest = head + nv * kVec + tid;
+    if (rest < n) q[rest] = from_f<T>(to_f(p[rest]) * c);
+    const uint4 *a = (const uint4 *)(p + head);
+    uint4 *b = (uint4 *)(q + head);
+    int i = tid;
+    for (; i + 768 < nv; i += 1024) {
+        uint4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = a[i + 256 * k];
+#pragma unroll
+        for (int k = 0; k < 4; k++) __stcs(b + i + 256 * k, scaled<T>(v[k], c));
+    }
+    for (; i < nv; i += 256) __stcs(b + i, scaled<T>(a[i], c));
+}
+
+// The same in every lane.
+__device__ __forceinline__ double warp_sum(double s) {
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     return s;
 }
 
-__global__ void __launch_bounds__(256) k_clip_norm(const ClipItem *items, double *part) {
-    ClipItem it = items[blockIdx.x];
-    double s = it.dtype == GBM_TYPE_F32    ? sum_sq((const float *)it.src, it.n)
-               : it.dtype == GBM_TYPE_BF16 ? sum_sq((const __nv_bfloat16 *)it.src, it.n)
-                                           : sum_sq((const __half *)it.src, it.n);
+__global__ void __launch_bounds__(256, kClipBlocks) k_clip(const ClipItem *__restrict__ items, int64_t n_items, double max_norm, float *norm, double *part) {
     __shared__ double red[8];
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = s;
+    double s[4] = {0, 0, 0, 0};
+    for (int64_t i = blockIdx.x; i < n_items; i += gridDim.x) {
+        const ClipItem it = items[i];
+        if (it.dtype == GBM_TYPE_F32)
+            sum_sq((const float *)it.src, it.n, s);
+        else if (it.dtype == GBM_TYPE_BF16)
+            sum_sq((const __nv_bfloat16 *)it.src, it.n, s);
+        else
+            sum_sq((const __half *)it.src, it.n, s);
+    }
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const double w = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
+    if (lane == 0) red[warp] = w;
     __syncthreads();
     if (threadIdx.x == 0) {
-        s = 0;
-        for (int k = 0; k < 8; k++) s += red[k];
-        part[blockIdx.x] = s;
+        double b = 0;
+        for (int k = 0; k < 8; k++) b += red[k];
+        part[blockIdx.x] = b;
     }
-}
-
-__global__ void __launch_bounds__(1024) k_clip_sum(const double *part, int64_t items, double max_norm, float *norm,
-                                                   float *scale) {
-    __shared__ double red[1024];
-    double s = 0;
-    for (int64_t i = threadIdx.x; i < items; i += 1024) s += part[i];
-    red[threadIdx.x] = s;
+    cooperative_groups::this_grid().sync();
+    double t = 0;
+    for (int k = threadIdx.x; k < (int)gridDim.x; k += 256) t += __ldcg(part + k);
+    t = warp_sum(t);
+    if (lane == 0) red[warp] = t;
     __syncthreads();
-    for (int o = 512; o; o >>= 1) {
-        if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-        __syncthreads();
+    t = 0;
+    for (int k = 0; k < 8; k++) t += red[k];
+    const double r = sqrt(t), f = max_norm / (r + 1e-6);
+    const float c = (float)(f > 1.0 ? 1.0 : f);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)r;
+    const int64_t mine = n_items > blockIdx.x ? (n_items - 1 - blockIdx.x) / gridDim.x : -1;
+    for (int64_t k = mine; k >= 0; k--) {
+        const ClipItem it = items[blockIdx.x + k * gridDim.x];
+        if (c == 1.f && it.src == it.dst) continue;
+        if (it.dtype == GBM_TYPE_F32)
+            scale_to((const float *)it.src, (float *)it.dst, it.n, c);
+        else if (it.dtype == GBM_TYPE_BF16)
+            scale_to((const __nv_bfloat16 *)it.src, (__nv_bfloat16 *)it.dst, it.n, c);
+        else
+            scale_to((const __half *)it.src, (__half *)it.dst, it.n, c);
     }
-    if (threadIdx.x == 0) {
-        double r = sqrt(red[0]), c = max_norm / (r + 1e-6);
-        *norm = (float)r;
-        *scale = (float)(c > 1.0 ? 1.0 : c);
-    }
-}
-
-template <class T> __device__ void scale_to(const T *p, T *q, int n, float c) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) q[i] = from_f<T>(to_f(p[i]) * c);
-}
-
-__global__ void __launch_bounds__(256) k_clip_scale(const ClipItem *items, const float *scale) {
-    ClipItem it = items[blockIdx.x];
-    const float c = *scale;
-    if (it.dtype == GBM_TYPE_F32)
-        scale_to((const float *)it.src, (float *)it.dst, it.n, c);
-    else if (it.dtype == GBM_TYPE_BF16)
-        scale_to((const __nv_bfloat16 *)it.src, (__nv_bfloat16 *)it.dst, it.n, c);
-    else
-        scale_to((const __half *)it.src, (__half *)it.dst, it.n, c);
 }
 
 int finish(const char *what, char *errbuf, int32_t errlen) {
@@ -1063,12 +1140,14 @@ int gbm_leaf_linear_grad(const void *x, int64_t ldx, const void *w, const int32_
 
 int64_t gbm_grad_clip_plan_bytes(const int64_t *sizes, int32_t n) {
     if (n < 0 || (n && !sizes)) return -1;
-    int64_t items = 0;
+    int64_t total = 0, items = 0;
     for (int32_t i = 0; i < n; i++) {
-        if (sizes[i] < 0 || sizes[i] > (1LL << 46)) return -1;
-        items += (sizes[i] + kClipChunk - 1) / kClipChunk;
-        if (items > INT32_MAX) return -1;
+        if (sizes[i] < 0 || sizes[i] > (1LL << 40)) return -1;
+        total += sizes[i];
+        if (total > (1LL << 40)) return -1;
     }
+    const int64_t chunk = clip_chunk(total);
+    for (int32_t i = 0; i < n; i++) items += (sizes[i] + chunk - 1) / chunk;
     return (int64_t)sizeof(ClipPlan) + items * (int64_t)sizeof(ClipItem);
 }
 
@@ -1114,11 +1193,14 @@ int gbm_grad_clip_plan(const void *const *src, void *const *dst, const int64_t *
     ClipItem *it = reinterpret_cast<ClipItem *>(plan + 1);
     plan->magic = kClipMagic;
     plan->items = 0;
+    int64_t total = 0;
+    for (int32_t i = 0; i < n; i++) total += sizes[i];
+    const int64_t chunk = clip_chunk(total);
     for (int32_t i = 0; i < n; i++) {
         const int b = type_size(dtypes[i]);
-        for (int64_t at = 0; at < sizes[i]; at += kClipChunk)
+        for (int64_t at = 0; at < sizes[i]; at += chunk)
             it[plan->items++] = {(const char *)src[i] + at * b, (char *)dst[i] + at * b,
-                                 (int32_t)std::min(kClipChunk, sizes[i] - at), dtypes[i]};
+                                 (int32_t)std::min(chunk, sizes[i] - at), dtypes[i]};
     }
     return GBM_OK;
 }
@@ -1126,7 +1208,7 @@ int gbm_grad_clip_plan(const void *const *src, void *const *dst, const int64_t *
 int64_t gbm_grad_clip_workspace(const void *plan_host) {
     const ClipPlan *plan = static_cast<const ClipPlan *>(plan_host);
     if (!plan || plan->magic != kClipMagic) return -1;
-    return 16 + plan->items * 8;
+    return std::max<int64_t>(1, std::min<int64_t>(plan->items, 512LL * kClipBlocks)) * 8;
 }
 
 int gbm_grad_clip(const void *plan_host, const void *plan_dev, double max_norm, float *norm, void *ws,
@@ -1137,15 +1219,15 @@ int gbm_grad_clip(const void *plan_host, const void *plan_dev, double max_norm, 
     if (!plan_dev || !norm || !ws || ws_bytes < need || !aligned(ws, 16) || !aligned(plan_dev, 16) || !aligned(norm, 4))
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: null or unaligned pointer, or a workspace below %lld bytes", what, (long long)need);
     if (!(max_norm >= 0)) return fail(errbuf, errlen, GBM_ERR_ARG, "%s: max_norm %g", what, max_norm);
-    const int64_t items = static_cast<const ClipPlan *>(plan_host)->items;
+    int64_t items = static_cast<const ClipPlan *>(plan_host)->items;
     const ClipItem *it = reinterpret_cast<const ClipItem *>(static_cast<const ClipPlan *>(plan_dev) + 1);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    float *scale = static_cast<float *>(ws);
-    double *part = reinterpret_cast<double *>(static_cast<char *>(ws) + 16);
-    if (items) k_clip_norm<<<(unsigned)items, 256, 0, st>>>(it, part);
-    k_clip_sum<<<1, 1024, 0, st>>>(part, items, max_norm, norm, scale);
-    if (items) k_clip_scale<<<(unsigned)items, 256, 0, st>>>(it, scale);
-    return finish(what, errbuf, errlen);
+    double *part = static_cast<double *>(ws);
+    // all blocks are on the device at once
+    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(items, std::min(sm_count(), 512) * kClipBlocks));
+    void *args[] = {&it, &items, &max_norm, &norm, &part};
+    cudaError_t e = cudaLaunchCooperativeKernel((const void *)k_clip, dim3((unsigned)blocks), dim3(256), args, 0, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return fail(errbuf, errlen, GBM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    return GBM_OK;
 }
 
 int gbm_ops_status(void *stream, char *errbuf, int32_t errlen) {
