@@ -103,15 +103,36 @@ Err encode(CUtensorMap *map, const View &v, bool bf16, int box) {
     return {};
 }
 
-// One launch of the frame: `units` tiles at most, a cluster of two CTAs for each, at most one CTA an SM.
-template <class Op> Err launch(const View &a, const View &b, const Op &op, bool bf16, int64_t units, cudaStream_t st) {
+// A kernel whose set-up may overlap the end of the launch in front of it: each
+// of this file's kernels waits for that one itself (tc::depend).
+template <class... P, class... A> Err start(void (*kernel)(P...), int64_t blocks, int threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaError_t c = cudaLaunchKernelEx(&cfg, kernel, P(args)...); c != cudaSuccess) return {GBM_ERR_CUDA, cudaGetErrorString(c)};
+    return {};
+}
+
+// One launch of the frame: `units` tiles at most, a cluster of two CTAs for
+// each, at most one CTA an SM.  views: A and B, for a launch of two products
+// twice.
+template <class Op> Err launch(const View *views, const Op &op, bool bf16, int64_t units, cudaStream_t st) {
     using S = tc::Shape<Op::kBN>;
     if (units <= 0) return {};
     if (units > INT_MAX - 1024) return {GBM_ERR_ARG, "more than 2^31 tiles"};
-    CUtensorMap ma, mb;
-    Err e = encode(&ma, a, bf16, Op::kAMN ? 64 : 128);
-    if (!e.bad()) e = encode(&mb, b, bf16, Op::kBMN ? 64 : Op::kBN / 2);
-    if (e.bad()) return e;
+    tc::Maps maps;
+    for (int i = 0; i < (Op::kDual ? 4 : 2); i++) {
+        const bool mn = i & 1 ? Op::kBMN : Op::kDual ? i == 2 : Op::kAMN;
+        Err e = encode(&maps.m[i], views[i], bf16, mn ? 64 : i & 1 ? Op::kBN / 2 : 128);
+        if (e.bad()) return e;
+    }
     static std::atomic<uint64_t> ready;     // devices whose limit for this kernel is set
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return {GBM_ERR_CUDA, "no current CUDA device"};
@@ -123,9 +144,7 @@ template <class Op> Err launch(const View &a, const View &b, const Op &op, bool 
     }
     const int64_t clusters = std::min<int64_t>(units, sm_count() / 2);
     if (clusters < 1) return {GBM_ERR_CUDA, "no SMs"};
-    tc::k_tc<Op><<<(unsigned)(2 * clusters), tc::kThreads, S::kSmem, st>>>(ma, mb, op, tc::make_idesc(bf16, Op::kAMN, Op::kBMN, Op::kBN));
-    if (cudaError_t c = cudaGetLastError(); c != cudaSuccess) return {GBM_ERR_CUDA, cudaGetErrorString(c)};
-    return {};
+    return start(tc::k_tc<Op>, 2 * clusters, tc::kThreads, S::kSmem, st, maps, op, tc::make_idesc(bf16, Op::kBMN, Op::kBN));
 }
 
 // Whether TMA can read the rows in place: 16-byte boundaries.
@@ -133,43 +152,101 @@ bool tma_rows(const void *p, int64_t ld) { return aligned(p, 16) && ld % 8 == 0;
 
 // Rows of 16-bit values to rows on 16-byte boundaries, zeros behind the last
 // column; a row whose target is ignored becomes zeros where `target` is given.
-__global__ void __launch_bounds__(256) k_pack(const uint16_t *__restrict__ src, int64_t ld, int64_t rows, int64_t cols, uint16_t *__restrict__ dst,
-                                              int64_t ldp, bool vec, const int64_t *__restrict__ target, int64_t v) {
-    const int64_t per = ldp / 8, total = rows * per;
-    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-        const int64_t r = i / per, c = (i - r * per) * 8;
-        uint4 q = make_uint4(0, 0, 0, 0);
-        bool has = true;
-        if (target) {
-            const int64_t y = target[r];
-            has = y >= 0 && y < v;
+struct PackJob {
+    const uint16_t *src;
+    int64_t ld, rows, cols;
+    uint16_t *dst;
+    int64_t ldp;
+    bool vec;
+    const int64_t *target;
+    int64_t v;
+    int64_t chunks() const { return rows * (ldp / 8); }
+};
+
+// What a call's other launches need first: copies of operands, tickets set to
+// 0, and the power of two that takes the largest |grad_loss| of the rows that
+// count to at most 2^14, half precision's range (scale[0], its inverse in
+// scale[1]; by the last block).
+struct Prep {
+    PackJob job[3];
+    int jobs = 0;
+    uint32_t *tickets = nullptr;
+    int n_tickets = 0;
+    const float *grad_loss = nullptr;
+    const int64_t *target = nullptr;
+    int64_t n = 0, v = 0;
+    float *scale = nullptr;
+};
+
+__global__ void __launch_bounds__(256) k_prep(const __grid_constant__ Prep p) {
+    tc::depend();
+    const int work = gridDim.x - (p.scale ? 1 : 0);
+    if ((int)blockIdx.x == work) {
+        __shared__ float red[8];
+        float m = 0.f;
+#pragma unroll 8
+        for (int64_t i = threadIdx.x; i < p.n; i += 256) {
+            const int64_t y = p.target[i];
+            m = fmaxf(m, y >= 0 && y < p.v ? fabsf(p.grad_loss[i]) : 0.f);
         }
-        if (has) {
-            const uint16_t *p = src + r * ld + c;
-            if (vec && c + 8 <= cols) {
-                q = *(const uint4 *)p;
-            } else {
-                uint32_t h[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) h[j] = c + j < cols ? p[j] : 0;
-                q = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
+        __syncthreads();
+        if (threadIdx.x) return;
+        for (int k = 1; k < 8; k++) m = fmaxf(m, red[k]);
+        int e = 0;
+        if (m > 0.f && m < INFINITY) e = min(max(14 - (ilogbf(m) + 1), -100), 100);
+        p.scale[0] = ldexpf(1.f, e);
+        p.scale[1] = ldexpf(1.f, -e);
+        return;
+    }
+    const int64_t first = blockIdx.x * 256LL + threadIdx.x, step = work * 256LL;
+    for (int64_t i = first; i < p.n_tickets; i += step) p.tickets[i] = 0;
+    for (int k = 0; k < p.jobs; k++) {
+        const PackJob &j = p.job[k];
+        const int64_t per = j.ldp / 8, total = j.rows * per;
+        for (int64_t i = first; i < total; i += step) {
+            // 32 bits where they do: a 64-bit division costs more than the copy
+            const int64_t r = total >> 31 ? i / per : (int64_t)((uint32_t)i / (uint32_t)per), c = (i - r * per) * 8;
+            uint4 q = make_uint4(0, 0, 0, 0);
+            bool has = true;
+            if (j.target) {
+                const int64_t y = j.target[r];
+                has = y >= 0 && y < j.v;
             }
+            if (has) {
+                const uint16_t *s = j.src + r * j.ld + c;
+                if (j.vec && c + 8 <= j.cols) {
+                    q = *(const uint4 *)s;
+                } else {
+                    uint32_t h[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) h[e] = c + e < j.cols ? s[e] : 0;
+                    q = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                }
+            }
+            *(uint4 *)(j.dst + r * j.ldp + c) = q;
         }
-        *(uint4 *)(dst + r * ldp + c) = q;
     }
 }
 
-void pack(const void *src, int64_t ld, int64_t rows, int64_t cols, void *dst, int64_t ldp, const int64_t *target, int64_t v, cudaStream_t st) {
-    const int64_t blocks = std::min<int64_t>((rows * (ldp / 8) + 255) / 256, sm_count() * 16LL);
-    if (blocks > 0)
-        k_pack<<<(unsigned)blocks, 256, 0, st>>>((const uint16_t *)src, ld, rows, cols, (uint16_t *)dst, ldp, tma_rows(src, ld), target, v);
+Err run_prep(const Prep &p, cudaStream_t st) {
+    int64_t most = p.n_tickets / 4;
+    for (int k = 0; k < p.jobs; k++) most = std::max(most, p.job[k].chunks());
+    if (!p.jobs && !p.n_tickets && !p.scale) return {};
+    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((most + 255) / 256, sm_count() * 8LL));
+    return start(k_prep, blocks + (p.scale ? 1 : 0), 256, 0, st, p);
 }
 
-// `v` itself, or its packed copy at `room`.
-View readable(View v, void *room, cudaStream_t st) {
+void add_pack(Prep &p, const View &v, void *room, int64_t ldp, const int64_t *target, int64_t classes) {
+    p.job[p.jobs++] = {(const uint16_t *)v.p, v.ld, v.rows * v.batch, v.inner, (uint16_t *)room, ldp, tma_rows(v.p, v.ld), target, classes};
+}
+
+// `v` itself, or its copy at `room`, which the prep makes.
+View readable(Prep &p, View v, void *room) {
     if (tma_rows(v.p, v.ld)) return v;
     const int64_t ldp = round_up(v.inner, 8);
-    pack(v.p, v.ld, v.rows * v.batch, v.inner, room, ldp, nullptr, 0, st);
+    add_pack(p, v, room, ldp, nullptr, 0);
     v.p = room;
     v.ld = ldp;
     return v;
@@ -188,35 +265,38 @@ struct Dense {
     int splits;        // parts of the k axis
     int mt, nt;        // tiles
     int per;           // stages of a part
-    static constexpr int kBN = 256;
-    Dense(int64_t m_, int64_t n_, int64_t k, int splits_)
-        : m((int)m_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK)), splits(splits_), mt((int)((m_ + 255) / 256)), nt((int)((n_ + kBN - 1) / kBN)),
+    Dense() : m(0), n(0), nkb(0), splits(1), mt(0), nt(0), per(0) {}
+    Dense(int64_t m_, int64_t n_, int64_t k, int bn, int splits_ = 1, int laps = 1)
+        : m((int)m_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK) * laps), splits(splits_), mt((int)((m_ + 255) / 256)), nt((int)((n_ + bn - 1) / bn)),
           per((nkb + splits_ - 1) / splits_) {}
-    int64_t units() const { return (int64_t)mt * nt * splits; }
+    int64_t tiles() const { return (int64_t)mt * nt; }
+    int64_t units() const { return tiles() * splits; }
+    // A tile's place is found in 32 bits (64-bit divisions between two tiles
+    // held the products up by some 1000 clocks); launch() refuses more units.
+    template <int BN> __device__ void place(uint32_t at, tc::Tile &t) const {
+        const uint32_t all = mt * nt, part = splits > 1 ? at / all : 0, i = at - part * all;
+        const uint32_t band = 8 * nt, block = i / band, rest = i - block * band, wide = min(8u, mt - block * 8);
+        const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
+        t.m0 = t.am = (int)(tm * 256);
+        t.n0 = (int)(tn * BN);
+        t.mend = min(m - t.m0, 256) + t.m0;
+        t.nend = min(n - t.n0, BN) + t.n0;
+        t.k0 = 0;
+        t.q0 = min((int)part * per, nkb);
+        t.nkb = min(per, nkb - t.q0);
+        t.bz = 0;
+        t.tail = 0;
+        t.kind = 0;
+        t.aux = (int)part;
+    }
 };
 
-// A tile's place is found in 32 bits (64-bit divisions between two tiles held
-// the products up by some 1000 clocks); launch() refuses more units.
 struct DenseIter {
     uint32_t at, step;
     template <class Op> __device__ DenseIter(const Op &, int cid, int ncl) : at(cid), step(ncl) {}
     template <class Op> __device__ bool next(const Op &op, tc::Tile &t) {
-        const Dense &g = op.dense;
-        const uint32_t tiles = g.mt * g.nt;
-        if (at >= tiles * g.splits) return false;
-        const uint32_t part = g.splits > 1 ? at / tiles : 0, i = at - part * tiles;
-        const uint32_t band = 8 * g.nt, block = i / band, rest = i - block * band, wide = min(8u, g.mt - block * 8);
-        const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
-        const int k0 = min((int)part * g.per, g.nkb);
-        t.m0 = t.am = (int)(tm * 256);
-        t.n0 = t.bn = (int)(tn * Dense::kBN);
-        t.mend = min(g.m - t.m0, 256) + t.m0;
-        t.nend = min(g.n - t.n0, Dense::kBN) + t.n0;
-        t.ka = t.kb = k0 * tc::kBK;
-        t.nkb = min(g.per, g.nkb - k0);
-        t.az = t.bz = 0;
-        t.tail = 0;
-        t.aux = (int)part;
+        if (at >= (uint32_t)(op.dense.mt * op.dense.nt) * op.dense.splits) return false;
+        op.dense.template place<Op::kBN>(at, t);
         at += step;
         return true;
     }
@@ -247,7 +327,8 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 // is needed.
 struct XentStats {
     static constexpr int kBN = 256;
-    static constexpr bool kAMN = false, kBMN = false, kTail = false;
+    static constexpr bool kAMN = false, kBMN = false, kTail = false, kDual = false;
+    static constexpr int laps = 1;
     using Iter = DenseIter;
     Dense dense;
     const int64_t *target;
@@ -297,6 +378,7 @@ struct XentStats {
 // lse and loss from the tiles' parts: 8 rows a block, 32 threads a row.
 __global__ void __launch_bounds__(256) k_xent_join(const float2 *__restrict__ part, int64_t n, int64_t nt, int64_t v, const int64_t *__restrict__ target,
                                                    const float *__restrict__ ly, float *__restrict__ loss, float *__restrict__ lse) {
+    tc::depend();
     __shared__ float2 sh[32][9];
     const int r = threadIdx.x % 8, q = threadIdx.x / 8;
     const int64_t row = blockIdx.x * 8LL + r;
@@ -317,39 +399,20 @@ __global__ void __launch_bounds__(256) k_xent_join(const float2 *__restrict__ pa
     loss[row] = y >= 0 && y < v ? z - ly[row] : 0.f;
 }
 
-// The power of two that takes the largest |grad_loss| of the rows that count
-// to at most 2^14, half precision's range (scale[0], its inverse in scale[1]).
-__global__ void __launch_bounds__(1024) k_xent_scale(const float *__restrict__ grad_loss, const int64_t *__restrict__ target, int64_t n, int64_t v,
-                                                     float *scale) {
-    __shared__ float red[32];
-    float m = 0.f;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) {
-        const int64_t y = target[i];
-        if (y >= 0 && y < v) m = fmaxf(m, fabsf(grad_loss[i]));
-    }
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
-    __syncthreads();
-    if (threadIdx.x) return;
-    for (int k = 1; k < 32; k++) m = fmaxf(m, red[k]);
-    int e = 0;
-    if (m > 0.f && m < INFINITY) e = min(max(14 - (ilogbf(m) + 1), -100), 100);
-    scale[0] = ldexpf(1.f, e);
-    scale[1] = ldexpf(1.f, -e);
-}
-
 // One piece of G: the logits once more, G = c (exp(l - lse) - [k = target])
-// times the scale, rounded to the products' type.
+// times the scale, rounded to the products' type.  With two parts what the
+// rounding leaves is rounded too and follows in a second matrix.
 template <class T> struct XentG {
     static constexpr int kBN = 256;
-    static constexpr bool kAMN = false, kBMN = false, kTail = false;
+    static constexpr bool kAMN = false, kBMN = false, kTail = false, kDual = false;
+    static constexpr int laps = 1;
     using Iter = DenseIter;
     Dense dense;
     int64_t c0, v;      // the piece's first class; classes in all
     const int64_t *target;
     const float *lse, *grad_loss, *scale;
     T *g;
-    int64_t ldg;
+    int64_t ldg, part;  // row stride; from the leading to the trailing part (0: one part)
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
         const int row = t.m0 + p.row, h0 = p.half * 128;
         int64_t y = -1;
@@ -365,136 +428,182 @@ template <class T> struct XentG {
         const int64_t off = y - c0 - t.n0 - h0;
         const int yc = has && off >= 0 && off < 128 ? (int)off : -1;
         const int row0 = t.m0 + p.row - p.lane;
-        tc::store_tile<T, 128>(
-            p, addr, g + (int64_t)row0 * ldg + t.n0 + h0, ldg, t.mend - row0, t.nend - t.n0 - h0, true, false,
-            [&](float (&x)[32], int col) {
-                const bool here = __any_sync(~0u, yc >= col && yc < col + 32);
+        auto value = [&](float (&x)[32], int col) {
+            const bool here = __any_sync(~0u, yc >= col && yc < col + 32);
 #pragma unroll
-                for (int i = 0; i < 32; i++) x[i] = c * ex2(fmaf(x[i], kLog2e, -z));
-                if (here) {
+            for (int i = 0; i < 32; i++) x[i] = c * ex2(fmaf(x[i], kLog2e, -z));
+            if (here) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (yc == col + i) x[i] -= c;
-                }
-                if (!all) {    // whatever an ignored row's features hold
+                for (int i = 0; i < 32; i++)
+                    if (yc == col + i) x[i] -= c;
+            }
+            if (!all) {    // whatever an ignored row's features hold
 #pragma unroll
-                    for (int i = 0; i < 32; i++) x[i] = has ? x[i] : 0.f;
-                }
-            },
-            release);
+                for (int i = 0; i < 32; i++) x[i] = has ? x[i] : 0.f;
+            }
+        };
+        T *out = g + (int64_t)row0 * ldg + t.n0 + h0;
+        const int rows = t.mend - row0, cols = t.nend - t.n0 - h0;
+        if (part) {
+            tc::store_tile<T, 128>(p, addr, out, ldg, rows, cols, 8, false, value, [] {});
+            tc::store_tile<T, 128>(
+                p, addr, out + part, ldg, rows, cols, 8, false,
+                [&](float (&x)[32], int col) {
+                    value(x, col);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] -= to_f(from_f<T>(x[i]));
+                },
+                release);
+        } else {
+            tc::store_tile<T, 128>(p, addr, out, ldg, rows, cols, 8, false, value, release);
+        }
     }
 };
 
-// C = A B with B's n axis contiguous: G w (A K-major), G^T x (A's m axis
-// contiguous too).  The result is rounded and stored when one launch makes all
-// of it (acc null); else its f32 sums go to acc [split][m][ldacc], on top of
-// what an earlier piece left there (add).
-template <class T, bool AMN> struct Product {
-    static constexpr int kBN = 256;
-    static constexpr bool kAMN = AMN, kBMN = true, kTail = false;
-    using Iter = DenseIter;
-    Dense dense;
+// Where a product's sums go.  One unit makes all of a tile where acc is null
+// or (with add) `last` says so; else the units leave f32 sums in acc
+// [split][m][ldacc], on top of an earlier piece's (add), and the last unit of
+// a tile to arrive (by a ticket a warp) adds the splits up, always in the
+// same order, so that the result does not depend on who came last.
+template <class T> struct Sink {
     const int64_t *target;     // rows whose target is ignored are 0 (null: none)
     int64_t v;
     const float *scale;        // scale[1] takes G's scale back (null: 1)
     T *out;
     int64_t ld;
-    bool vec;
+    int width;
     float *acc;
     int64_t ldacc;
-    bool add;
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
-        const int row = t.m0 + p.row, row0 = row - p.lane, h0 = p.half * 128, cols = t.nend - t.n0 - h0;
-        if (!acc) {
-            float c = scale ? scale[1] : 1.f;
-            bool has = true;
-            if (target && row < t.mend) {
-                const int64_t y = target[row];
-                has = y >= 0 && y < v;
-            }
-            tc::store_tile<T, 128>(
-                p, addr, out + (int64_t)row0 * ld + t.n0 + h0, ld, t.mend - row0, cols, vec, t.nkb == 0,
-                [&](float (&x)[32], int) {
-#pragma unroll
-                    for (int i = 0; i < 32; i++) x[i] = has ? x[i] * c : 0.f;
-                },
-                release);
-            return;
-        }
-        float *q = acc + ((int64_t)t.aux * dense.m + row) * ldacc + t.n0 + h0;
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-            float x[32];
-            if (t.nkb) {
-                tc::tmem_ld32(addr + c, x);
-                tc::tmem_wait(x);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; i++) x[i] = 0.f;
-            }
-            if (c == 96) release();
-            if (row < t.mend && c < cols) {     // ldacc is a multiple of 64: whole groups of 32 fit
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float4 w = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-                    float4 *d = (float4 *)(q + c) + i;
-                    if (add) {
-                        const float4 o = *d;
-                        w.x += o.x, w.y += o.y, w.z += o.z, w.w += o.w;
-                    }
-                    *d = w;
-                }
-            }
-        }
-    }
+    bool add, last;
+    uint32_t *tickets;         // [tile][16 warps of the pair]
 };
 
-// out = the splits' sums, scaled back and rounded; ignored rows 0.
-template <class T>
-__global__ void __launch_bounds__(256) k_sum_splits(const float *__restrict__ acc, int64_t ldacc, int64_t m, int64_t n, int splits,
-                                                    const float *__restrict__ scale, const int64_t *__restrict__ target, int64_t v, T *__restrict__ out,
-                                                    int64_t ld) {
-    const int64_t per = (n + 3) / 4, total = m * per;
-    const float c = scale ? scale[1] : 1.f;
-    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-        const int64_t r = i / per, k = (i - r * per) * 4;
-        float4 s = *(const float4 *)(acc + r * ldacc + k);
-        for (int q = 1; q < splits; q++) {
-            const float4 o = *(const float4 *)(acc + (q * m + r) * ldacc + k);
-            s.x += o.x, s.y += o.y, s.z += o.z, s.w += o.w;
-        }
-        bool has = true;
-        if (target) {
-            const int64_t y = target[r];
-            has = y >= 0 && y < v;
-        }
-        const float x[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (k + j < n) out[r * ld + k + j] = from_f<T>(has ? x[j] * c : 0.f);
+// f32 sums of a warp's 32 x COLS block: its place in acc.
+template <int COLS, class T, class R>
+__device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, const tc::Tile &t, const tc::Place &p, uint32_t addr, R release, int tile) {
+    const int row = t.m0 + p.row, row0 = row - p.lane, h0 = p.half * COLS, cols = t.nend - t.n0 - h0;
+    const float scale = k.scale ? k.scale[1] : 1.f;
+    bool has = row < t.mend;
+    if (k.target && has) {
+        const int64_t y = k.target[row];
+        has = y >= 0 && y < k.v;
     }
+    T *out = k.out + (int64_t)row0 * k.ld + t.n0 + h0;
+    const bool one = splits == 1;
+    float *q = k.acc ? k.acc + ((int64_t)t.aux * m + row) * k.ldacc + t.n0 + h0 : nullptr;
+    // ldacc is a multiple of 64: whole groups of 32 columns fit
+    const auto mine = [&](int c) { return row < t.mend && c < cols; };
+    if (!k.acc || (one && k.last)) {
+        tc::store_tile<T, COLS>(
+            p, addr, out, k.ld, t.mend - row0, cols, k.width, t.nkb == 0,
+            [&](float (&x)[32], int c) {
+                if (k.acc && k.add && mine(c)) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float4 o = ((const float4 *)(q + c))[i];
+                        x[4 * i] += o.x, x[4 * i + 1] += o.y, x[4 * i + 2] += o.z, x[4 * i + 3] += o.w;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i++) x[i] = has ? x[i] * scale : 0.f;
+            },
+            release);
+        return;
+    }
+#pragma unroll 1
+    for (int c = 0; c < COLS; c += 32) {
+        float x[32];
+        if (t.nkb) {
+            tc::tmem_ld32(addr + c, x);
+            tc::tmem_wait(x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; i++) x[i] = 0.f;
+        }
+        if (c == COLS - 32) release();
+        if (mine(c)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                float4 w = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                float4 *d = (float4 *)(q + c) + i;
+                if (k.add) {
+                    const float4 o = *d;
+                    w.x += o.x, w.y += o.y, w.z += o.z, w.w += o.w;
+                }
+                *d = w;
+            }
+        }
+    }
+    if (!k.last || one) return;
+    const int warp = p.rank * 8 + p.half * 4 + p.sub;
+    uint32_t n = 0;
+    __threadfence();
+    __syncwarp();
+    if (p.lane == 0) n = atomicAdd(k.tickets + (int64_t)tile * 16 + warp, 1u);
+    n = __shfl_sync(~0u, n, 0);
+    if (n != (uint32_t)splits - 1) return;
+    __threadfence();
+    const float *first = k.acc + (int64_t)row * k.ldacc + t.n0 + h0;
+    const int64_t step = (int64_t)m * k.ldacc;
+    tc::store_tile<T, COLS>(
+        p, addr, out, k.ld, t.mend - row0, cols, k.width, true,
+        [&](float (&x)[32], int c) {
+            if (!mine(c)) return;
+            for (int s = 0; s < splits; s++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float4 o = __ldcg((const float4 *)(first + s * step + c) + i);
+                    x[4 * i] += o.x, x[4 * i + 1] += o.y, x[4 * i + 2] += o.z, x[4 * i + 3] += o.w;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) x[i] = has ? x[i] * scale : 0.f;
+        },
+        [] {});
 }
 
-template <class T>
-Err sum_splits(const float *acc, int64_t ldacc, int64_t m, int64_t n, int splits, const float *scale, const int64_t *target, int64_t v, T *out,
-               int64_t ld, cudaStream_t st) {
-    const int64_t blocks = std::min<int64_t>((m * ((n + 3) / 4) + 255) / 256, sm_count() * 16LL);
-    k_sum_splits<T><<<(unsigned)blocks, 256, 0, st>>>(acc, ldacc, m, n, splits, scale, target, v, out, ld);
-    return {};
-}
+// dx = G w (A K-major) and dw = G^T x (A's m axis contiguous), B's n axis
+// contiguous in both, as one pool of tiles: neither alone fills its last wave.
+// The product with the longer k axis goes first.
+template <class T, int BN> struct XentPair {
+    static constexpr int kBN = BN;
+    static constexpr bool kAMN = false, kBMN = true, kTail = false, kDual = true;
+    struct Iter {
+        uint32_t at, step;
+        __device__ Iter(const XentPair &, int cid, int ncl) : at(cid), step(ncl) {}
+        __device__ bool next(const XentPair &op, tc::Tile &t) {
+            const uint32_t u0 = (uint32_t)(op.dense[0].mt * op.dense[0].nt) * op.dense[0].splits,
+                           u1 = (uint32_t)(op.dense[1].mt * op.dense[1].nt) * op.dense[1].splits;
+            if (at >= u0 + u1) return false;
+            const int kind = op.first ? at < u1 : at >= u0;
+            const uint32_t i = op.first ? (kind ? at : at - u1) : (kind ? at - u0 : at);
+            op.dense[kind].template place<BN>(i, t);
+            t.kind = kind;
+            at += step;
+            return true;
+        }
+    };
+    Dense dense[2];
+    Sink<T> sink[2];
+    int first, laps;
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+        const Dense &g = dense[t.kind];
+        sink_tile<BN / 2>(sink[t.kind], g.m, g.splits, t, p, addr, release, (t.m0 / 256) * g.nt + t.n0 / BN);
+    }
+};
 
 // Parts of the k axis for a product of `tiles` tiles and `nkb` stages: as many
 // as make the longest chain of stages one cluster works through shortest,
 // counting about 8 stages' time for a tile's start and end and the time the
-// f32 sums take to be written and read again (65536 x 8 bytes a tile: about a
-// sixth of a stage's 0.27 us spread over 74 clusters).
+// f32 sums take to be written and read again (512 KB a tile of 256 x 256,
+// 0.08 us at the memory's rate: 0.3 of a stage's 0.27 us).
 int choose_splits(int64_t tiles, int64_t nkb) {
     constexpr int64_t kClusters = 74;      // 148 SMs; fixed, so that sizes alone set the workspace
     int best = 1;
     double least = 1e300;
     for (int s = 1; s <= 32 && s <= nkb; s++) {
         const int64_t waves = (tiles * s + kClusters - 1) / kClusters;
-        const double t = (double)waves * ((nkb + s - 1) / s + 8) + (s > 1 ? 10.0 + tiles * s * 0.3 : 0.0);
+        const double t = (double)waves * ((nkb + s - 1) / s + 8) + (s > 1 ? 8.0 + tiles * s * 0.3 : 0.0);
         if (t < least * 0.98) least = t, best = s;
     }
     return best;
@@ -507,21 +616,32 @@ struct XentPlan {
     int64_t pc;        // classes of a piece, a multiple of 256 unless there is one piece
     int64_t ldg;       // row stride of G
     int64_t ldacc;
+    int bn;            // columns of the products' tiles
+    int parts;         // of G: see below
     int pieces, sx, sw;
+    int64_t tx, tw;    // tiles
     XentPlan(int64_t n, int64_t d, int64_t v) {
         dp = round_up(d, 8);
+        // One tile of rows: the products are bound by memory and launches,
+        // and few rounded values of G weigh in a result (with one row a
+        // single one), whose rounding does not average out: keep G in two parts.
+        parts = n <= 256 ? 2 : 1;
+        bn = d <= 128 ? 128 : 256;
         constexpr int64_t kMost = 256 << 20;
-        pieces = (int)std::min<int64_t>((n * v * 2 + kMost - 1) / kMost, (v + 255) / 256);
+        pieces = (int)std::min<int64_t>((n * v * 2 * parts + kMost - 1) / kMost, (v + 255) / 256);
         pieces = std::max(pieces, 1);
         pc = pieces > 1 ? std::min(v, round_up((v + pieces - 1) / pieces, 256)) : v;
         pieces = (int)((v + pc - 1) / pc);
         ldg = round_up(pc, 64);
         ldacc = round_up(d, 64);
-        const int64_t mt = (n + 255) / 256, vt = (pc + 255) / 256, dt = (d + 255) / 256;
-        sx = choose_splits(mt * dt, (pc + 63) / 64);
-        sw = choose_splits(vt * dt, (n + 63) / 64);
+        const int64_t dt = (d + bn - 1) / bn;
+        tx = (n + 255) / 256 * dt;
+        tw = (pc + 255) / 256 * dt;
+        sx = choose_splits(tx, (pc + 63) / 64 * parts);
+        sw = choose_splits(tw, (n + 63) / 64 * parts);
     }
     bool dx_acc() const { return pieces > 1 || sx > 1; }
+    int64_t tickets() const { return 16 * (tx + tw * pieces); }
 };
 
 struct Room {
@@ -554,14 +674,16 @@ struct XentLoss {
 struct XentGrad {
     uint16_t *x, *w, *g;
     float *accx, *accw, *scale;
+    uint32_t *tickets;
     int64_t bytes;
     XentGrad(void *ws, int64_t n, int64_t d, int64_t v, bool in_place) {
         Room r(ws);
         const XentPlan pl(n, d, v);
         scale = r.take<float>(2);
+        tickets = r.take<uint32_t>(pl.tickets());
         x = r.take<uint16_t>(n * pl.dp);
         w = r.take<uint16_t>(in_place ? 0 : v * pl.dp);
-        g = r.take<uint16_t>(n * pl.ldg);
+        g = r.take<uint16_t>(n * pl.ldg * pl.parts);
         accx = r.take<float>(pl.dx_acc() ? pl.sx * n * pl.ldacc : 0);
         accw = r.take<float>(pl.sw > 1 ? pl.sw * pl.pc * pl.ldacc : 0);
         bytes = r.bytes();
@@ -575,54 +697,66 @@ bool sizes_ok(int64_t n, int64_t d, int64_t v) {
 Err xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, bool bf16, int64_t n, int64_t d, int64_t v, const int64_t *target, float *loss,
                  float *lse, void *ws, cudaStream_t st) {
     XentLoss q(ws, n, d, v, tma_rows(x, ldx) && tma_rows(w, ldw));
-    const View a = readable({x, d, n, ldx}, q.x, st), b = readable({w, d, v, ldw}, q.w, st);
-    XentStats op{Dense(n, v, d, 1), target, q.part, q.ly};
-    Err e = launch(a, b, op, bf16, op.dense.units(), st);
+    Prep prep;
+    const View a = readable(prep, {x, d, n, ldx}, q.x), b = readable(prep, {w, d, v, ldw}, q.w);
+    Err e = run_prep(prep, st);
     if (e.bad()) return e;
-    k_xent_join<<<(unsigned)((n + 7) / 8), 256, 0, st>>>(q.part, n, (v + 255) / 256 * 2, v, target, q.ly, loss, lse);
-    return {};
+    XentStats op{Dense(n, v, d, 256), target, q.part, q.ly};
+    const View ab[2] = {a, b};
+    e = launch(ab, op, bf16, op.dense.units(), st);
+    if (e.bad()) return e;
+    return start(k_xent_join, (n + 7) / 8, 256, 0, st, q.part, n, (v + 255) / 256 * 2, v, target, q.ly, loss, lse);
+}
+
+template <class T, int BN>
+Err xent_pair(const XentPlan &pl, const XentGrad &q, const View &xs, const View &wp, const float *scale, int64_t n, int64_t d, int64_t v, int64_t c, int64_t pc,
+              const int64_t *target, T *dx, int64_t lddx, T *dw, int64_t lddw, cudaStream_t st) {
+    const View gv{q.g, pc, n, pl.ldg, pl.parts};
+    const View views[4] = {gv, wp, gv, xs};
+    XentPair<T, BN> op{};
+    if (dx) {
+        op.dense[0] = Dense(n, d, pc, BN, pl.sx, pl.parts);
+        op.sink[0] = {target, v, scale, dx, lddx, tc::store_width(dx, lddx), pl.dx_acc() ? q.accx : nullptr, pl.ldacc, c > 0, c + pc == v, q.tickets};
+    }
+    if (dw) {
+        T *o = dw + c * lddw;
+        op.dense[1] = Dense(pc, d, n, BN, pl.sw, pl.parts);
+        op.sink[1] = {nullptr, 0, scale, o, lddw, tc::store_width(o, lddw), pl.sw > 1 ? q.accw : nullptr, pl.ldacc, false, true,
+                      q.tickets + 16 * (pl.tx + pl.tw * (c / pl.pc))};
+    }
+    op.first = op.dense[1].per > op.dense[0].per;
+    op.laps = pl.parts;
+    return launch(views, op, std::is_same<T, __nv_bfloat16>::value, op.dense[0].units() + op.dense[1].units(), st);
 }
 
 template <class T>
 Err xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t n, int64_t d, int64_t v, const int64_t *target, const float *lse,
                   const float *grad_loss, T *dx, int64_t lddx, T *dw, int64_t lddw, void *ws, cudaStream_t st) {
-    constexpr bool bf16 = sizeof(T) && std::is_same<T, __nv_bfloat16>::value;
+    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
     const XentPlan pl(n, d, v);
-    XentGrad q(ws, n, d, v, tma_rows(x, ldx) && tma_rows(w, ldw));
+    const XentGrad q(ws, n, d, v, tma_rows(x, ldx) && tma_rows(w, ldw));
+    Prep prep;
     // rows that count, zeros in the others': an ignored row's features must not reach dw
-    pack(x, ldx, n, d, q.x, pl.dp, target, v, st);
-    const View xs{q.x, d, n, pl.dp}, wv = readable({w, d, v, ldw}, q.w, st);
-    const float *scale = nullptr;
-    if (!bf16) {
-        k_xent_scale<<<1, 1024, 0, st>>>(grad_loss, target, n, v, q.scale);
-        scale = q.scale;
-    }
+    add_pack(prep, {x, d, n, ldx}, q.x, pl.dp, target, v);
+    const View xs{q.x, d, n, pl.dp}, wv = readable(prep, {w, d, v, ldw}, q.w);
+    if (pl.sx > 1 || pl.sw > 1) prep.tickets = q.tickets, prep.n_tickets = (int)pl.tickets();
+    if (!bf16) prep.grad_loss = grad_loss, prep.target = target, prep.n = n, prep.v = v, prep.scale = q.scale;
+    Err e = run_prep(prep, st);
+    const float *scale = prep.scale;
     T *g = (T *)q.g;
-    for (int64_t c = 0; c < v; c += pl.pc) {
+    for (int64_t c = 0; c < v && !e.bad(); c += pl.pc) {
         const int64_t pc = std::min(pl.pc, v - c);
         View wp = wv;
         wp.p = (const char *)wv.p + c * wv.ld * 2;
         wp.rows = pc;
-        XentG<T> og{Dense(n, pc, d, 1), c, v, target, lse, grad_loss, scale, g, pl.ldg};
-        Err e = launch(xs, wp, og, bf16, og.dense.units(), st);
-        if (e.bad()) return e;
-        const View gv{g, pc, n, pl.ldg};
-        if (dx) {
-            const bool acc = pl.dx_acc();
-            Product<T, false> op{Dense(n, d, pc, pl.sx), target, v, scale, dx, lddx, tma_rows(dx, lddx), acc ? q.accx : nullptr, pl.ldacc, c > 0};
-            e = launch(gv, wp, op, bf16, op.dense.units(), st);
-            if (e.bad()) return e;
-        }
-        if (dw) {
-            T *o = dw + c * lddw;
-            Product<T, true> op{Dense(pc, d, n, pl.sw), nullptr, 0, scale, o, lddw, tma_rows(o, lddw), pl.sw > 1 ? q.accw : nullptr, pl.ldacc, false};
-            e = launch(gv, xs, op, bf16, op.dense.units(), st);
-            if (!e.bad() && pl.sw > 1) e = sum_splits<T>(q.accw, pl.ldacc, pc, d, pl.sw, scale, nullptr, 0, o, lddw, st);
-            if (e.bad()) return e;
-        }
+        XentG<T> og{Dense(n, pc, d, 256), c, v, target, lse, grad_loss, scale, g, pl.ldg, pl.parts > 1 ? n * pl.ldg : 0};
+        const View xw[2] = {xs, wp};
+        e = launch(xw, og, bf16, og.dense.units(), st);
+        if (e.bad()) break;
+        e = pl.bn == 128 ? xent_pair<T, 128>(pl, q, xs, wp, scale, n, d, v, c, pc, target, dx, lddx, dw, lddw, st)
+                         : xent_pair<T, 256>(pl, q, xs, wp, scale, n, d, v, c, pc, target, dx, lddx, dw, lddw, st);
     }
-    if (dx && pl.dx_acc()) return sum_splits<T>(q.accx, pl.ldacc, n, d, pl.sx, scale, target, v, dx, lddx, st);
-    return {};
+    return e;
 }
 
 // ---------------------------------------------------------------------------
@@ -680,14 +814,14 @@ struct LeafIter {
         const uint32_t band = 8 * nt, block = i / band, rest = i - block * band, wide = min(8u, rt - block * 8);
         const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
         t.m0 = t.am = a + (int)tm * 256;
-        t.n0 = t.bn = (int)(tn * 256);
+        t.n0 = (int)(tn * 256);
         t.mend = min(b - t.m0, 256) + t.m0;
         t.nend = min(op.leaves.n - t.n0, 256) + t.n0;
-        t.ka = t.kb = 0;
+        t.k0 = t.q0 = 0;
         t.nkb = op.leaves.nkb;
-        t.az = 0;
         t.bz = first + l;
         t.tail = 0;
+        t.kind = 0;
         t.aux = 0;
         at += step;
         return true;
@@ -699,15 +833,16 @@ struct LeafIter {
 // computed with this leaf's weights and not stored.
 template <class T, bool BMN> struct LeafRows {
     static constexpr int kBN = 256;
-    static constexpr bool kAMN = false, kBMN = BMN, kTail = false;
+    static constexpr bool kAMN = false, kBMN = BMN, kTail = false, kDual = false;
+    static constexpr int laps = 1;
     using Iter = LeafIter;
     Leaves leaves;
     T *out;
     int64_t ld;
-    bool vec;
+    int width;
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
         const int row0 = t.m0 + p.row - p.lane, h0 = p.half * 128;
-        tc::store_tile<T, 128>(p, addr, out + (int64_t)row0 * ld + t.n0 + h0, ld, t.mend - row0, t.nend - t.n0 - h0, vec, false, [](float (&)[32], int) {}, release);
+        tc::store_tile<T, 128>(p, addr, out + (int64_t)row0 * ld + t.n0 + h0, ld, t.mend - row0, t.nend - t.n0 - h0, width, false, [](float (&)[32], int) {}, release);
     }
 };
 
@@ -725,12 +860,14 @@ struct LeafDwIter {
         const int nkb = (hi - lo + 63) / 64, each = op.splits > 1 ? (nkb + op.splits - 1) / op.splits : nkb, k0 = min((int)part * each, nkb),
                   k1 = min(k0 + each, nkb);
         t.m0 = t.am = (int)tm * 256;
-        t.n0 = t.bn = (int)tn * 256;
+        t.n0 = (int)tn * 256;
         t.mend = min((int)op.dout - t.m0, 256) + t.m0;
         t.nend = min((int)op.din - t.n0, 256) + t.n0;
-        t.ka = t.kb = lo + k0 * 64;
+        t.k0 = lo;
+        t.q0 = k0;
         t.nkb = k1 - k0;
-        t.az = t.bz = 0;
+        t.bz = 0;
+        t.kind = 0;
         // behind the last row of all TMA fills zeros
         t.tail = k1 == nkb && hi < op.t ? (hi - lo) % 64 : 0;
         t.aux = (int)(part * op.groups + g);
@@ -741,45 +878,28 @@ struct LeafDwIter {
 
 template <class T> struct LeafDw {
     static constexpr int kBN = 256;
-    static constexpr bool kAMN = true, kBMN = true, kTail = true;
+    static constexpr bool kAMN = true, kBMN = true, kTail = true, kDual = false;
+    static constexpr int laps = 1;
     using Iter = LeafDwIter;
     const int32_t *off;
     int64_t t, din, dout;
     int32_t groups;
     int splits, mt, nt;
-    T *out;
-    bool vec;
-    float *acc;         // [split][groups * dout][ldacc] where there are several
-    int64_t ldacc;
+    Sink<T> sink;       // of the (groups * dout) x din matrix of all leaves' dw
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
-        const int row = t.m0 + p.row, row0 = row - p.lane, h0 = p.half * 128, cols = t.nend - t.n0 - h0;
-        if (!acc) {
-            tc::store_tile<T, 128>(p, addr, out + ((int64_t)t.aux * dout + row0) * din + t.n0 + h0, din, t.mend - row0, cols, vec, t.nkb == 0,
-                                   [](float (&)[32], int) {}, release);
-            return;
-        }
-        float *q = acc + ((int64_t)t.aux * dout + row) * ldacc + t.n0 + h0;
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-            float x[32];
-            if (t.nkb) {
-                tc::tmem_ld32(addr + c, x);
-                tc::tmem_wait(x);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; i++) x[i] = 0.f;
-            }
-            if (c == 96) release();
-            if (row < t.mend && c < cols) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) ((float4 *)(q + c))[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-            }
-        }
+        // the leaf's tile as one of that matrix
+        tc::Tile all = t;
+        const int g = t.aux % groups, base = g * (int)dout;
+        all.m0 += base;
+        all.mend += base;
+        all.aux = t.aux / groups;
+        sink_tile<128>(sink, groups * (int)dout, splits, all, p, addr, release, (g * mt + t.m0 / 256) * nt + t.n0 / 256);
     }
 };
 
 // The rows before the first leaf and behind the last one as zeros.
 template <class T> __global__ void k_leaf_rest(const int32_t *off, int32_t groups, int64_t t, int64_t cols, T *y, int64_t ldy) {
+    tc::depend();
     const int64_t lo = min(max((int64_t)off[0], (int64_t)0), t), hi = max(min((int64_t)off[groups], t), lo);
     const int64_t rest = lo + (t - hi);
     for (int64_t r = blockIdx.x; r < rest; r += gridDim.x) {
@@ -795,7 +915,8 @@ int leaf_splits(int64_t t, int32_t groups, int64_t din, int64_t dout) {
 struct LeafWs {
     uint16_t *x, *w, *dy;
     float *acc;
-    int64_t ldacc, bytes;
+    uint32_t *tickets;
+    int64_t ldacc, n_tickets, bytes;
     LeafWs(void *ws, int64_t t, int32_t groups, int64_t din, int64_t dout, bool grad, bool in_place) {
         Room r(ws);
         const int64_t ip = round_up(din, 8), op = round_up(dout, 8);
@@ -805,6 +926,8 @@ struct LeafWs {
         ldacc = round_up(din, 64);
         const int s = grad ? leaf_splits(t, groups, din, dout) : 1;
         acc = r.take<float>(s > 1 ? s * groups * dout * ldacc : 0);
+        n_tickets = s > 1 ? 16 * groups * ((din + 255) / 256) * ((dout + 255) / 256) : 0;
+        tickets = r.take<uint32_t>(n_tickets);
         bytes = r.bytes();
     }
 };
@@ -813,18 +936,21 @@ template <class T, bool BMN>
 Err leaf_rows_launch(const View &a, const View &w, const int32_t *off, int64_t t, int32_t groups, int64_t k, int64_t n, T *y, int64_t ldy, bool zero_rest,
                      cudaStream_t st) {
     constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    LeafRows<T, BMN> op{Leaves(off, t, groups, k, n), y, ldy, tma_rows(y, ldy)};
-    Err e = launch(a, w, op, bf16, op.leaves.units(), st);
-    if (!e.bad() && zero_rest) k_leaf_rest<T><<<(unsigned)std::min<int64_t>(t, sm_count()), 256, 0, st>>>(off, groups, t, n, y, ldy);
+    LeafRows<T, BMN> op{Leaves(off, t, groups, k, n), y, ldy, tc::store_width(y, ldy)};
+    const View views[2] = {a, w};
+    Err e = launch(views, op, bf16, op.leaves.units(), st);
+    if (!e.bad() && zero_rest) e = start(k_leaf_rest<T>, std::min<int64_t>(t, sm_count()), 256, 0, st, off, groups, t, n, y, ldy);
     return e;
 }
 
 template <class T>
 Err leaf_forward(const void *x, int64_t ldx, const void *w, const int32_t *off, int64_t t, int32_t groups, int64_t din, int64_t dout, T *y, int64_t ldy,
                  bool zero_rest, void *ws, cudaStream_t st) {
-    LeafWs q(ws, t, groups, din, dout, false, tma_rows(x, ldx) && tma_rows(w, din));
-    const View a = readable({x, din, t, ldx}, q.x, st), b = readable({w, din, dout, din, groups}, q.w, st);
-    return leaf_rows_launch<T, false>(a, b, off, t, groups, din, dout, y, ldy, zero_rest, st);
+    const LeafWs q(ws, t, groups, din, dout, false, tma_rows(x, ldx) && tma_rows(w, din));
+    Prep prep;
+    const View a = readable(prep, {x, din, t, ldx}, q.x), b = readable(prep, {w, din, dout, din, groups}, q.w);
+    Err e = run_prep(prep, st);
+    return e.bad() ? e : leaf_rows_launch<T, false>(a, b, off, t, groups, din, dout, y, ldy, zero_rest, st);
 }
 
 template <class T>
@@ -832,25 +958,28 @@ Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off,
                   int64_t dout, T *dx, int64_t lddx, bool zero_rest, T *dw, void *ws, cudaStream_t st) {
     constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
     const bool in_place = (!dw || tma_rows(x, ldx)) && (!dx || tma_rows(w, din)) && tma_rows(dy, lddy);
-    LeafWs q(ws, t, groups, din, dout, true, in_place);
+    const LeafWs q(ws, t, groups, din, dout, true, in_place);
     if (!t) {
         if (dw && cudaMemsetAsync(dw, 0, (size_t)groups * dout * din * 2, st) != cudaSuccess) return {GBM_ERR_CUDA, "cudaMemsetAsync"};
         return {};
     }
-    const View g = readable({dy, dout, t, lddy}, q.dy, st);
-    if (dx) {
-        const View b = readable({w, din, dout, din, groups}, q.w, st);
-        Err e = leaf_rows_launch<T, true>(g, b, off, t, groups, dout, din, dx, lddx, zero_rest, st);
-        if (e.bad()) return e;
+    Prep prep;
+    const View g = readable(prep, {dy, dout, t, lddy}, q.dy);
+    View a{}, b{};
+    if (dx) b = readable(prep, {w, din, dout, din, groups}, q.w);
+    if (dw) {
+        a = readable(prep, {x, din, t, ldx}, q.x);
+        prep.tickets = q.tickets;
+        prep.n_tickets = (int)q.n_tickets;
     }
-    if (!dw) return {};
-    const View a = readable({x, din, t, ldx}, q.x, st);
-    const int s = leaf_splits(t, groups, din, dout);
-    const int mt = (int)((dout + 255) / 256), nt = (int)((din + 255) / 256);
-    LeafDw<T> op{off, t, din, dout, groups, s, mt, nt, dw, tma_rows(dw, din), s > 1 ? q.acc : nullptr, q.ldacc};
-    Err e = launch(g, a, op, bf16, (int64_t)groups * s * mt * nt, st);
-    if (!e.bad() && s > 1) e = sum_splits<T>(q.acc, q.ldacc, groups * dout, din, s, nullptr, nullptr, 0, dw, din, st);
-    return e;
+    Err e = run_prep(prep, st);
+    if (dx && !e.bad()) e = leaf_rows_launch<T, true>(g, b, off, t, groups, dout, din, dx, lddx, zero_rest, st);
+    if (!dw || e.bad()) return e;
+    const int s = leaf_splits(t, groups, din, dout), mt = (int)((dout + 255) / 256), nt = (int)((din + 255) / 256);
+    LeafDw<T> op{off, t, din, dout, groups, s, mt, nt,
+                 {nullptr, 0, nullptr, dw, din, tc::store_width(dw, din), s > 1 ? q.acc : nullptr, q.ldacc, false, true, q.tickets}};
+    const View views[2] = {g, a};
+    return launch(views, op, bf16, (int64_t)groups * s * mt * nt, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -1079,7 +1208,7 @@ int gbm_softmax_xent_grad(const void *x, int64_t ldx, const void *w, int64_t ldw
 }
 
 int64_t gbm_leaf_linear_workspace(int64_t t, int32_t groups, int64_t din, int64_t dout, int32_t grad, int32_t in_place) {
-    if (!sizes_ok(t, din, dout) || groups < 1 || groups >= 65536) return -1;
+    if (!sizes_ok(t, din, dout) || groups < 1 || groups >= 65536 || groups * dout > kMaxDim) return -1;
     return LeafWs(nullptr, t, groups, din, dout, grad != 0, in_place != 0).bytes;
 }
 
@@ -1087,7 +1216,7 @@ static int leaf_check(const char *what, const int32_t *offsets, int32_t dtype, i
                       int64_t dout, bool in_place, const void *ws, int64_t ws_bytes, int32_t grad, char *errbuf, int32_t errlen) {
     if (dtype != GBM_TYPE_BF16 && dtype != GBM_TYPE_F16)
         return fail(errbuf, errlen, GBM_ERR_UNSUPPORTED, "%s: type %d is neither bf16 nor f16", what, dtype);
-    if (!sizes_ok(t, din, dout) || groups < 1 || groups >= 65536)
+    if (!sizes_ok(t, din, dout) || groups < 1 || groups >= 65536 || groups * dout > kMaxDim)
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: sizes t=%lld groups=%d din=%lld dout=%lld out of range", what,
                     (long long)t, groups, (long long)din, (long long)dout);
     if (!offsets || !aligned(offsets, 4)) return fail(errbuf, errlen, GBM_ERR_ARG, "%s: offsets null or not aligned", what);

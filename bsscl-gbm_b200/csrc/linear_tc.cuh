@@ -166,27 +166,40 @@ __device__ __forceinline__ void tmem_wait(float *v) {
     for (int i = 0; i < 32; i++) asm volatile("" : "+f"(v[i]));
 }
 
-// kind::f16: sums in f32; A and B bf16 (1) or f16 (0); M = 256, N = BN
-inline uint32_t make_idesc(bool bf16, bool a_mn, bool b_mn, int bn) {
-    return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 |
+// kind::f16: sums in f32; A and B bf16 (1) or f16 (0); M = 256, N = BN;
+// bit 15 (A's m axis contiguous) is set tile by tile
+inline uint32_t make_idesc(bool bf16, bool b_mn, int bn) {
+    return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10  | (b_mn ? 1u : 0u) << 16 |
            (uint32_t)(bn >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
+}
+
+// A launch may start before the one in front of it has ended (its set-up
+// overlaps that one's end); from here on that one's results are there.
+__device__ __forceinline__ void depend() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // ---- the frame --------------------------------------------------------------
 
-// One unit of work: C[m0 .. mend) x [n0 .. nend) (256 x BN at most) over
-// nkb stages from k0.  ka/kb_: where the k axis starts in A and B (they
-// differ where B is one piece of a longer axis).  tail: rows of k that count
-// in the last stage where the operands go on behind the k axis' end (0: the
-// maps end there, TMA fills zeros).
+// One unit of work: C[m0 .. mend) x [n0 .. nend) (256 x BN at most), the
+// stages q0 .. q0 + nkb - 1 of its k axis, which starts at k0 in the maps.
+// With two parts of A (batches 0 and 1 of its map: a value's leading and
+// trailing bits), the stages take both parts of one block of k in turn.
+// tail: rows of k that count in the last stage where the operands go on
+// behind the k axis' end (0: the maps end there, TMA fills zeros).
 struct Tile {
     int m0, n0, mend, nend;
-    int am, bn;       // first row of A's m axis and B's n axis in their maps
-    int ka, kb;
-    int nkb;
-    int az, bz;       // batch coordinates
+    int am;           // A's first row in its map (m0 but for a piece of a longer axis)
+    int k0, q0, nkb;
+    int bz;           // B's batch
     int tail;
+    int kind;         // which of a launch's two products
     int aux;
+};
+// The operands' maps: A and B of the first product, A and B of the second.
+struct Maps {
+    alignas(64) CUtensorMap m[4];
 };
 
 // What one epilogue warp knows of its place.
@@ -198,7 +211,7 @@ struct Place {
 
 template <class Op>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Op op, const uint32_t idesc) {
+k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uint32_t idesc) {
     constexpr int BN = Op::kBN;
     using S = Shape<BN>;
     constexpr int kCols = 2 * BN < 32 ? 32 : 2 * BN;    // tensor memory columns: a power of two
@@ -216,8 +229,7 @@ k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensor
     const int cid = blockIdx.x / 2, ncl = gridDim.x / 2;
 
     if (warp == 0 && lane == 0) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+        for (int i = 0; i < (Op::kDual ? 4 : 2); i++) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.m[i]) : "memory");
         for (int s = 0; s < S::kStages; s++) {
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
@@ -241,6 +253,7 @@ k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensor
     cluster_sync();
     fence_after();
     const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+    depend();
 
     if (warp == 0) {
         // ---- fetch
@@ -271,19 +284,20 @@ k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensor
                         else
                             tma_pair(dst, m, bar, x, y, z);
                     };
-                    const int am = t.am + (int)rank * 128, ka = t.ka + k * kBK;
-                    if (Op::kAMN) {
-                        load(a, &map_a, am, ka, t.az);
-                        load(a + 8192, &map_a, am + 64, ka, t.az);
+                    const CUtensorMap *ma = &maps.m[Op::kDual ? 2 * t.kind : 0], *mb = ma + 1;
+                    const int q = t.q0 + k, z = op.laps == 2 ? q & 1 : 0, at = t.k0 + (op.laps == 2 ? q >> 1 : q) * kBK;
+                    const int am = t.am + (int)rank * 128, bn = t.n0 + (int)rank * (BN / 2);
+                    if (Op::kDual ? t.kind == 1 : Op::kAMN) {
+                        load(a, ma, am, at, z);
+                        load(a + 8192, ma, am + 64, at, z);
                     } else {
-                        load(a, &map_a, ka, am, t.az);
+                        load(a, ma, at, am, z);
                     }
-                    const int bn = t.bn + (int)rank * (BN / 2), kb = t.kb + k * kBK;
                     if (Op::kBMN) {
 #pragma unroll
-                        for (int j = 0; j < BN / 2; j += 64) load(b + j * 128, &map_b, bn + j, kb, t.bz);
+                        for (int j = 0; j < BN / 2; j += 64) load(b + j * 128, mb, bn + j, at, t.bz);
                     } else {
-                        load(b, &map_b, kb, bn, t.bz);
+                        load(b, mb, at, bn, t.bz);
                     }
                 }
                 if (tail) {
@@ -318,6 +332,9 @@ k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensor
                 n++;
                 fence_after();
                 const uint32_t d = tmem + buf * BN;
+                const bool amn = Op::kDual ? t.kind == 1 : Op::kAMN;
+                const uint32_t id = idesc | (uint32_t)amn << 15;
+                const uint64_t astep = amn ? kKStep<true> : kKStep<false>;
                 for (int k = 0; k < t.nkb; k++) {
                     if (!mbar_wait(full + 8 * s, ph, dead)) {
                         ok = false;
@@ -333,11 +350,11 @@ k_tc(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensor
                     fence_after();
                     if (lane == 0) {
                         const uint32_t a = stages + s * S::kStage, b = a + kABytes;
-                        uint64_t da = make_desc<Op::kAMN>(a), db = make_desc<Op::kBMN>(b);
+                        uint64_t da = amn ? make_desc<true>(a) : make_desc<false>(a), db = make_desc<Op::kBMN>(b);
 #pragma unroll
                         for (int j = 0; j < kBK / 16; j++) {
-                            mma_pair(d, da, db, idesc, k > 0 || j > 0);
-                            da += kKStep<Op::kAMN>;
+                            mma_pair(d, da, db, id, k > 0 || j > 0);
+                            da += astep;
                             db += kKStep<Op::kBMN>;
                         }
                         commit_pair(empty + 8 * s);
@@ -393,24 +410,48 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
     return *reinterpret_cast<uint32_t *>(&v);
 }
 
+// Elements of one store that rows at `p`, `ld` apart, allow: 8, 4, 2 or 1.
+__host__ __device__ inline int store_width(const void *p, int64_t ld) {
+    const uint64_t a = (uint64_t)(uintptr_t)p | (uint64_t)ld * 2;
+    return a & 15 ? a & 7 ? a & 3 ? 1 : 2 : 4 : 8;
+}
+
+// Stores elements [0, n) (n <= 8) of the 16 bytes q.
+template <class T> __device__ __forceinline__ void store8(T *dst, uint4 q, int n, int width) {
+    if (width == 8 && n >= 8) {
+        *(uint4 *)dst = q;
+    } else if (width >= 4 && (n & 3) == 0) {
+        *(uint2 *)dst = make_uint2(q.x, q.y);
+        if (n == 8) *(uint2 *)(dst + 4) = make_uint2(q.z, q.w);
+    } else if (width >= 2 && (n & 1) == 0) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (2 * j < n) *(uint32_t *)(dst + 2 * j) = w[j];
+    } else {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < n) *(uint16_t *)(dst + j) = (uint16_t)(w[j / 2] >> (j & 1) * 16);
+    }
+}
+
 // The sums of this warp's 32 rows, COLS columns from `addr` on, through f(v,
 // col) (32 columns at a time, col from the tile's first), rounded to T and
-// stored at out[(row0 + r) * ld + col0 + c] for r < rows, c < cols: 64 columns
-// at a time pass through the warp's staging memory, so that eight lanes store
-// one row's 128 bytes.  vec: rows start on 16-byte boundaries.  release()
-// hands the tensor memory back once it is read.
+// stored at out[r * ld + c] for r < rows, c < cols: 64 columns at a time pass
+// through the warp's staging memory, so that eight lanes store one row's 128
+// bytes.  width: store_width of the rows.  empty: no products, the sums are
+// 0.  release() hands the tensor memory back once it is read.
 template <class T, int COLS, class F, class R>
-__device__ __forceinline__ void store_tile(const Place &p, uint32_t addr, T *out, int64_t ld, int rows, int cols, bool vec, bool zero, F f, R release) {
-    static_assert(COLS % 32 == 0, "");
-    constexpr int kStep = COLS < 64 ? 32 : 64;      // columns a pass
-    constexpr int kChunks = kStep / 8;              // 16-byte pieces of a row
+__device__ __forceinline__ void store_tile(const Place &p, uint32_t addr, T *out, int64_t ld, int rows, int cols, int width, bool empty, F f, R release) {
+    static_assert(COLS % 64 == 0, "");
 #pragma unroll 1
-    for (int c = 0; c < COLS; c += kStep) {
+    for (int c = 0; c < COLS; c += 64) {
         __syncwarp();
 #pragma unroll
-        for (int h = 0; h < kStep; h += 32) {
+        for (int h = 0; h < 64; h += 32) {
             float v[32];
-            if (zero) {
+            if (empty) {
 #pragma unroll
                 for (int i = 0; i < 32; i++) v[i] = 0.f;
             } else {
@@ -428,24 +469,14 @@ __device__ __forceinline__ void store_tile(const Place &p, uint32_t addr, T *out
                 *(uint4 *)(p.staging + p.lane * 128 + (((h / 8 + i) ^ (p.lane & 7)) * 16)) = q;
             }
         }
-        if (c + kStep >= COLS) release();
+        if (c + 64 >= COLS) release();
         __syncwarp();
-        if (c < cols) {
+        if (c >= cols) continue;
 #pragma unroll
-            for (int i = 0; i < kChunks; i++) {
-                const int r = i * (32 / kChunks) + p.lane / kChunks, ch = p.lane % kChunks, col = c + ch * 8;
-                const uint4 q = *(const uint4 *)(p.staging + r * 128 + ((ch ^ (r & 7)) * 16));
-                if (r >= rows || col >= cols) continue;
-                T *dst = out + (int64_t)r * ld + col;
-                if (vec && col + 8 <= cols) {
-                    *(uint4 *)dst = q;
-                } else {
-                    const T *e = reinterpret_cast<const T *>(&q);
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (col + j < cols) dst[j] = e[j];
-                }
-            }
+        for (int i = 0; i < 8; i++) {
+            const int r = i * 4 + p.lane / 8, ch = p.lane % 8, col = c + ch * 8;
+            if (r < rows && col < cols)
+                store8(out + (int64_t)r * ld + col, *(const uint4 *)(p.staging + r * 128 + ((ch ^ (r & 7)) * 16)), min(cols - col, 8), width);
         }
     }
 }
