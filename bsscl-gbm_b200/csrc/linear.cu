@@ -334,12 +334,13 @@ struct XentStats {
     const int64_t *target;
     float2 *part;
     float *ly;
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+    __device__ int64_t rows(const tc::Tile &t, const tc::Place &p) const { return t.m0 + p.row < t.mend ? target[t.m0 + p.row] : -1; }
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int64_t y, uint32_t addr, R release) const {
         const int row = t.m0 + p.row, c0 = p.half * 128, left = t.nend - t.n0 - c0;    // columns of this half that exist
         const bool in = row < t.mend;
-        const int64_t y = in ? target[row] : -1;
         const int64_t off = y - t.n0 - c0;
         const int yc = off >= 0 && off < min(128, left) ? (int)off : -1;
+        const tc::F2 log2e = tc::f2(kLog2e, kLog2e);
         float m = -INFINITY, s = 0.f;
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
@@ -358,17 +359,22 @@ struct XentStats {
                 for (int i = 0; i < 32; i++)
                     if (c + i >= left) v[i] = -INFINITY;
             }
-            float top[4];
+            float top[4] = {m, v[29], v[30], v[31]};
 #pragma unroll
-            for (int i = 0; i < 4; i++) top[i] = fmaxf(fmaxf(v[i], v[i + 4]), fmaxf(v[i + 8], v[i + 12]));
-#pragma unroll
-            for (int i = 0; i < 4; i++) top[i] = fmaxf(fmaxf(top[i], fmaxf(v[i + 16], v[i + 20])), fmaxf(v[i + 24], v[i + 28]));
-            const float mc = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
+            for (int i = 0; i < 28; i += 2) top[i / 2 % 4] = tc::max3(top[i / 2 % 4], v[i], v[i + 1]);
+            const float mc = fmaxf(tc::max3(top[0], top[1], top[2]), fmaxf(top[3], v[28]));
             const float shift = mc == -INFINITY ? 0.f : mc, z = shift * kLog2e;
-            float e[4] = {s * ex2((m - shift) * kLog2e), 0.f, 0.f, 0.f};
+            const tc::F2 minus = tc::f2(-z, -z);
+            tc::F2 e[4] = {tc::f2(s * ex2((m - shift) * kLog2e), 0.f), tc::f2(0.f, 0.f), tc::f2(0.f, 0.f), tc::f2(0.f, 0.f)};
 #pragma unroll
-            for (int i = 0; i < 32; i++) e[i & 3] += ex2(fmaf(v[i], kLog2e, -z));
-            s = (e[0] + e[1]) + (e[2] + e[3]);
+            for (int i = 0; i < 32; i += 2) {
+                float a, b;
+                tc::f2_out(tc::f2_fma(tc::f2(v[i], v[i + 1]), log2e, minus), a, b);
+                e[i / 2 & 3] = tc::f2_add(e[i / 2 & 3], tc::f2(ex2(a), ex2(b)));
+            }
+            float a, b;
+            tc::f2_out(tc::f2_add(tc::f2_add(e[0], e[1]), tc::f2_add(e[2], e[3])), a, b);
+            s = a + b;
             m = mc;
         }
         if (in) part[((int64_t)(t.n0 / kBN) * 2 + p.half) * dense.m + row] = make_float2(m, s);
@@ -413,25 +419,33 @@ template <class T> struct XentG {
     const float *lse, *grad_loss, *scale;
     T *g;
     int64_t ldg, part;  // row stride; from the leading to the trailing part (0: one part)
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
-        const int row = t.m0 + p.row, h0 = p.half * 128;
-        int64_t y = -1;
-        float c = 0.f, z = 0.f;
-        if (row < t.mend) {
-            y = target[row];
-            if (y >= 0 && y < v) {
-                c = grad_loss[row] * (scale ? *scale : 1.f);
-                z = lse[row] * kLog2e;
-            }
-        }
+    struct Rows {
+        int64_t y;
+        float c, z;
+    };
+    __device__ Rows rows(const tc::Tile &t, const tc::Place &p) const {
+        const int row = t.m0 + p.row;
+        Rows r{-1, 0.f, 0.f};
+        if (row < t.mend) r = {target[row], grad_loss[row] * (scale ? *scale : 1.f), lse[row] * kLog2e};
+        return r;
+    }
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, Rows r, uint32_t addr, R release) const {
+        const int h0 = p.half * 128;
+        const int64_t y = r.y;
+        const float c = r.c, z = r.z;
         const bool has = y >= 0 && y < v, all = __all_sync(~0u, has);
         const int64_t off = y - c0 - t.n0 - h0;
         const int yc = has && off >= 0 && off < 128 ? (int)off : -1;
         const int row0 = t.m0 + p.row - p.lane;
         auto value = [&](float (&x)[32], int col) {
             const bool here = __any_sync(~0u, yc >= col && yc < col + 32);
+            const tc::F2 log2e = tc::f2(kLog2e, kLog2e), minus = tc::f2(-z, -z), cc = tc::f2(c, c);
 #pragma unroll
-            for (int i = 0; i < 32; i++) x[i] = c * ex2(fmaf(x[i], kLog2e, -z));
+            for (int i = 0; i < 32; i += 2) {
+                float a, b;
+                tc::f2_out(tc::f2_fma(tc::f2(x[i], x[i + 1]), log2e, minus), a, b);
+                tc::f2_out(tc::f2_mul(tc::f2(ex2(a), ex2(b)), cc), x[i], x[i + 1]);
+            }
             if (here) {
 #pragma unroll
                 for (int i = 0; i < 32; i++)
@@ -586,7 +600,8 @@ template <class T, int BN> struct XentPair {
     Dense dense[2];
     Sink<T> sink[2];
     int first, laps;
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+    __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const {
         const Dense &g = dense[t.kind];
         sink_tile<BN / 2>(sink[t.kind], g.m, g.splits, t, p, addr, release, (t.m0 / 256) * g.nt + t.n0 / BN);
     }
@@ -840,7 +855,8 @@ template <class T, bool BMN> struct LeafRows {
     T *out;
     int64_t ld;
     int width;
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+    __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const {
         const int row0 = t.m0 + p.row - p.lane, h0 = p.half * 128;
         tc::store_tile<T, 128>(p, addr, out + (int64_t)row0 * ld + t.n0 + h0, ld, t.mend - row0, t.nend - t.n0 - h0, width, false, [](float (&)[32], int) {}, release);
     }
@@ -886,7 +902,8 @@ template <class T> struct LeafDw {
     int32_t groups;
     int splits, mt, nt;
     Sink<T> sink;       // of the (groups * dout) x din matrix of all leaves' dw
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
+    __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const {
         // the leaf's tile as one of that matrix
         tc::Tile all = t;
         const int g = t.aux % groups, base = g * (int)dout;

@@ -56,31 +56,46 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// arrive on the same barrier of the cluster's CTA `rank`
-__device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
-    asm volatile(
-        "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n"
-        " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}" ::"r"(bar), "r"(rank)
-        : "memory");
+// Arrive on the same barrier of the cluster's CTA `rank`.  DATA: with writes
+// to shared memory that the other side is to see; tensor memory has its own fences.
+template <bool DATA> __device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
+    if (DATA)
+        asm volatile(
+            "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n"
+            " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}" ::"r"(bar), "r"(rank)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n"
+            " mbarrier.arrive.shared::cluster.b64 _, [r];\n}" ::"r"(bar), "r"(rank)
+            : "memory");
 }
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+template <bool DATA> __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        " selp.b32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
+    if (DATA)
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+            " selp.b32 %0, 1, 0, p;\n}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            " selp.b32 %0, 1, 0, p;\n}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
     return ok;
 }
 // Waits for the phase of this parity; false when the wait ran out here or in another warp of the CTA.
 // Called by whole warps, whose lanes all get the same answer.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead) {
-    bool ok = mbar_try(bar, parity);
+template <bool DATA = false> __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead) {
+    bool ok = mbar_try<DATA>(bar, parity);
     if (__all_sync(~0u, ok)) return true;
     const long long t0 = clock64();
     for (uint32_t i = 1; !ok; i++) {
-        ok = mbar_try(bar, parity);
+        ok = mbar_try<DATA>(bar, parity);
         if ((i & 31) == 0 && !ok) {
             if (*dead) break;
             if (clock64() - t0 > kWaitClocks) {
@@ -164,6 +179,37 @@ __device__ __forceinline__ void tmem_wait(float *v) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; i++) asm volatile("" : "+f"(v[i]));
+}
+
+// Two f32 operations at a time.
+struct F2 {
+    uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_out(F2 x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 // kind::f16: sums in f32; A and B bf16 (1) or f16 (0); M = 256, N = BN;
@@ -312,7 +358,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                         for (int i = t.tail * 8 + lane; i < 64 * 8; i += 32) *(uint4 *)(st + box * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_at(fixed + 8 * s, 0);
+                    if (lane == 0) mbar_arrive_at<true>(fixed + 8 * s, 0);
                 }
                 __syncwarp();
                 if (++s == S::kStages) s = 0, ph ^= 1;
@@ -341,7 +387,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                         break;
                     }
                     if (Op::kTail && t.tail && k == t.nkb - 1) {
-                        if (!mbar_wait(fixed + 8 * s, fixed_ph >> s & 1, dead)) {
+                        if (!mbar_wait<true>(fixed + 8 * s, fixed_ph >> s & 1, dead)) {
                             ok = false;
                             break;
                         }
@@ -380,13 +426,14 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         Tile t;
         while (it.next(op, t)) {
             const int buf = n & 1;
+            const auto rows = op.rows(t, p);     // the rows' scalars, on their way while the products run
             if (!mbar_wait(tfull + 8 * buf, (n >> 1) & 1, dead)) break;
             n++;
             fence_after();
-            op.epilogue(t, p, tmem + buf * BN + ((uint32_t)(p.sub * 32) << 16) + p.half * (BN / 2), [&] {
+            op.epilogue(t, p, rows, tmem + buf * BN + ((uint32_t)(p.sub * 32) << 16) + p.half * (BN / 2), [&] {
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_at(tempty + 8 * buf, 0);
+                if (lane == 0) mbar_arrive_at<false>(tempty + 8 * buf, 0);
             });
         }
     }
