@@ -334,6 +334,7 @@ struct XentStats {
     const int64_t *target;
     float2 *part;
     float *ly;
+    __device__ void finish(int, int, int) const {}
     __device__ int64_t rows(const tc::Tile &t, const tc::Place &p) const { return t.m0 + p.row < t.mend ? target[t.m0 + p.row] : -1; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int64_t y, uint32_t addr, R release) const {
         const int row = t.m0 + p.row, c0 = p.half * 128, left = t.nend - t.n0 - c0;    // columns of this half that exist
@@ -423,6 +424,7 @@ template <class T> struct XentG {
         int64_t y;
         float c, z;
     };
+    __device__ void finish(int, int, int) const {}
     __device__ Rows rows(const tc::Tile &t, const tc::Place &p) const {
         const int row = t.m0 + p.row;
         Rows r{-1, 0.f, 0.f};
@@ -582,9 +584,8 @@ __device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, c
 template <class T, int BN> struct XentPair {
     static constexpr int kBN = BN;
     static constexpr bool kAMN = false, kBMN = true, kTail = false, kDual = true;
-    struct Iter {
-        uint32_t at, step;
-        __device__ Iter(const XentPair &, int cid, int ncl) : at(cid), step(ncl) {}
+    struct Iter : tc::Snake {
+        __device__ Iter(const XentPair &, int cid, int ncl) : tc::Snake(cid, ncl) {}
         __device__ bool next(const XentPair &op, tc::Tile &t) {
             const uint32_t u0 = (uint32_t)(op.dense[0].mt * op.dense[0].nt) * op.dense[0].splits,
                            u1 = (uint32_t)(op.dense[1].mt * op.dense[1].nt) * op.dense[1].splits;
@@ -593,13 +594,14 @@ template <class T, int BN> struct XentPair {
             const uint32_t i = op.first ? (kind ? at : at - u1) : (kind ? at - u0 : at);
             op.dense[kind].template place<BN>(i, t);
             t.kind = kind;
-            at += step;
+            step();
             return true;
         }
     };
     Dense dense[2];
     Sink<T> sink[2];
     int first, laps;
+    __device__ void finish(int, int, int) const {}
     __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const {
         const Dense &g = dense[t.kind];
@@ -607,21 +609,36 @@ template <class T, int BN> struct XentPair {
     }
 };
 
-// Parts of the k axis for a product of `tiles` tiles and `nkb` stages: as many
-// as make the longest chain of stages one cluster works through shortest,
-// counting about 8 stages' time for a tile's start and end and the time the
-// f32 sums take to be written and read again (512 KB a tile of 256 x 256,
-// 0.08 us at the memory's rate: 0.3 of a stage's 0.27 us).
-int choose_splits(int64_t tiles, int64_t nkb) {
+// Time, in stages of 0.27 us, in which 74 clusters work through u0 units of l0
+// stages and then u1 units of l1 <= l0, dealt out back and forth: the longest
+// cluster's, counting about 8 stages for a unit's start and end.
+double chain(int64_t u0, int64_t l0, int64_t u1, int64_t l1) {
     constexpr int64_t kClusters = 74;      // 148 SMs; fixed, so that sizes alone set the workspace
-    int best = 1;
+    l0 += 8;
+    l1 += 8;
+    const int64_t all = (u0 * l0 + u1 * l1 + kClusters - 1) / kClusters, waves = (u0 + u1 + kClusters - 1) / kClusters,
+                  r0 = (u0 + kClusters - 1) / kClusters;
+    // at least the mean; a cluster of the fullest wave, which holds as many long units as fit
+    return (double)std::max(all, std::min(r0, waves) * l0 + (waves - std::min(r0, waves)) * l1);
+}
+
+// Parts of both products' k axes (tx tiles of kx stages, tw of kw): those that
+// end first.  Split sums cost a launch's worth of waits and the time the f32
+// sums take to be written and read again (512 KB a tile, 0.08 us at the
+// memory's rate: 0.3 of a stage).
+void choose_splits(int64_t tx, int64_t kx, int64_t tw, int64_t kw, int &sx, int &sw) {
+    static constexpr int kTry[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
     double least = 1e300;
-    for (int s = 1; s <= 32 && s <= nkb; s++) {
-        const int64_t waves = (tiles * s + kClusters - 1) / kClusters;
-        const double t = (double)waves * ((nkb + s - 1) / s + 8) + (s > 1 ? 8.0 + tiles * s * 0.3 : 0.0);
-        if (t < least * 0.98) least = t, best = s;
+    for (int a : kTry) {
+        if (a > 1 && (a > kx || !tx)) break;
+        for (int b : kTry) {
+            if (b > 1 && (b > kw || !tw)) break;
+            const int64_t la = (kx + a - 1) / a, lb = (kw + b - 1) / b;
+            double t = la >= lb ? chain(tx * a, la, tw * b, lb) : chain(tw * b, lb, tx * a, la);
+            t += (a > 1 ? 4 + tx * a * 0.3 : 0) + (b > 1 ? 4 + tw * b * 0.3 : 0);
+            if (t < least * 0.98) least = t, sx = a, sw = b;
+        }
     }
-    return best;
 }
 
 // How the gradient's work is cut: pieces of classes whose G takes at most
@@ -652,8 +669,7 @@ struct XentPlan {
         const int64_t dt = (d + bn - 1) / bn;
         tx = (n + 255) / 256 * dt;
         tw = (pc + 255) / 256 * dt;
-        sx = choose_splits(tx, (pc + 63) / 64 * parts);
-        sw = choose_splits(tw, (n + 63) / 64 * parts);
+        choose_splits(tx, (pc + 63) / 64 * parts, tw, (n + 63) / 64 * parts, sx, sw);
     }
     bool dx_acc() const { return pieces > 1 || sx > 1; }
     int64_t tickets() const { return 16 * (tx + tw * pieces); }
@@ -843,96 +859,139 @@ struct LeafIter {
     }
 };
 
-// y = x w^T (B K-major) or dx = dy w (B's n axis contiguous), leaf by leaf.
-// Rows behind a leaf's last one belong to the next leaf: they are
-// computed with this leaf's weights and not stored.
-template <class T, bool BMN> struct LeafRows {
-    static constexpr int kBN = 256;
-    static constexpr bool kAMN = false, kBMN = BMN, kTail = false, kDual = false;
-    static constexpr int laps = 1;
-    using Iter = LeafIter;
-    Leaves leaves;
+// Zeros in the rows before the first leaf and behind the last one, a warp a row.
+template <class T> __device__ void leaf_rest(const Leaves &l, T *out, int64_t ld, int warp, int warps, int lane) {
+    const int64_t lo = min(max((int64_t)l.off[0], (int64_t)0), l.t), hi = max(min((int64_t)l.off[l.groups], l.t), lo), rest = lo + (l.t - hi);
+    for (int64_t r = warp; r < rest; r += warps) {
+        T *row = out + (r < lo ? r : hi + r - lo) * ld;
+        for (int64_t c = lane; c < l.n; c += 32) row[c] = from_f<T>(0.f);
+    }
+}
+
+// One 256 x 256 tile of leaf's rows times its weights.  Rows behind a leaf's last one belong to the next
+// leaf: they are computed with this leaf's weights and not stored.
+template <class T> struct LeafOut {
     T *out;
     int64_t ld;
-    int width;
-    __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const {
+    int width, rest;
+    template <class R> __device__ void store(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
         const int row0 = t.m0 + p.row - p.lane, h0 = p.half * 128;
         tc::store_tile<T, 128>(p, addr, out + (int64_t)row0 * ld + t.n0 + h0, ld, t.mend - row0, t.nend - t.n0 - h0, width, false, [](float (&)[32], int) {}, release);
     }
 };
 
-// dw: one 256 x 256 tile of one leaf (and one part of its rows) a unit; the k
-// axis is the leaf's rows.
-struct LeafDwIter {
-    uint32_t at, step;
-    template <class Op> __device__ LeafDwIter(const Op &, int cid, int ncl) : at(cid), step(ncl) {}
-    template <class Op> __device__ bool next(const Op &op, tc::Tile &t) {
-        const uint32_t tiles = op.mt * op.nt, per = tiles * op.splits;
-        if (at >= per * op.groups) return false;
-        const uint32_t g = at / per, i = at - g * per, part = op.splits > 1 ? i / tiles : 0, tile = i - part * tiles, tm = tile / op.nt, tn = tile - tm * op.nt;
-        int lo, hi;
-        leaf_rows(op.off, g, op.t, lo, hi);
-        const int nkb = (hi - lo + 63) / 64, each = op.splits > 1 ? (nkb + op.splits - 1) / op.splits : nkb, k0 = min((int)part * each, nkb),
-                  k1 = min(k0 + each, nkb);
-        t.m0 = t.am = (int)tm * 256;
-        t.n0 = (int)tn * 256;
-        t.mend = min((int)op.dout - t.m0, 256) + t.m0;
-        t.nend = min((int)op.din - t.n0, 256) + t.n0;
-        t.k0 = lo;
-        t.q0 = k0;
-        t.nkb = k1 - k0;
-        t.bz = 0;
-        t.kind = 0;
-        // behind the last row of all TMA fills zeros
-        t.tail = k1 == nkb && hi < op.t ? (hi - lo) % 64 : 0;
-        t.aux = (int)(part * op.groups + g);
-        at += step;
-        return true;
-    }
-};
-
-template <class T> struct LeafDw {
+// y = x w^T, leaf by leaf.
+template <class T> struct LeafRows {
     static constexpr int kBN = 256;
-    static constexpr bool kAMN = true, kBMN = true, kTail = true, kDual = false;
+    static constexpr bool kAMN = false, kBMN = false, kTail = false, kDual = false;
     static constexpr int laps = 1;
-    using Iter = LeafDwIter;
-    const int32_t *off;
-    int64_t t, din, dout;
-    int32_t groups;
-    int splits, mt, nt;
-    Sink<T> sink;       // of the (groups * dout) x din matrix of all leaves' dw
-    __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const {
-        // the leaf's tile as one of that matrix
-        tc::Tile all = t;
-        const int g = t.aux % groups, base = g * (int)dout;
-        all.m0 += base;
-        all.mend += base;
-        all.aux = t.aux / groups;
-        sink_tile<128>(sink, groups * (int)dout, splits, all, p, addr, release, (g * mt + t.m0 / 256) * nt + t.n0 / 256);
+    using Iter = LeafIter;
+    Leaves leaves;
+    LeafOut<T> y;
+    __device__ void finish(int warp, int warps, int lane) const {
+        if (y.rest) leaf_rest(leaves, y.out, y.ld, warp, warps, lane);
     }
+    __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const { y.store(t, p, addr, release); }
 };
 
-// The rows before the first leaf and behind the last one as zeros.
-template <class T> __global__ void k_leaf_rest(const int32_t *off, int32_t groups, int64_t t, int64_t cols, T *y, int64_t ldy) {
+// The leaves in order of their rows, longest first, for the tiles of dw.
+constexpr int kSortLeaves = 2048;
+
+__global__ void __launch_bounds__(1024) k_leaf_order(const int32_t *__restrict__ off, int32_t groups, int64_t t, int32_t *__restrict__ order) {
     tc::depend();
-    const int64_t lo = min(max((int64_t)off[0], (int64_t)0), t), hi = max(min((int64_t)off[groups], t), lo);
-    const int64_t rest = lo + (t - hi);
-    for (int64_t r = blockIdx.x; r < rest; r += gridDim.x) {
-        T *row = y + (r < lo ? r : hi + r - lo) * ldy;
-        for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) row[c] = from_f<T>(0.f);
+    __shared__ int rows[kSortLeaves];
+    for (int g = threadIdx.x; g < groups; g += 1024) {
+        int lo, hi;
+        leaf_rows(off, g, t, lo, hi);
+        rows[g] = hi - lo;
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < groups; g += 1024) {
+        const int mine = rows[g];
+        int before = 0;
+        for (int k = 0; k < groups; k++) before += rows[k] > mine || (rows[k] == mine && k < g);
+        order[before] = g;
     }
 }
 
+// dw = dy^T x and dx = dy w of all leaves as one pool of units: first dw's
+// tiles (of one leaf and one part of its rows, the k axis; longest leaf
+// first), then dx's, all of the same short k axis.
+template <class T> struct LeafPair {
+    static constexpr int kBN = 256;
+    static constexpr bool kAMN = false, kBMN = true, kTail = true, kDual = true;
+    static constexpr int laps = 1;
+    struct Iter : tc::Snake {
+        LeafIter dx;
+        __device__ Iter(const LeafPair &op, int cid, int ncl) : tc::Snake(cid, ncl), dx(op, 0, 0) {}
+        __device__ bool next(const LeafPair &op, tc::Tile &t) {
+            const uint32_t tiles = op.mt * op.nt, per = tiles * op.splits, first = op.sink.out ? per * op.leaves.groups : 0;
+            if (at >= first) {
+                if (!op.dx.out) return false;
+                dx.at = at - first;
+                step();
+                return dx.next(op, t);
+            }
+            const uint32_t k = at / per, i = at - k * per, part = op.splits > 1 ? i / tiles : 0, tile = i - part * tiles, tm = tile / op.nt,
+                           tn = tile - tm * op.nt;
+            const int g = op.order ? op.order[k] : (int)k;
+            int lo, hi;
+            leaf_rows(op.leaves.off, g, op.leaves.t, lo, hi);
+            const int nkb = (hi - lo + 63) / 64, each = op.splits > 1 ? (nkb + op.splits - 1) / op.splits : nkb, k0 = min((int)part * each, nkb),
+                      k1 = min(k0 + each, nkb);
+            t.m0 = t.am = (int)tm * 256;
+            t.n0 = (int)tn * 256;
+            t.mend = min(op.dout - t.m0, 256) + t.m0;
+            t.nend = min(op.leaves.n - t.n0, 256) + t.n0;
+            t.k0 = lo;
+            t.q0 = k0;
+            t.nkb = k1 - k0;
+            t.bz = 0;
+            t.kind = 1;
+            // behind the last row of all TMA fills zeros
+            t.tail = k1 == nkb && hi < op.leaves.t ? (hi - lo) % 64 : 0;
+            t.aux = (int)(part * op.leaves.groups + g);
+            step();
+            return true;
+        }
+    };
+    Leaves leaves;         // of dx: its columns are dw's too
+    LeafOut<T> dx;         // out null: not wanted
+    const int32_t *order;  // of the leaves (null: as they are)
+    int dout, splits, mt, nt;
+    Sink<T> sink;          // of the (groups * dout) x din matrix of all leaves' dw; out null: not wanted
+    __device__ void finish(int warp, int warps, int lane) const {
+        if (dx.out && dx.rest) leaf_rest(leaves, dx.out, dx.ld, warp, warps, lane);
+    }
+    __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const {
+        if (!t.kind) {
+            dx.store(t, p, addr, release);
+            return;
+        }
+        // the leaf's tile as one of that matrix
+        tc::Tile all = t;
+        const int g = t.aux % leaves.groups, base = g * dout;
+        all.m0 += base;
+        all.mend += base;
+        all.aux = t.aux / leaves.groups;
+        sink_tile<128>(sink, leaves.groups * dout, splits, all, p, addr, release, (g * mt + t.m0 / 256) * nt + t.n0 / 256);
+    }
+};
+
+// Parts of dw's k axis, as if all leaves were alike.
 int leaf_splits(int64_t t, int32_t groups, int64_t din, int64_t dout) {
-    return choose_splits((int64_t)groups * ((din + 255) / 256) * ((dout + 255) / 256), (t / groups + 63) / 64);
+    int none = 1, s = 1;
+    choose_splits(0, 0, (int64_t)groups * ((din + 255) / 256) * ((dout + 255) / 256), (t / groups + 63) / 64, none, s);
+    return s;
 }
 
 struct LeafWs {
     uint16_t *x, *w, *dy;
     float *acc;
     uint32_t *tickets;
+    int32_t *order;
     int64_t ldacc, n_tickets, bytes;
     LeafWs(void *ws, int64_t t, int32_t groups, int64_t din, int64_t dout, bool grad, bool in_place) {
         Room r(ws);
@@ -945,20 +1004,10 @@ struct LeafWs {
         acc = r.take<float>(s > 1 ? s * groups * dout * ldacc : 0);
         n_tickets = s > 1 ? 16 * groups * ((din + 255) / 256) * ((dout + 255) / 256) : 0;
         tickets = r.take<uint32_t>(n_tickets);
+        order = r.take<int32_t>(grad ? groups : 0);
         bytes = r.bytes();
     }
 };
-
-template <class T, bool BMN>
-Err leaf_rows_launch(const View &a, const View &w, const int32_t *off, int64_t t, int32_t groups, int64_t k, int64_t n, T *y, int64_t ldy, bool zero_rest,
-                     cudaStream_t st) {
-    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    LeafRows<T, BMN> op{Leaves(off, t, groups, k, n), y, ldy, tc::store_width(y, ldy)};
-    const View views[2] = {a, w};
-    Err e = launch(views, op, bf16, op.leaves.units(), st);
-    if (!e.bad() && zero_rest) e = start(k_leaf_rest<T>, std::min<int64_t>(t, sm_count()), 256, 0, st, off, groups, t, n, y, ldy);
-    return e;
-}
 
 template <class T>
 Err leaf_forward(const void *x, int64_t ldx, const void *w, const int32_t *off, int64_t t, int32_t groups, int64_t din, int64_t dout, T *y, int64_t ldy,
@@ -967,7 +1016,11 @@ Err leaf_forward(const void *x, int64_t ldx, const void *w, const int32_t *off, 
     Prep prep;
     const View a = readable(prep, {x, din, t, ldx}, q.x), b = readable(prep, {w, din, dout, din, groups}, q.w);
     Err e = run_prep(prep, st);
-    return e.bad() ? e : leaf_rows_launch<T, false>(a, b, off, t, groups, din, dout, y, ldy, zero_rest, st);
+    if (e.bad()) return e;
+    LeafRows<T> op{Leaves(off, t, groups, din, dout), {y, ldy, tc::store_width(y, ldy), zero_rest}};
+    const View views[2] = {a, b};
+    // a cluster at least for the rows outside the leaves
+    return launch(views, op, std::is_same<T, __nv_bfloat16>::value, op.leaves.units(), st);
 }
 
 template <class T>
@@ -990,13 +1043,26 @@ Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off,
         prep.n_tickets = (int)q.n_tickets;
     }
     Err e = run_prep(prep, st);
-    if (dx && !e.bad()) e = leaf_rows_launch<T, true>(g, b, off, t, groups, dout, din, dx, lddx, zero_rest, st);
-    if (!dw || e.bad()) return e;
     const int s = leaf_splits(t, groups, din, dout), mt = (int)((dout + 255) / 256), nt = (int)((din + 255) / 256);
-    LeafDw<T> op{off, t, din, dout, groups, s, mt, nt,
-                 {nullptr, 0, nullptr, dw, din, tc::store_width(dw, din), s > 1 ? q.acc : nullptr, q.ldacc, false, true, q.tickets}};
-    const View views[2] = {g, a};
-    return launch(views, op, bf16, (int64_t)groups * s * mt * nt, st);
+    LeafPair<T> op{Leaves(off, t, groups, dout, din), {}, nullptr, (int)dout, s, mt, nt, {}};
+    int64_t units = 0;
+    if (dx) {
+        op.dx = {dx, lddx, tc::store_width(dx, lddx), zero_rest};
+        units += op.leaves.units();
+    }
+    if (dw) {
+        const int64_t own = (int64_t)groups * s * mt * nt;
+        // more units than clusters: their order decides how evenly the clusters end
+        if (own > sm_count() / 2 && groups > 1 && groups <= kSortLeaves && !e.bad()) {
+            e = start(k_leaf_order, 1, 1024, 0, st, off, groups, t, q.order);
+            op.order = q.order;
+        }
+        op.sink = {nullptr, 0, nullptr, dw, din, tc::store_width(dw, din), s > 1 ? q.acc : nullptr, q.ldacc, false, true, q.tickets};
+        units += own;
+    }
+    if (e.bad()) return e;
+    const View views[4] = {g, dx ? b : a, g, dw ? a : b};
+    return launch(views, op, bf16, units, st);
 }
 
 // ---------------------------------------------------------------------------

@@ -243,6 +243,18 @@ struct Tile {
     int kind;         // which of a launch's two products
     int aux;
 };
+// The units of cluster c of C: c, 2C - 1 - c, 2C + c, 4C - 1 - c, ... so that of units
+// in order of length each cluster gets as many long ones as the others.
+struct Snake {
+    uint32_t at, up, down;
+    __device__ Snake(int c, int n) : at(c), up(2 * (n - 1 - c) + 1), down(2 * c + 1) {}
+    __device__ void step() {
+        at += up;
+        const uint32_t u = up;
+        up = down;
+        down = u;
+    }
+};
 // The operands' maps: A and B of the first product, A and B of the second.
 struct Maps {
     alignas(64) CUtensorMap m[4];
@@ -436,6 +448,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                 if (lane == 0) mbar_arrive_at<false>(tempty + 8 * buf, 0);
             });
         }
+        op.finish((warp - 2) + kEpiWarps * (int)blockIdx.x, kEpiWarps * (int)gridDim.x, lane);
     }
     __syncwarp();
     if (*dead)
