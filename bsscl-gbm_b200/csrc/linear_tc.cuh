@@ -89,22 +89,24 @@ template <bool DATA> __device__ __forceinline__ bool mbar_try(uint32_t bar, uint
     return ok;
 }
 // Waits for the phase of this parity; false when the wait ran out here or in another warp of the CTA.
-// Called by whole warps, whose lanes all get the same answer.
 template <bool DATA = false> __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead) {
-    bool ok = mbar_try<DATA>(bar, parity);
-    if (__all_sync(~0u, ok)) return true;
+    if (mbar_try<DATA>(bar, parity)) return true;
     const long long t0 = clock64();
-    for (uint32_t i = 1; !ok; i++) {
-        ok = mbar_try<DATA>(bar, parity);
-        if ((i & 31) == 0 && !ok) {
-            if (*dead) break;
+    for (uint32_t i = 1;; i++) {
+        if (mbar_try<DATA>(bar, parity)) return true;
+        if ((i & 31) == 0) {
+            if (*dead) return false;
             if (clock64() - t0 > kWaitClocks) {
                 *dead = 1;
                 g_ops_timeout = 1;
-                break;
+                return false;
             }
         }
     }
+}
+// The same for a whole warp, whose lanes all get the same answer.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *dead) {
+    const bool ok = mbar_wait(bar, parity, dead);
     return __all_sync(~0u, ok);
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -267,6 +269,85 @@ struct Place {
     uint8_t *staging;    // 4096 bytes of this warp's own
 };
 
+// A place among the stages, and its barriers' parity.
+template <int N> struct Ring {
+    int s = 0;
+    uint32_t ph = 0;
+    __device__ void step() {
+        if (++s == N) s = 0, ph ^= 1;
+    }
+    __device__ void skip(int n) {
+        const uint32_t to = s + n;
+        ph ^= to / N & 1;
+        s = to % N;
+    }
+};
+
+// One stage of both operands into shared memory at `a`: boxes of 64 values of
+// k x 128 (BN/2) rows, or where the m (n) axis is contiguous 64 of its values x 64 of k.
+template <class Op, bool AMN, bool PAIR>
+__device__ __forceinline__ void load_stage(const CUtensorMap *maps, uint32_t a, uint32_t bar, int am, int bn, int at, int az, int bz) {
+    constexpr int BN = Op::kBN;
+    auto load = [&](uint32_t dst, const CUtensorMap *m, int x, int y, int z) {
+        if (PAIR)
+            tma_pair(dst, m, bar, x, y, z);
+        else
+            tma_own(dst, m, bar, x, y, z);
+    };
+    if (AMN) {
+        load(a, maps, am, at, az);
+        load(a + 8192, maps, am + 64, at, az);
+    } else {
+        load(a, maps, at, am, az);
+    }
+    const uint32_t b = a + kABytes;
+    if (Op::kBMN) {
+#pragma unroll
+        for (int j = 0; j < BN / 2; j += 64) load(b + j * 128, maps + 1, bn + j, at, bz);
+    } else {
+        load(b, maps + 1, at, bn, bz);
+    }
+}
+
+template <class Op, bool AMN>
+__device__ __forceinline__ bool fetch(const Op &op, const CUtensorMap *maps, const Tile &t, int n, Ring<Shape<Op::kBN>::kStages> r, uint32_t stages, uint32_t full,
+                                      uint32_t empty, uint32_t rank, volatile int *dead) {
+    using S = Shape<Op::kBN>;
+    const int am = t.am + (int)rank * 128, bn = t.n0 + (int)rank * (Op::kBN / 2);
+    const bool two = op.laps == 2;
+    for (int q = t.q0; q < t.q0 + n; q++) {
+        if (!mbar_wait(empty + 8 * r.s, r.ph ^ 1, dead)) return false;
+        const uint32_t bar = full + 8 * r.s;
+        if (rank == 0) mbar_expect(bar, 2 * S::kStage);
+        load_stage<Op, AMN, true>(maps, stages + r.s * S::kStage, bar, am, bn, t.k0 + (two ? q >> 1 : q) * kBK, two ? q & 1 : 0, t.bz);
+        r.step();
+    }
+    return true;
+}
+
+template <class Op, bool AMN> __device__ __forceinline__ void multiply_stage(uint32_t d, uint32_t a, uint32_t idesc, bool add) {
+    uint64_t da = make_desc<AMN>(a), db = make_desc<Op::kBMN>(a + kABytes);
+#pragma unroll
+    for (int j = 0; j < kBK / 16; j++) {
+        mma_pair(d, da, db, idesc | (uint32_t)AMN << 15, add || j > 0);
+        da += kKStep<AMN>;
+        db += kKStep<Op::kBMN>;
+    }
+}
+
+template <class Op, bool AMN>
+__device__ __forceinline__ bool multiply(uint32_t d, int n, Ring<Shape<Op::kBN>::kStages> &r, uint32_t stages, uint32_t full, uint32_t empty, uint32_t idesc,
+                                         volatile int *dead) {
+    for (int k = 0; k < n; k++) {
+        if (!mbar_wait(full + 8 * r.s, r.ph, dead)) return false;
+        fence_after();
+        multiply_stage<Op, AMN>(d, stages + r.s * Shape<Op::kBN>::kStage, idesc, k > 0);
+        commit_pair(empty + 8 * r.s);
+        r.step();
+    }
+    return true;
+}
+
 template <class Op>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uint32_t idesc) {
@@ -314,114 +395,71 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     depend();
 
     if (warp == 0) {
-        // ---- fetch
-        int s = 0;
-        uint32_t ph = 0, tail_ph = 0;
+        // ---- fetch: one thread runs a tile's stages (a stage has 512 clocks)
+        Ring<S::kStages> r;
+        uint32_t tail_ph = 0;
         typename Op::Iter it(op, cid, ncl);
         Tile t;
-        bool ok = true;
-        while (ok && it.next(op, t)) {
-            for (int k = 0; k < t.nkb; k++) {
-                if (!mbar_wait(empty + 8 * s, ph ^ 1, dead)) {
-                    ok = false;
-                    break;
-                }
-                const bool tail = Op::kTail && t.tail && k == t.nkb - 1;
-                const uint32_t a = stages + s * S::kStage, b = a + kABytes;
-                if (lane == 0) {
-                    const uint32_t bar = tail ? tailbar : full + 8 * s;
-                    if (tail) {
-                        mbar_expect(tailbar, S::kStage);
-                        if (rank == 0) mbar_arrive(full + 8 * s);
-                    } else if (rank == 0) {
-                        mbar_expect(full + 8 * s, 2 * S::kStage);
-                    }
-                    auto load = [&](uint32_t dst, const CUtensorMap *m, int x, int y, int z) {
-                        if (tail)
-                            tma_own(dst, m, bar, x, y, z);
-                        else
-                            tma_pair(dst, m, bar, x, y, z);
-                    };
-                    const CUtensorMap *ma = &maps.m[Op::kDual ? 2 * t.kind : 0], *mb = ma + 1;
-                    const int q = t.q0 + k, z = op.laps == 2 ? q & 1 : 0, at = t.k0 + (op.laps == 2 ? q >> 1 : q) * kBK;
-                    const int am = t.am + (int)rank * 128, bn = t.n0 + (int)rank * (BN / 2);
-                    if (Op::kDual ? t.kind == 1 : Op::kAMN) {
-                        load(a, ma, am, at, z);
-                        load(a + 8192, ma, am + 64, at, z);
-                    } else {
-                        load(a, ma, at, am, z);
-                    }
-                    if (Op::kBMN) {
-#pragma unroll
-                        for (int j = 0; j < BN / 2; j += 64) load(b + j * 128, mb, bn + j, at, t.bz);
-                    } else {
-                        load(b, mb, at, bn, t.bz);
-                    }
-                }
-                if (tail) {
-                    // rows of k behind the axis' end belong to the next leaf: zeros in their place
-                    if (!mbar_wait(tailbar, tail_ph, dead)) {
-                        ok = false;
-                        break;
-                    }
-                    tail_ph ^= 1;
-                    uint8_t *st = base + s * S::kStage;
-                    for (int box = 0; box < S::kStage / 8192; box++)
-                        for (int i = t.tail * 8 + lane; i < 64 * 8; i += 32) *(uint4 *)(st + box * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_at<true>(fixed + 8 * s, 0);
-                }
-                __syncwarp();
-                if (++s == S::kStages) s = 0, ph ^= 1;
+        while (it.next(op, t)) {
+            const bool tail = Op::kTail && t.tail && t.nkb;
+            const int n = t.nkb - tail;
+            bool ok = true;
+            if (lane == 0)
+                ok = Op::kDual && t.kind == 1 ? fetch<Op, true>(op, maps.m + 2, t, n, r, stages, full, empty, rank, dead)
+                                              : fetch<Op, Op::kAMN>(op, maps.m, t, n, r, stages, full, empty, rank, dead);
+            if (!__shfl_sync(~0u, ok, 0)) break;
+            r.skip(n);
+            if (!tail) continue;
+            // The last stage: rows of k behind the axis' end belong to the
+            // next leaf; zeros take their place before the products see them.
+            if (!mbar_wait_warp(empty + 8 * r.s, r.ph ^ 1, dead)) break;
+            if (lane == 0) {
+                mbar_expect(tailbar, S::kStage);
+                if (rank == 0) mbar_arrive(full + 8 * r.s);
+                load_stage<Op, true, false>(Op::kDual ? maps.m + 2 : maps.m, stages + r.s * S::kStage, tailbar, t.am + (int)rank * 128,
+                                            t.n0 + (int)rank * (BN / 2), t.k0 + (t.q0 + n) * kBK, 0, t.bz);
             }
+            if (!mbar_wait_warp(tailbar, tail_ph, dead)) break;
+            tail_ph ^= 1;
+            uint8_t *st = base + r.s * S::kStage;
+            for (int box = 0; box < S::kStage / 8192; box++)
+                for (int i = t.tail * 8 + lane; i < 64 * 8; i += 32) *(uint4 *)(st + box * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at<true>(fixed + 8 * r.s, 0);
+            r.skip(1);
         }
     } else if (warp == 1) {
-        // ---- products
+        // ---- products, issued by one thread too
         if (rank == 0) {
-            int s = 0, n = 0;
-            uint32_t ph = 0, fixed_ph = 0;
+            Ring<S::kStages> r;
+            int n = 0;
+            uint32_t fixed_ph = 0;
             typename Op::Iter it(op, cid, ncl);
             Tile t;
-            bool ok = true;
-            while (ok && it.next(op, t)) {
+            while (it.next(op, t)) {
                 const int buf = n & 1;
-                if (!mbar_wait(tempty + 8 * buf, ((n >> 1) & 1) ^ 1, dead)) break;
-                n++;
-                fence_after();
-                const uint32_t d = tmem + buf * BN;
-                const bool amn = Op::kDual ? t.kind == 1 : Op::kAMN;
-                const uint32_t id = idesc | (uint32_t)amn << 15;
-                const uint64_t astep = amn ? kKStep<true> : kKStep<false>;
-                for (int k = 0; k < t.nkb; k++) {
-                    if (!mbar_wait(full + 8 * s, ph, dead)) {
-                        ok = false;
-                        break;
-                    }
-                    if (Op::kTail && t.tail && k == t.nkb - 1) {
-                        if (!mbar_wait<true>(fixed + 8 * s, fixed_ph >> s & 1, dead)) {
-                            ok = false;
-                            break;
-                        }
-                        fixed_ph ^= 1u << s;
-                    }
+                bool ok = true;
+                if (lane == 0) {
+                    const bool tail = Op::kTail && t.tail && t.nkb, second = Op::kDual && t.kind == 1;
+                    ok = mbar_wait(tempty + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
                     fence_after();
-                    if (lane == 0) {
-                        const uint32_t a = stages + s * S::kStage, b = a + kABytes;
-                        uint64_t da = amn ? make_desc<true>(a) : make_desc<false>(a), db = make_desc<Op::kBMN>(b);
-#pragma unroll
-                        for (int j = 0; j < kBK / 16; j++) {
-                            mma_pair(d, da, db, id, k > 0 || j > 0);
-                            da += astep;
-                            db += kKStep<Op::kBMN>;
-                        }
-                        commit_pair(empty + 8 * s);
+                    const uint32_t d = tmem + buf * BN;
+                    Ring<S::kStages> q = r;
+                    if (ok)
+                        ok = second ? multiply<Op, true>(d, t.nkb - tail, q, stages, full, empty, idesc, dead)
+                                    : multiply<Op, Op::kAMN>(d, t.nkb - tail, q, stages, full, empty, idesc, dead);
+                    if (ok && tail) {
+                        ok = mbar_wait(full + 8 * q.s, q.ph, dead) && mbar_wait<true>(fixed + 8 * q.s, fixed_ph >> q.s & 1, dead);
+                        fence_after();
+                        if (ok) multiply_stage<Op, true>(d, stages + q.s * S::kStage, idesc, t.nkb > 1), commit_pair(empty + 8 * q.s);
+                        fixed_ph ^= 1u << q.s;
                     }
-                    __syncwarp();
-                    if (++s == S::kStages) s = 0, ph ^= 1;
+                    if (ok) commit_pair(tfull + 8 * buf);
                 }
-                if (ok && lane == 0) commit_pair(tfull + 8 * buf);
-                __syncwarp();
+                if (!__shfl_sync(~0u, ok, 0)) break;
+                r.skip(t.nkb);
+                n++;
             }
         }
     } else {
@@ -439,7 +477,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         while (it.next(op, t)) {
             const int buf = n & 1;
             const auto rows = op.rows(t, p);     // the rows' scalars, on their way while the products run
-            if (!mbar_wait(tfull + 8 * buf, (n >> 1) & 1, dead)) break;
+            if (!mbar_wait_warp(tfull + 8 * buf, (n >> 1) & 1, dead)) break;
             n++;
             fence_after();
             op.epilogue(t, p, rows, tmem + buf * BN + ((uint32_t)(p.sub * 32) << 16) + p.half * (BN / 2), [&] {
