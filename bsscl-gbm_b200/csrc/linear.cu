@@ -898,7 +898,7 @@ template <class T> struct LeafRows {
 // The leaves in order of their rows, longest first, for the tiles of dw.
 constexpr int kSortLeaves = 2048;
 
-__global__ void __launch_bounds__(1024) k_leaf_order(const int32_t *__restrict__ off, int32_t groups, int64_t t, int32_t *__restrict__ order) {
+__global__ void __launch_bounds__(1024) k_leaf_order(const int32_t *__restrict__ off, int32_t groups, int64_t t, int4 *__restrict__ order) {
     tc::depend();
     __shared__ int rows[kSortLeaves];
     for (int g = threadIdx.x; g < groups; g += 1024) {
@@ -911,7 +911,9 @@ __global__ void __launch_bounds__(1024) k_leaf_order(const int32_t *__restrict__
         const int mine = rows[g];
         int before = 0;
         for (int k = 0; k < groups; k++) before += rows[k] > mine || (rows[k] == mine && k < g);
-        order[before] = g;
+        int lo, hi;
+        leaf_rows(off, g, t, lo, hi);
+        order[before] = make_int4(g, lo, hi, 0);
     }
 }
 
@@ -924,20 +926,35 @@ template <class T> struct LeafPair {
     static constexpr int laps = 1;
     struct Iter : tc::Snake {
         LeafIter dx;
-        __device__ Iter(const LeafPair &op, int cid, int ncl) : tc::Snake(cid, ncl), dx(op, 0, 0) {}
+        uint32_t per, first;     // units of one leaf's dw, of all leaves'
+        int4 leaf;               // the next unit's leaf and rows: loaded one unit ahead
+        __device__ Iter(const LeafPair &op, int cid, int ncl) : tc::Snake(cid, ncl), dx(op, 0, 0) {
+            per = op.mt * op.nt * op.splits;
+            first = op.sink.out ? per * op.leaves.groups : 0;
+            look(op);
+        }
+        __device__ void look(const LeafPair &op) {
+            if (at >= first) return;
+            const uint32_t k = at / per;
+            if (op.order) {
+                leaf = op.order[k];
+            } else {
+                leaf.x = (int)k;
+                leaf_rows(op.leaves.off, (int)k, op.leaves.t, leaf.y, leaf.z);
+            }
+        }
         __device__ bool next(const LeafPair &op, tc::Tile &t) {
-            const uint32_t tiles = op.mt * op.nt, per = tiles * op.splits, first = op.sink.out ? per * op.leaves.groups : 0;
             if (at >= first) {
                 if (!op.dx.out) return false;
                 dx.at = at - first;
                 step();
                 return dx.next(op, t);
             }
-            const uint32_t k = at / per, i = at - k * per, part = op.splits > 1 ? i / tiles : 0, tile = i - part * tiles, tm = tile / op.nt,
+            const uint32_t tiles = op.mt * op.nt, i = at % per, part = op.splits > 1 ? i / tiles : 0, tile = i - part * tiles, tm = tile / op.nt,
                            tn = tile - tm * op.nt;
-            const int g = op.order ? op.order[k] : (int)k;
-            int lo, hi;
-            leaf_rows(op.leaves.off, g, op.leaves.t, lo, hi);
+            const int g = leaf.x, lo = leaf.y, hi = leaf.z;
+            step();
+            look(op);
             const int nkb = (hi - lo + 63) / 64, each = op.splits > 1 ? (nkb + op.splits - 1) / op.splits : nkb, k0 = min((int)part * each, nkb),
                       k1 = min(k0 + each, nkb);
             t.m0 = t.am = (int)tm * 256;
@@ -952,13 +969,12 @@ template <class T> struct LeafPair {
             // behind the last row of all TMA fills zeros
             t.tail = k1 == nkb && hi < op.leaves.t ? (hi - lo) % 64 : 0;
             t.aux = (int)(part * op.leaves.groups + g);
-            step();
             return true;
         }
     };
     Leaves leaves;         // of dx: its columns are dw's too
     LeafOut<T> dx;         // out null: not wanted
-    const int32_t *order;  // of the leaves (null: as they are)
+    const int4 *order;     // of the leaves (null: as they are)
     int dout, splits, mt, nt;
     Sink<T> sink;          // of the (groups * dout) x din matrix of all leaves' dw; out null: not wanted
     __device__ void finish(int warp, int warps, int lane) const {
@@ -991,7 +1007,7 @@ struct LeafWs {
     uint16_t *x, *w, *dy;
     float *acc;
     uint32_t *tickets;
-    int32_t *order;
+    int4 *order;
     int64_t ldacc, n_tickets, bytes;
     LeafWs(void *ws, int64_t t, int32_t groups, int64_t din, int64_t dout, bool grad, bool in_place) {
         Room r(ws);
@@ -1004,7 +1020,7 @@ struct LeafWs {
         acc = r.take<float>(s > 1 ? s * groups * dout * ldacc : 0);
         n_tickets = s > 1 ? 16 * groups * ((din + 255) / 256) * ((dout + 255) / 256) : 0;
         tickets = r.take<uint32_t>(n_tickets);
-        order = r.take<int32_t>(grad ? groups : 0);
+        order = r.take<int4>(grad ? groups : 0);
         bytes = r.bytes();
     }
 };

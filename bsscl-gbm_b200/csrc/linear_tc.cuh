@@ -12,7 +12,11 @@
 //
 // Warp 0 fetches, warp 1 of the leading CTA issues the products, warps 2..9
 // run the epilogue (warp w reads the tensor memory lanes 32 (w % 4) .. +31,
-// warps 2..5 the tile's left columns, warps 6..9 its right ones).
+// warps 2..5 the tile's left columns, warps 6..9 its right ones), warp 10
+// puts zeros behind a k axis that ends inside a stage.  The thread that
+// fetches and the one that issues products are chosen by elect.sync: under a
+// plain test of the lane the compiler does not know that one thread runs, and
+// the loops took up to 20 % more clocks than the products.
 //
 // Every wait is bounded: when one runs out, the kernel notes it in
 // g_ops_timeout, all roles leave their loops, the copies in flight get time
@@ -27,7 +31,7 @@
 
 namespace tc {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 352;
 constexpr int kEpiWarps = 8;
 constexpr int kBK = 64;                       // values of k a stage: 128 bytes
 constexpr int kABytes = 128 * kBK * 2;        // A of one CTA and stage
@@ -108,6 +112,12 @@ template <bool DATA = false> __device__ __forceinline__ bool mbar_wait(uint32_t 
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *dead) {
     const bool ok = mbar_wait(bar, parity, dead);
     return __all_sync(~0u, ok);
+}
+// One thread of a converged warp, known as such to the compiler.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -360,8 +370,8 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     uint64_t *bars = (uint64_t *)(staging + kStaging);
     const uint32_t stages = smem_u32(base);
     const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, tfull = empty + 8 * S::kStages, tempty = tfull + 16,
-                   tailbar = tempty + 16, fixed = tailbar + 8;
-    uint32_t *tmem_slot = (uint32_t *)(bars + 3 * S::kStages + 5);
+                   fixed = tempty + 16, tailbar = fixed + 8 * S::kStages;
+    uint32_t *tmem_slot = (uint32_t *)(bars + 4 * S::kStages + 4);
     volatile int *dead = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cluster_rank();
@@ -374,12 +384,12 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
             mbar_init(empty + 8 * s, 1);
             // one a stage: a CTA ahead of the other by a whole short tile must not count for both
             mbar_init(fixed + 8 * s, 2);
+            mbar_init(tailbar + 8 * s, 1);
         }
         for (int s = 0; s < 2; s++) {
             mbar_init(tfull + 8 * s, 1);
             mbar_init(tempty + 8 * s, 2 * kEpiWarps);
         }
-        mbar_init(tailbar, 1);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -397,37 +407,31 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     if (warp == 0) {
         // ---- fetch: one thread runs a tile's stages (a stage has 512 clocks)
         Ring<S::kStages> r;
-        uint32_t tail_ph = 0;
         typename Op::Iter it(op, cid, ncl);
         Tile t;
         while (it.next(op, t)) {
-            const bool tail = Op::kTail && t.tail && t.nkb;
-            const int n = t.nkb - tail;
-            bool ok = true;
-            if (lane == 0)
-                ok = Op::kDual && t.kind == 1 ? fetch<Op, true>(op, maps.m + 2, t, n, r, stages, full, empty, rank, dead)
-                                              : fetch<Op, Op::kAMN>(op, maps.m, t, n, r, stages, full, empty, rank, dead);
-            if (!__shfl_sync(~0u, ok, 0)) break;
-            r.skip(n);
-            if (!tail) continue;
-            // The last stage: rows of k behind the axis' end belong to the
-            // next leaf; zeros take their place before the products see them.
-            if (!mbar_wait_warp(empty + 8 * r.s, r.ph ^ 1, dead)) break;
-            if (lane == 0) {
-                mbar_expect(tailbar, S::kStage);
-                if (rank == 0) mbar_arrive(full + 8 * r.s);
-                load_stage<Op, true, false>(Op::kDual ? maps.m + 2 : maps.m, stages + r.s * S::kStage, tailbar, t.am + (int)rank * 128,
-                                            t.n0 + (int)rank * (BN / 2), t.k0 + (t.q0 + n) * kBK, 0, t.bz);
-            }
-            if (!mbar_wait_warp(tailbar, tail_ph, dead)) break;
-            tail_ph ^= 1;
-            uint8_t *st = base + r.s * S::kStage;
-            for (int box = 0; box < S::kStage / 8192; box++)
-                for (int i = t.tail * 8 + lane; i < 64 * 8; i += 32) *(uint4 *)(st + box * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive_at<true>(fixed + 8 * r.s, 0);
-            r.skip(1);
+            if (elect_one()) {
+                const bool tail = Op::kTail && t.tail && t.nkb;
+                const int n = t.nkb - tail;
+                bool ok = Op::kDual && t.kind == 1 ? fetch<Op, true>(op, maps.m + 2, t, n, r, stages, full, empty, rank, dead)
+                                                   : fetch<Op, Op::kAMN>(op, maps.m, t, n, r, stages, full, empty, rank, dead);
+                if (ok && tail) {
+                    // the last stage's bytes count for warp 10, not for the products
+                    Ring<S::kStages> q = r;
+                    q.skip(n);
+                    ok = mbar_wait(empty + 8 * q.s, q.ph ^ 1, dead);
+                    if (ok) {
+                        mbar_expect(tailbar + 8 * q.s, S::kStage);
+                        if (rank == 0) mbar_arrive(full + 8 * q.s);
+                        load_stage<Op, true, false>(Op::kDual ? maps.m + 2 : maps.m, stages + q.s * S::kStage, tailbar + 8 * q.s, t.am + (int)rank * 128,
+                                                    t.n0 + (int)rank * (BN / 2), t.k0 + (t.q0 + n) * kBK, 0, t.bz);
+                    }
+                }
+            }
+            __syncwarp();
+            if (*dead) break;
+            r.skip(t.nkb);
         }
     } else if (warp == 1) {
         // ---- products, issued by one thread too
@@ -439,10 +443,11 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
             Tile t;
             while (it.next(op, t)) {
                 const int buf = n & 1;
-                bool ok = true;
-                if (lane == 0) {
-                    const bool tail = Op::kTail && t.tail && t.nkb, second = Op::kDual && t.kind == 1;
-                    ok = mbar_wait(tempty + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
+                const bool tail = Op::kTail && t.tail && t.nkb, second = Op::kDual && t.kind == 1;
+                const int last = (r.s + t.nkb - 1) % S::kStages;     // the tail's stage
+                __syncwarp();
+                if (elect_one()) {
+                    bool ok = mbar_wait(tempty + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
                     fence_after();
                     const uint32_t d = tmem + buf * BN;
                     Ring<S::kStages> q = r;
@@ -452,14 +457,41 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                     if (ok && tail) {
                         ok = mbar_wait(full + 8 * q.s, q.ph, dead) && mbar_wait<true>(fixed + 8 * q.s, fixed_ph >> q.s & 1, dead);
                         fence_after();
-                        if (ok) multiply_stage<Op, true>(d, stages + q.s * S::kStage, idesc, t.nkb > 1), commit_pair(empty + 8 * q.s);
-                        fixed_ph ^= 1u << q.s;
+                        if (ok) {
+                            multiply_stage<Op, true>(d, stages + q.s * S::kStage, idesc, t.nkb > 1);
+                            commit_pair(empty + 8 * q.s);
+                        }
                     }
                     if (ok) commit_pair(tfull + 8 * buf);
                 }
-                if (!__shfl_sync(~0u, ok, 0)) break;
+                __syncwarp();
+                if (*dead) break;
+                if (tail) fixed_ph ^= 1u << last;
                 r.skip(t.nkb);
                 n++;
+            }
+        }
+    } else if (warp == 2 + kEpiWarps) {
+        // ---- the last stage of a k axis that ends inside it: rows behind the
+        // end belong to the next leaf; zeros take their place before the
+        // products see them
+        if (Op::kTail) {
+            Ring<S::kStages> r;
+            uint32_t ph = 0;
+            typename Op::Iter it(op, cid, ncl);
+            Tile t;
+            while (it.next(op, t)) {
+                r.skip(t.nkb);
+                if (!t.tail || !t.nkb) continue;
+                const int s = r.s == 0 ? S::kStages - 1 : r.s - 1;
+                if (!mbar_wait_warp(tailbar + 8 * s, ph >> s & 1, dead)) break;
+                ph ^= 1u << s;
+                uint8_t *st = base + s * S::kStage;
+                for (int box = 0; box < S::kStage / 8192; box++)
+                    for (int i = t.tail * 8 + lane; i < 64 * 8; i += 32) *(uint4 *)(st + box * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at<true>(fixed + 8 * s, 0);
             }
         }
     } else {
