@@ -107,11 +107,11 @@ def softmax_xent(x, w, target):
     y = _vector(target, "target", torch.int64, n, x)
     px, pw, device = x.data_ptr(), w.data_ptr(), x.device
     loss = torch.empty(n, dtype=torch.float32, device=device)
-    lse = torch.empty(n, dtype=torch.float32, device=device)
+    lse = loss.new_empty(n)
     L = lib()
     size = L.gbm_softmax_xent_workspace(n, d, v, 0, _in_place(px, ldx, pw, ldw))
-    ws = _workspace(size, device)
-    _call(L.gbm_softmax_xent, device, px, ldx, pw, ldw, _TYPES[x.dtype], n, d, v, y, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), size)
+    ws = _workspace(size, device) if size else None
+    _call(L.gbm_softmax_xent, device, px, ldx, pw, ldw, _TYPES[x.dtype], n, d, v, y, loss.data_ptr(), lse.data_ptr(), ws.data_ptr() if size else None, size)
     return loss, lse
 
 
@@ -130,8 +130,8 @@ def softmax_xent_grad(x, w, target, lse, grad_loss, want_dx=True, want_dw=True):
     if not (want_dx or want_dw):
         raise ValueError("neither dx nor dw is wanted")
     px, pw, device = x.data_ptr(), w.data_ptr(), x.device
-    dx = torch.empty((n, d), dtype=x.dtype, device=device) if want_dx else None
-    dw = torch.empty((v, d), dtype=x.dtype, device=device) if want_dw else None
+    dx = x.new_empty((n, d)) if want_dx else None
+    dw = x.new_empty((v, d)) if want_dw else None
     if n == 0 and not want_dw:
         return dx, dw
     L = lib()
@@ -165,7 +165,7 @@ def leaf_linear(x, w, offsets, out=None):
     n, ldx, e, dout, din, off = _leaf_args(x, w, offsets)
     px, pw, device = x.data_ptr(), w.data_ptr(), x.device
     if out is None:
-        y, ldy = torch.empty((n, dout), dtype=x.dtype, device=device), dout
+        y, ldy = x.new_empty((n, dout)), dout
     else:
         y = out
         rows, cols, ldy = _matrix(out, "out", x)
@@ -192,8 +192,8 @@ def leaf_linear_grad(x, w, offsets, dy, want_dx=True, want_dw=True):
     if not (want_dx or want_dw):
         raise ValueError("neither dx nor dw is wanted")
     px, pw, pg, device = x.data_ptr(), w.data_ptr(), dy.data_ptr(), x.device
-    dx = torch.empty((n, din), dtype=x.dtype, device=device) if want_dx else None
-    dw = torch.empty((e, dout, din), dtype=x.dtype, device=device) if want_dw else None
+    dx = x.new_empty((n, din)) if want_dx else None
+    dw = x.new_empty((e, dout, din)) if want_dw else None
     if n == 0 and not want_dw:
         return dx, dw
     L = lib()

@@ -315,6 +315,13 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// A row's loss and lse from its sum of exponentials and its target's logit.
+__device__ __forceinline__ void xent_row(float2 a, float ly, int64_t y, int64_t v, float &loss, float &lse) {
+    const float z = a.x == -INFINITY ? logf(a.y) : a.x + logf(a.y);
+    lse = z;
+    loss = y >= 0 && y < v ? z - ly : 0.f;
+}
+
 // (m, s) stands for the sum s exp(m) of exponentials.  With no finite m yet
 // the shift is 0, so that s stays 0 (or NaN, if a NaN is among them).
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
@@ -324,26 +331,54 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 
 // x w^T, of which each tile leaves the maximum and the sum of exponentials of
 // its 256 classes for each row (part [128 classes][row]), and the target's
-// logit.  One lane of the epilogue has one row, so no exchange between lanes
-// is needed.
+// logit; or, where one cluster takes all classes of its rows (whole), the
+// rows' loss and lse at once.  One lane of the epilogue has one row, so no
+// exchange between lanes is needed.
 struct XentStats {
     static constexpr int kBN = 256;
     static constexpr bool kAMN = false, kBMN = false, kTail = false, kDual = false;
     static constexpr int laps = 1;
-    using Iter = DenseIter;
+    struct Iter {
+        uint32_t at, step, c;
+        __device__ Iter(const XentStats &, int cid, int ncl) : at(cid), step(ncl), c(0) {}
+        __device__ bool next(const XentStats &op, tc::Tile &t) {
+            const Dense &g = op.dense;
+            if (!op.whole) {
+                if (at >= (uint32_t)(g.mt * g.nt)) return false;
+                g.place<kBN>(at, t);
+                at += step;
+                return true;
+            }
+            if (at >= (uint32_t)g.mt) return false;
+            t.m0 = t.am = (int)at * 256;
+            t.n0 = (int)c * kBN;
+            t.mend = min(g.m - t.m0, 256) + t.m0;
+            t.nend = min(g.n - t.n0, kBN) + t.n0;
+            t.k0 = t.q0 = t.bz = t.tail = t.kind = t.aux = 0;
+            t.nkb = g.nkb;
+            if (++c == (uint32_t)g.nt) c = 0, at += step;
+            return true;
+        }
+    };
+    struct State {
+        float m, s, ly;
+        int turn;
+    };
     Dense dense;
+    bool whole;
     const int64_t *target;
     float2 *part;
-    float *ly;
+    float *ly, *loss, *lse;
     __device__ void finish(int, int, int) const {}
     __device__ int64_t rows(const tc::Tile &t, const tc::Place &p) const { return t.m0 + p.row < t.mend ? target[t.m0 + p.row] : -1; }
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int64_t y, uint32_t addr, R release) const {
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int64_t y, State &st, uint32_t addr, R release) const {
         const int row = t.m0 + p.row, c0 = p.half * 128, left = t.nend - t.n0 - c0;    // columns of this half that exist
         const bool in = row < t.mend;
         const int64_t off = y - t.n0 - c0;
         const int yc = off >= 0 && off < min(128, left) ? (int)off : -1;
         const tc::F2 log2e = tc::f2(kLog2e, kLog2e);
-        float m = -INFINITY, s = 0.f;
+        const bool fresh = !whole || t.n0 == 0;
+        float m = fresh ? -INFINITY : st.m, s = fresh ? 0.f : st.s, z = fresh ? 0.f : st.ly;
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
             float v[32];
@@ -351,10 +386,8 @@ struct XentStats {
             tc::tmem_wait(v);
             if (c == 96) release();
             if (__any_sync(~0u, yc >= c && yc < c + 32)) {
-                float z = 0.f;
 #pragma unroll
                 for (int i = 0; i < 32; i++) z = yc == c + i ? v[i] : z;
-                if (yc >= c && yc < c + 32) ly[row] = z;
             }
             if (c + 32 > left) {
 #pragma unroll
@@ -365,8 +398,8 @@ struct XentStats {
 #pragma unroll
             for (int i = 0; i < 28; i += 2) top[i / 2 % 4] = tc::max3(top[i / 2 % 4], v[i], v[i + 1]);
             const float mc = fmaxf(tc::max3(top[0], top[1], top[2]), fmaxf(top[3], v[28]));
-            const float shift = mc == -INFINITY ? 0.f : mc, z = shift * kLog2e;
-            const tc::F2 minus = tc::f2(-z, -z);
+            const float shift = mc == -INFINITY ? 0.f : mc, zs = shift * kLog2e;
+            const tc::F2 minus = tc::f2(-zs, -zs);
             tc::F2 e[4] = {tc::f2(s * ex2((m - shift) * kLog2e), 0.f), tc::f2(0.f, 0.f), tc::f2(0.f, 0.f), tc::f2(0.f, 0.f)};
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
@@ -379,7 +412,31 @@ struct XentStats {
             s = a + b;
             m = mc;
         }
-        if (in) part[((int64_t)(t.n0 / kBN) * 2 + p.half) * dense.m + row] = make_float2(m, s);
+        if (!whole) {
+            if (yc >= 0) ly[row] = z;
+            if (in) part[((int64_t)(t.n0 / kBN) * 2 + p.half) * dense.m + row] = make_float2(m, s);
+            return;
+        }
+        st.m = m;
+        st.s = s;
+        st.ly = z;
+        if (t.nend < dense.n) return;
+        // The right half's sums through shared memory.  Of four places: the
+        // right warp is never four row tiles ahead of the left one, whose
+        // release of tensor memory the products two tiles on wait for.
+        const int slot = st.turn & 3, phase = st.turn >> 2 & 1;
+        st.turn++;
+        if (p.half) {
+            *(float4 *)(p.staging + slot * 512 + p.lane * 16) = make_float4(m, s, z, 0.f);
+            __syncwarp();
+            if (p.lane == 0) tc::mbar_arrive(p.swap + 8 * slot);
+            return;
+        }
+        if (!tc::mbar_wait_warp(p.swap + 8 * slot, phase, p.dead)) return;
+        const float4 o = *(const float4 *)(p.staging + 4 * 4096 + slot * 512 + p.lane * 16);
+        if (!in) return;
+        // one of the halves has the target's logit, the other 0
+        xent_row(join(make_float2(m, s), make_float2(o.x, o.y)), z + o.z, y, dense.n, loss[row], lse[row]);
     }
 };
 
@@ -400,11 +457,7 @@ __global__ void __launch_bounds__(256) k_xent_join(const float2 *__restrict__ pa
         __syncthreads();
     }
     if (q || row >= n) return;
-    a = sh[0][r];
-    const float z = a.x == -INFINITY ? logf(a.y) : a.x + logf(a.y);
-    const int64_t y = target[row];
-    lse[row] = z;
-    loss[row] = y >= 0 && y < v ? z - ly[row] : 0.f;
+    xent_row(sh[0][r], ly[row], target[row], v, loss[row], lse[row]);
 }
 
 // One piece of G: the logits once more, G = c (exp(l - lse) - [k = target])
@@ -421,6 +474,7 @@ template <class T> struct XentG {
     const float *lse, *grad_loss, *scale;
     T *g;
     int64_t ldg, part;  // row stride; from the leading to the trailing part (0: one part)
+    using State = tc::None;
     struct Rows {
         int64_t y;
         float c, z;
@@ -432,7 +486,7 @@ template <class T> struct XentG {
         if (row < t.mend) r = {target[row], grad_loss[row] * (scale ? *scale : 1.f), lse[row] * kLog2e};
         return r;
     }
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, Rows r, uint32_t addr, R release) const {
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, Rows r, tc::None &, uint32_t addr, R release) const {
         const int h0 = p.half * 128;
         const int64_t y = r.y;
         const float c = r.c, z = r.z;
@@ -603,8 +657,9 @@ template <class T, int BN> struct XentPair {
     Sink<T> sink[2];
     int first, laps;
     __device__ void finish(int, int, int) const {}
+    using State = tc::None;
     __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const {
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, tc::None &, uint32_t addr, R release) const {
         const Dense &g = dense[t.kind];
         sink_tile<BN / 2>(sink[t.kind], g.m, g.splits, t, p, addr, release, (t.m0 / 256) * g.nt + t.n0 / BN);
     }
@@ -624,10 +679,11 @@ double chain(int64_t u0, int64_t l0, int64_t u1, int64_t l1) {
 }
 
 // Parts of both products' k axes (tx tiles of kx stages, tw of kw): those that
-// end first.  Split sums cost a launch's worth of waits and the time the f32
-// sums take to be written and read again (512 KB a tile, 0.08 us at the
-// memory's rate: 0.3 of a stage).
-void choose_splits(int64_t tx, int64_t kx, int64_t tw, int64_t kw, int &sx, int &sw) {
+// end first.  Split sums cost some 5 us of fences, tickets and reading back,
+// and the time the f32 sums take to be written and read again (512 KB a tile,
+// 0.08 us at the memory's rate: 0.3 of a stage).  cost: a stage's time against
+// that of a 256 x 256 tile.
+void choose_splits(int64_t tx, int64_t kx, int64_t tw, int64_t kw, double cost, int &sx, int &sw) {
     static constexpr int kTry[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
     double least = 1e300;
     for (int a : kTry) {
@@ -635,8 +691,8 @@ void choose_splits(int64_t tx, int64_t kx, int64_t tw, int64_t kw, int &sx, int 
         for (int b : kTry) {
             if (b > 1 && (b > kw || !tw)) break;
             const int64_t la = (kx + a - 1) / a, lb = (kw + b - 1) / b;
-            double t = la >= lb ? chain(tx * a, la, tw * b, lb) : chain(tw * b, lb, tx * a, la);
-            t += (a > 1 ? 4 + tx * a * 0.3 : 0) + (b > 1 ? 4 + tw * b * 0.3 : 0);
+            double t = cost * (la >= lb ? chain(tx * a, la, tw * b, lb) : chain(tw * b, lb, tx * a, la));
+            t += (a > 1 || b > 1 ? 20 : 0) + (a > 1 ? tx * a * 0.3 * cost : 0) + (b > 1 ? tw * b * 0.3 * cost : 0);
             if (t < least * 0.98) least = t, sx = a, sw = b;
         }
     }
@@ -670,7 +726,7 @@ struct XentPlan {
         const int64_t dt = (d + bn - 1) / bn;
         tx = (n + 255) / 256 * dt;
         tw = (pc + 255) / 256 * dt;
-        choose_splits(tx, (pc + 63) / 64 * parts, tw, (n + 63) / 64 * parts, sx, sw);
+        choose_splits(tx, (pc + 63) / 64 * parts, tw, (n + 63) / 64 * parts, bn / 256.0, sx, sw);
     }
     bool dx_acc() const { return pieces > 1 || sx > 1; }
     int64_t tickets() const { return 16 * (tx + tw * pieces); }
@@ -687,6 +743,14 @@ struct Room {
     int64_t bytes() const { return at - base; }
 };
 
+// Whether one cluster takes all classes of its rows: where that takes no
+// longer than tiles for all clusters and a second launch that joins their
+// parts (about 16 stages' time; a tile 4 stages on top of its own).
+bool xent_whole(int64_t n, int64_t d, int64_t v) {
+    const int64_t mt = (n + 255) / 256, nt = (v + 255) / 256, k = (d + 63) / 64 + 4;
+    return (mt + 73) / 74 * nt * k <= (mt * nt + 73) / 74 * k + 16;
+}
+
 struct XentLoss {
     uint16_t *x, *w;
     float2 *part;
@@ -697,8 +761,9 @@ struct XentLoss {
         const int64_t dp = round_up(d, 8);
         x = r.take<uint16_t>(in_place ? 0 : n * dp);
         w = r.take<uint16_t>(in_place ? 0 : v * dp);
-        part = r.take<float2>((v + 255) / 256 * 2 * n);
-        ly = r.take<float>(n);
+        const bool parts = !xent_whole(n, d, v);
+        part = r.take<float2>(parts ? (v + 255) / 256 * 2 * n : 0);
+        ly = r.take<float>(parts ? n : 0);
         bytes = r.bytes();
     }
 };
@@ -733,10 +798,11 @@ Err xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, bool bf
     const View a = readable(prep, {x, d, n, ldx}, q.x), b = readable(prep, {w, d, v, ldw}, q.w);
     Err e = run_prep(prep, st);
     if (e.bad()) return e;
-    XentStats op{Dense(n, v, d, 256), target, q.part, q.ly};
+    const Dense g(n, v, d, 256);
+    XentStats op{g, xent_whole(n, d, v), target, q.part, q.ly, loss, lse};
     const View ab[2] = {a, b};
-    e = launch(ab, op, bf16, op.dense.units(), st);
-    if (e.bad()) return e;
+    e = launch(ab, op, bf16, op.whole ? g.mt : g.units(), st);
+    if (e.bad() || op.whole) return e;
     return start(k_xent_join, (n + 7) / 8, 256, 0, st, q.part, n, (v + 255) / 256 * 2, v, target, q.ly, loss, lse);
 }
 
@@ -892,8 +958,9 @@ template <class T> struct LeafRows {
     __device__ void finish(int warp, int warps, int lane) const {
         if (y.rest) leaf_rest(leaves, y.out, y.ld, warp, warps, lane);
     }
+    using State = tc::None;
     __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const { y.store(t, p, addr, release); }
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, tc::None &, uint32_t addr, R release) const { y.store(t, p, addr, release); }
 };
 
 // The leaves in order of their rows, longest first, for the tiles of dw.
@@ -981,8 +1048,9 @@ template <class T> struct LeafPair {
     __device__ void finish(int warp, int warps, int lane) const {
         if (dx.out && dx.rest) leaf_rest(leaves, dx.out, dx.ld, warp, warps, lane);
     }
+    using State = tc::None;
     __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, uint32_t addr, R release) const {
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, tc::None &, uint32_t addr, R release) const {
         if (!t.kind) {
             dx.store(t, p, addr, release);
             return;
@@ -1000,7 +1068,7 @@ template <class T> struct LeafPair {
 // Parts of dw's k axis, as if all leaves were alike.
 int leaf_splits(int64_t t, int32_t groups, int64_t din, int64_t dout) {
     int none = 1, s = 1;
-    choose_splits(0, 0, (int64_t)groups * ((din + 255) / 256) * ((dout + 255) / 256), (t / groups + 63) / 64, none, s);
+    choose_splits(0, 0, (int64_t)groups * ((din + 255) / 256) * ((dout + 255) / 256), (t / groups + 63) / 64, 1.0, none, s);
     return s;
 }
 

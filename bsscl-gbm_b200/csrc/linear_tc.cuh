@@ -272,11 +272,16 @@ struct Maps {
     alignas(64) CUtensorMap m[4];
 };
 
+// An epilogue that keeps nothing from tile to tile.
+struct None {};
+
 // What one epilogue warp knows of its place.
 struct Place {
     int sub, half, lane, rank;
     int row;             // row of the tile (0..255) of this lane
     uint8_t *staging;    // 4096 bytes of this warp's own
+    uint32_t swap;       // 4 barriers of the two warps of these rows (left and right columns)
+    volatile int *dead;
 };
 
 // A place among the stages, and its barriers' parity.
@@ -371,7 +376,8 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     const uint32_t stages = smem_u32(base);
     const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, tfull = empty + 8 * S::kStages, tempty = tfull + 16,
                    fixed = tempty + 16, tailbar = fixed + 8 * S::kStages;
-    uint32_t *tmem_slot = (uint32_t *)(bars + 4 * S::kStages + 4);
+    const uint32_t swap = tailbar + 8 * S::kStages;
+    uint32_t *tmem_slot = (uint32_t *)(bars + 4 * S::kStages + 20);
     volatile int *dead = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cluster_rank();
@@ -390,6 +396,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
             mbar_init(tfull + 8 * s, 1);
             mbar_init(tempty + 8 * s, 2 * kEpiWarps);
         }
+        for (int s = 0; s < 16; s++) mbar_init(swap + 8 * s, 1);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -503,6 +510,9 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         p.rank = (int)rank;
         p.row = (int)rank * 128 + p.sub * 32 + lane;
         p.staging = staging + (warp - 2) * 4096;
+        p.swap = swap + 32 * p.sub;
+        p.dead = dead;
+        typename Op::State state{};
         int n = 0;
         typename Op::Iter it(op, cid, ncl);
         Tile t;
@@ -512,7 +522,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
             if (!mbar_wait_warp(tfull + 8 * buf, (n >> 1) & 1, dead)) break;
             n++;
             fence_after();
-            op.epilogue(t, p, rows, tmem + buf * BN + ((uint32_t)(p.sub * 32) << 16) + p.half * (BN / 2), [&] {
+            op.epilogue(t, p, rows, state, tmem + buf * BN + ((uint32_t)(p.sub * 32) << 16) + p.half * (BN / 2), [&] {
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_at<false>(tempty + 8 * buf, 0);

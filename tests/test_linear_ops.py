@@ -547,8 +547,9 @@ def _rc(f, *a):
 
 
 def test_xent_refusals(L):
-    need = L.gbm_softmax_xent_workspace(10, 16, 20, 0, 1)
-    good = [PTR, 16, PTR, 16, BF16, 10, 16, 20, PTR, PTR, PTR, PTR, need]
+    assert L.gbm_softmax_xent_workspace(10, 16, 20, 0, 1) == 0      # few classes: no parts to join
+    need = L.gbm_softmax_xent_workspace(10, 16, 100000, 0, 1)
+    good = [PTR, 16, PTR, 16, BF16, 10, 16, 100000, PTR, PTR, PTR, PTR, need]
     for at, value, rc, word in ((0, None, ARG, "null"), (1, 15, ARG, "stride"), (2, None, ARG, "null"), (3, 8, ARG, "stride"),
                                 (4, F32, UNSUPPORTED, "type"), (4, 9, UNSUPPORTED, "type"), (5, -1, ARG, "sizes"), (6, 0, ARG, "sizes"),
                                 (7, 0, ARG, "sizes"), (7, 1 << 31, ARG, "sizes"), (8, None, ARG, "null"), (9, None, ARG, "null"),
