@@ -266,17 +266,17 @@ struct Dense {
     int splits;        // parts of the k axis
     int mt, nt;        // tiles
     int per;           // stages of a part
+    tc::Div all, band; // tiles in all, in 8 rows of tiles
     Dense() : m(0), n(0), nkb(0), splits(1), mt(0), nt(0), per(0) {}
     Dense(int64_t m_, int64_t n_, int64_t k, int bn, int splits_ = 1, int laps = 1)
         : m((int)m_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK) * laps), splits(splits_), mt((int)((m_ + 255) / 256)), nt((int)((n_ + bn - 1) / bn)),
-          per((nkb + splits_ - 1) / splits_) {}
+          per((nkb + splits_ - 1) / splits_), all((uint32_t)std::min<int64_t>(tiles(), INT_MAX)), band((uint32_t)std::min<int64_t>(8LL * nt, INT_MAX)) {}
     int64_t tiles() const { return (int64_t)mt * nt; }
     int64_t units() const { return tiles() * splits; }
-    // A tile's place is found in 32 bits (64-bit divisions between two tiles
-    // held the products up by some 1000 clocks); launch() refuses more units.
+    // A tile's place is found in 32 bits; launch() refuses more units.
     template <int BN> __device__ void place(uint32_t at, tc::Tile &t) const {
-        const uint32_t all = mt * nt, part = splits > 1 ? at / all : 0, i = at - part * all;
-        const uint32_t band = 8 * nt, block = i / band, rest = i - block * band, wide = min(8u, mt - block * 8);
+        const uint32_t part = splits > 1 ? all(at) : 0, i = at - part * all.d;
+        const uint32_t block = band(i), rest = i - block * band.d, wide = min(8u, mt - block * 8);
         const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
         t.m0 = t.am = (int)(tm * 256);
         t.n0 = (int)(tn * BN);
@@ -369,7 +369,7 @@ struct XentStats {
     const int64_t *target;
     float2 *part;
     float *ly, *loss, *lse;
-    __device__ void finish(int, int, int) const {}
+    __device__ void rest(int, int, int) const {}
     __device__ int64_t rows(const tc::Tile &t, const tc::Place &p) const { return t.m0 + p.row < t.mend ? target[t.m0 + p.row] : -1; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int64_t y, State &st, uint32_t addr, R release) const {
         const int row = t.m0 + p.row, c0 = p.half * 128, left = t.nend - t.n0 - c0;    // columns of this half that exist
@@ -479,7 +479,7 @@ template <class T> struct XentG {
         int64_t y;
         float c, z;
     };
-    __device__ void finish(int, int, int) const {}
+    __device__ void rest(int, int, int) const {}
     __device__ Rows rows(const tc::Tile &t, const tc::Place &p) const {
         const int row = t.m0 + p.row;
         Rows r{-1, 0.f, 0.f};
@@ -656,7 +656,7 @@ template <class T, int BN> struct XentPair {
     Dense dense[2];
     Sink<T> sink[2];
     int first, laps;
-    __device__ void finish(int, int, int) const {}
+    __device__ void rest(int, int, int) const {}
     using State = tc::None;
     __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, tc::None &, uint32_t addr, R release) const {
@@ -873,8 +873,10 @@ struct Leaves {
     int32_t groups;
     int n;              // columns of the result
     int nkb, nt;
+    tc::Div band;       // tiles in 8 rows of tiles
     Leaves(const int32_t *off_, int64_t t_, int32_t groups_, int64_t k, int64_t n_)
-        : off(off_), t(t_), groups(groups_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK)), nt((int)((n_ + 255) / 256)) {}
+        : off(off_), t(t_), groups(groups_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK)), nt((int)((n_ + 255) / 256)),
+          band((uint32_t)std::min<int64_t>(8LL * nt, INT_MAX)) {}
     // tiles at most: each leaf may end in a part of one
     int64_t units() const { return ((t + 255) / 256 + groups) * nt; }
 };
@@ -884,7 +886,7 @@ struct Leaves {
 struct LeafIter {
     uint32_t at, step, base, total, upto;    // tiles before these 32 leaves, in them, in them up to this lane's
     int first, lo, hi;
-    template <class Op> __device__ LeafIter(const Op &op, int cid, int ncl) : at(cid), step(ncl), base(0), first(0) { look(op); }
+    template <class Op> __device__ LeafIter(const Op &, int cid, int ncl) : at(cid), step(ncl), base(0), total(0), first(-32) {}
     template <class Op> __device__ void look(const Op &op) {
         const int lane = threadIdx.x % 32, g = first + lane;
         lo = hi = 0;
@@ -898,7 +900,7 @@ struct LeafIter {
         total = __shfl_sync(~0u, upto, 31);
     }
     template <class Op> __device__ bool next(const Op &op, tc::Tile &t) {
-        while (at >= base + total) {
+        while (first < 0 || at >= base + total) {
             base += total;
             first += 32;
             if (first >= op.leaves.groups) return false;
@@ -909,7 +911,7 @@ struct LeafIter {
         const int a = __shfl_sync(~0u, lo, l), b = __shfl_sync(~0u, hi, l);
         const uint32_t end = __shfl_sync(~0u, upto, l), rt = (b - a + 255) / 256, i = rel - (end - rt * nt);
         // 8 row tiles beside one another, as in Dense
-        const uint32_t band = 8 * nt, block = i / band, rest = i - block * band, wide = min(8u, rt - block * 8);
+        const uint32_t block = op.leaves.band(i), rest = i - block * op.leaves.band.d, wide = min(8u, rt - block * 8);
         const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
         t.m0 = t.am = a + (int)tm * 256;
         t.n0 = (int)(tn * 256);
@@ -955,7 +957,7 @@ template <class T> struct LeafRows {
     using Iter = LeafIter;
     Leaves leaves;
     LeafOut<T> y;
-    __device__ void finish(int warp, int warps, int lane) const {
+    __device__ void rest(int warp, int warps, int lane) const {
         if (y.rest) leaf_rest(leaves, y.out, y.ld, warp, warps, lane);
     }
     using State = tc::None;
@@ -1003,7 +1005,7 @@ template <class T> struct LeafPair {
         }
         __device__ void look(const LeafPair &op) {
             if (at >= first) return;
-            const uint32_t k = at / per;
+            const uint32_t k = op.per(at);
             if (op.order) {
                 leaf = op.order[k];
             } else {
@@ -1018,7 +1020,7 @@ template <class T> struct LeafPair {
                 step();
                 return dx.next(op, t);
             }
-            const uint32_t tiles = op.mt * op.nt, i = at % per, part = op.splits > 1 ? i / tiles : 0, tile = i - part * tiles, tm = tile / op.nt,
+            const uint32_t i = at - op.per(at) * per, part = op.splits > 1 ? op.tiles(i) : 0, tile = i - part * op.tiles.d, tm = op.cols(tile),
                            tn = tile - tm * op.nt;
             const int g = leaf.x, lo = leaf.y, hi = leaf.z;
             step();
@@ -1044,8 +1046,9 @@ template <class T> struct LeafPair {
     LeafOut<T> dx;         // out null: not wanted
     const int4 *order;     // of the leaves (null: as they are)
     int dout, splits, mt, nt;
+    tc::Div per, tiles, cols;    // units of one leaf's dw, its tiles, tiles side by side
     Sink<T> sink;          // of the (groups * dout) x din matrix of all leaves' dw; out null: not wanted
-    __device__ void finish(int warp, int warps, int lane) const {
+    __device__ void rest(int warp, int warps, int lane) const {
         if (dx.out && dx.rest) leaf_rest(leaves, dx.out, dx.ld, warp, warps, lane);
     }
     using State = tc::None;
@@ -1129,7 +1132,11 @@ Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off,
     }
     Err e = run_prep(prep, st);
     const int s = leaf_splits(t, groups, din, dout), mt = (int)((dout + 255) / 256), nt = (int)((din + 255) / 256);
-    LeafPair<T> op{Leaves(off, t, groups, dout, din), {}, nullptr, (int)dout, s, mt, nt, {}};
+    LeafPair<T> op{Leaves(off, t, groups, dout, din), {}, nullptr, (int)dout, s, mt, nt, {}, {}, {}, {}};
+    if ((int64_t)mt * nt * s > INT_MAX) return {GBM_ERR_ARG, "more than 2^31 tiles"};
+    op.per = tc::Div((uint32_t)(mt * nt * s));
+    op.tiles = tc::Div((uint32_t)(mt * nt));
+    op.cols = tc::Div((uint32_t)nt);
     int64_t units = 0;
     if (dx) {
         op.dx = {dx, lddx, tc::store_width(dx, lddx), zero_rest};
