@@ -1,0 +1,209 @@
+"""Linear models in a tree's leaves under one softmax head.
+
+The reference's leaves hold constants (E:517-823) and its multi-class fit
+grows a tree per class and round (E:2949-3065; the engine takes up to 64
+classes).  :class:`LeafLinearClassifier` lets one trained tree route the rows,
+gives every leaf a linear map of its own and classifies with a head shared by
+all leaves, over any number of classes.  Its training step is made of the
+device operators of :mod:`bsscl_gbm_b200.linear`.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+
+from .estimator import _device_index
+
+
+def leaf_of_rows(model, X, tree=0, class_index=0):
+    """Index (0 .. leaves-1, in node order) of the leaf that each row of X
+    reaches in tree ``tree`` of a fitted estimator (of class ``class_index``'s
+    trees for a multi-class one), and the number of leaves.  The rows are
+    binned on the GPU with the model's edges and walked like predict_batch_jit
+    (E:843-861)."""
+    X = model._prep_X(X)
+    t = (model.mc_trees[class_index] if model._is_multiclass else model.trees)[tree]
+    tf, tt, _, tl, tr, nc = t[:6]
+    tf, tt, tl, tr = (np.asarray(a)[:nc] for a in (tf, tt, tl, tr))
+    nan_right = None
+    if not model._is_multiclass and tree < len(model._tree_nan_right):
+        nan_right = model._tree_nan_right[tree]
+    xb = model._get_engine().bin_features(X, model.bin_edges, model.feature_bin_counts, model._nan_bin_id)
+    node, rows = np.zeros(len(X), np.int64), np.arange(len(X))
+    while True:
+        f = tf[node]
+        inner = f >= 0
+        if not inner.any():
+            break
+        b = xb[rows, np.where(inner, f, 0)].astype(np.int64)
+        left = b <= tt[node]
+        if nan_right is not None:
+            left &= ~((nan_right[node] != 0) & (b == 0))
+        node = np.where(inner, np.where(left, tl[node], tr[node]), node)
+    leaves = np.flatnonzero(tf < 0)
+    return np.searchsorted(leaves, node).astype(np.int32), len(leaves)
+
+
+class LeafLinearClassifier:
+    """Softmax classifier whose hidden rows are linear in the features, with a
+    map of their own in every leaf of a routing tree: for a row x of leaf g,
+    ``logits = head @ (w[g] @ [x, 1])``.
+
+    router: a fitted HybridHistGBMNumbaV1_0_1 (binary, multi-class or
+    regression) whose tree ``tree`` routes the rows; None = one leaf.  Trained
+    by stochastic gradient descent on the class-weighted log-loss
+    (class_weight as the estimator's), the gradients clipped to ``max_norm``.
+    Weights are kept in float32 and multiplied in ``dtype``.  Features are standardised; a missing value counts as the mean.
+    """
+
+    def __init__(self, router=None, tree=0, n_hidden=64, learning_rate=0.5, max_norm=1.0, n_epochs=10, batch_size=8192,
+                 class_weight='balanced_sqrt', dtype='bfloat16', random_state=0, device='b200'):
+        if dtype not in ('bfloat16', 'float16'):
+            raise ValueError(f"dtype must be 'bfloat16' or 'float16', got {dtype!r}")
+        if n_hidden < 1 or n_epochs < 1 or batch_size < 1:
+            raise ValueError("n_hidden, n_epochs and batch_size must be at least 1")
+        _device_index(device)
+        self.router, self.tree, self.n_hidden = router, tree, int(n_hidden)
+        self.learning_rate, self.max_norm = float(learning_rate), float(max_norm)
+        self.n_epochs, self.batch_size = int(n_epochs), int(batch_size)
+        self.class_weight, self.dtype, self.random_state, self.device = class_weight, dtype, random_state, device
+        self.loss_history_ = []
+
+    # -- data ---------------------------------------------------------------
+    def _device(self):
+        import torch
+        return torch.device("cuda", _device_index(self.device) or 0)
+
+    def _routes(self, X):
+        if self.router is None:
+            return np.zeros(len(X), np.int32), 1
+        return leaf_of_rows(self.router, X, self.tree)
+
+    def _features(self, X):
+        """Standardised features and a column of ones, on the device."""
+        import torch
+        Z = np.nan_to_num((np.asarray(X, np.float64) - self._mean) / self._std, nan=0.0, posinf=0.0, neginf=0.0)
+        Z = np.column_stack([Z, np.ones(len(Z))]).astype(np.float32)
+        return torch.from_numpy(Z).to(self._device()).to(getattr(torch, self.dtype))
+
+    def _by_leaf(self, rows, leaf):
+        """The rows in order of their leaves, and the leaves' offsets."""
+        import torch
+        order = torch.argsort(leaf[rows], stable=True)
+        rows = rows[order]
+        count = torch.bincount(leaf[rows], minlength=self.n_leaves_)
+        offsets = torch.zeros(self.n_leaves_ + 1, dtype=torch.int32, device=rows.device)
+        offsets[1:] = torch.cumsum(count, 0)
+        return rows, offsets
+
+    def _check(self, X):
+        X = np.asarray(X)
+        if X.ndim != 2 or len(X) == 0:
+            raise ValueError(f"X must be 2-D with rows, got shape {X.shape}")
+        return X
+
+    # -- training -----------------------------------------------------------
+    def fit(self, X, y):
+        import torch
+
+        from . import linear
+        X, y = self._check(X), np.asarray(y)
+        if len(y) != len(X):
+            raise ValueError(f"X has {len(X)} rows but y has {len(y)}")
+        self.classes_, index = np.unique(y, return_inverse=True)
+        if len(self.classes_) < 2:
+            raise ValueError("y holds a single class")
+        self.n_features_in_, K = X.shape[1], len(self.classes_)
+        finite = np.where(np.isfinite(X), X, np.nan).astype(np.float64)
+        seen = np.isfinite(finite).sum(0) > 0
+        self._mean, self._std = np.zeros(X.shape[1]), np.ones(X.shape[1])
+        self._mean[seen], self._std[seen] = np.nanmean(finite[:, seen], 0), np.nanstd(finite[:, seen], 0)
+        self._std[self._std == 0] = 1.0
+        weight = np.ones(K)
+        if self.class_weight in ('balanced', 'balanced_sqrt'):   # E:2570-2603
+            weight = len(y) / (K * np.bincount(index, minlength=K))
+            if self.class_weight == 'balanced_sqrt':
+                weight = weight ** 0.35
+        route, self.n_leaves_ = self._routes(X)
+        dev, dt = self._device(), getattr(torch, self.dtype)
+        x, leaf = self._features(X), torch.from_numpy(route.astype(np.int64)).to(dev)
+        target = torch.from_numpy(index.astype(np.int64).reshape(-1)).to(dev)
+        weight = torch.from_numpy(weight).to(dev, torch.float32)
+        g = torch.Generator(device=dev).manual_seed(int(self.random_state))
+        p = x.shape[1]
+        # one start for all leaves: they part where their rows differ
+        first = torch.randn(1, self.n_hidden, p, generator=g, device=dev) * p ** -0.5
+        self._w = first.expand(self.n_leaves_, -1, -1).contiguous()
+        self._head = torch.randn(K, self.n_hidden, generator=g, device=dev) * 0.1 * self.n_hidden ** -0.5
+        w, head = self._w.to(dt), self._head.to(dt)
+        dw, dhead = torch.empty_like(w), torch.empty_like(head)
+        clip = linear.GradClip([dw, dhead])
+        self.loss_history_ = []
+        for _ in range(self.n_epochs):
+            total = torch.zeros((), dtype=torch.float64, device=dev)
+            shuffled = torch.randperm(len(x), generator=g, device=dev)
+            for at in range(0, len(x), self.batch_size):
+                rows, offsets = self._by_leaf(shuffled[at:at + self.batch_size], leaf)
+                xb, yb = x[rows], target[rows]
+                c = weight[yb]
+                h = linear.leaf_linear(xb, w, offsets)
+                loss, lse = linear.softmax_xent(h, head, yb)
+                dh, _ = linear.softmax_xent_grad(h, head, yb, lse, c / c.sum(), dw_out=dhead)
+                linear.leaf_linear_grad(xb, w, offsets, dh, want_dx=False, dw_out=dw)
+                clip.clip(self.max_norm)
+                for master, copy, grad in ((self._w, w, dw), (self._head, head, dhead)):
+                    master.add_(grad.float(), alpha=-self.learning_rate)
+                    copy.copy_(master)
+                total += loss.sum(dtype=torch.float64)
+            self.loss_history_.append(float(total) / len(x))
+        return self
+
+    # -- answers ------------------------------------------------------------
+    def _hidden(self, X):
+        """Blocks of (rows of X, their hidden rows)."""
+        import torch
+
+        from . import linear
+        if not hasattr(self, '_w'):
+            raise ValueError("This LeafLinearClassifier instance is not fitted yet.")
+        X = self._check(X)
+        if X.shape[1] != self.n_features_in_:
+            raise ValueError(f"X has {X.shape[1]} features; the model has {self.n_features_in_}")
+        route, _ = self._routes(X)
+        w = self._w.to(getattr(torch, self.dtype))
+        for at in range(0, len(X), 1 << 16):
+            x = self._features(X[at:at + (1 << 16)])
+            leaf = torch.from_numpy(route[at:at + (1 << 16)].astype(np.int64)).to(x.device)
+            rows, offsets = self._by_leaf(torch.arange(len(x), device=x.device), leaf)
+            yield at + rows, linear.leaf_linear(x[rows], w, offsets)
+
+    def predict_proba(self, X):
+        """Class probabilities [n, classes] (float64)."""
+        import torch
+        out = np.empty((len(X), len(self.classes_) if hasattr(self, 'classes_') else 0))
+        for rows, h in self._hidden(X):
+            head = self._head.to(h.dtype).double()
+            out[rows.cpu().numpy()] = torch.softmax(h.double() @ head.T, 1).cpu().numpy()
+        return out
+
+    def predict(self, X):
+        return self.classes_[np.argmax(self.predict_proba(X), axis=1)]
+
+    def log_loss(self, X, y):
+        """Mean log-loss of the labels, without the n x classes matrix of
+        probabilities; labels that fit() did not see raise KeyError."""
+        import torch
+
+        from . import linear
+        y = np.asarray(y)
+        if len(y) != len(X):
+            raise ValueError(f"X has {len(X)} rows but y has {len(y)}")
+        total = 0.0
+        for rows, h in self._hidden(X):
+            labels = y[rows.cpu().numpy()]
+            index = np.minimum(np.searchsorted(self.classes_, labels), len(self.classes_) - 1)
+            if np.any(self.classes_[index] != labels):
+                raise KeyError("y holds a label that fit() did not see")
+            loss, _ = linear.softmax_xent(h, self._head.to(h.dtype), torch.from_numpy(index.astype(np.int64)).to(h.device))
+            total += float(loss.sum(dtype=torch.float64))
+        return total / len(y)

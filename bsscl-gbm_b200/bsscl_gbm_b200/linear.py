@@ -115,11 +115,13 @@ def softmax_xent(x, w, target):
     return loss, lse
 
 
-def softmax_xent_grad(x, w, target, lse, grad_loss, want_dx=True, want_dw=True):
+def softmax_xent_grad(x, w, target, lse, grad_loss, want_dx=True, want_dw=True, dw_out=None):
     """Gradients ``(dx, dw)`` of ``sum(grad_loss * loss)`` in the operands'
     type; lse as :func:`softmax_xent` returned it, grad_loss float32 [n].
     Ignored rows get dx = 0 and add nothing to dw.  ``want_dx=False`` /
-    ``want_dw=False`` give None in that place and save its product."""
+    ``want_dw=False`` give None in that place and save its product;
+    ``dw_out`` (of w's shape and type, rows contiguous) takes dw, so that a :class:`GradClip`
+    made once for it stays good."""
     n, d, ldx = _matrix(x, "x")
     v, dw, ldw = _matrix(w, "w", x)
     if d != dw:
@@ -131,14 +133,23 @@ def softmax_xent_grad(x, w, target, lse, grad_loss, want_dx=True, want_dw=True):
         raise ValueError("neither dx nor dw is wanted")
     px, pw, device = x.data_ptr(), w.data_ptr(), x.device
     dx = x.new_empty((n, d)) if want_dx else None
-    dw = x.new_empty((v, d)) if want_dw else None
+    lddw = d
+    if not want_dw:
+        dw = None
+    elif dw_out is None:
+        dw = x.new_empty((v, d))
+    else:
+        dw = dw_out
+        rows, cols, lddw = _matrix(dw, "dw_out", x)
+        if (rows, cols) != (v, d):
+            raise ValueError(f"dw_out must have shape ({v}, {d}), got ({rows}, {cols})")
     if n == 0 and not want_dw:
         return dx, dw
     L = lib()
     size = L.gbm_softmax_xent_workspace(n, d, v, 1, _in_place(px, ldx, pw, ldw))
     ws = _workspace(size, device)
     _call(L.gbm_softmax_xent_grad, device, px, ldx, pw, ldw, _TYPES[x.dtype], n, d, v, y, z, c, dx.data_ptr() if want_dx and n else None, d,
-          dw.data_ptr() if want_dw else None, d, ws.data_ptr(), size)
+          dw.data_ptr() if want_dw else None, lddw, ws.data_ptr(), size)
     return dx, dw
 
 
@@ -174,17 +185,20 @@ def leaf_linear(x, w, offsets, out=None):
     if n == 0:
         return y
     L = lib()
-    size = L.gbm_leaf_linear_workspace(n, e, din, dout, 0, _in_place(px, ldx, pw, din))
-    ws = _workspace(size, device) if size else None
+    size, ws = 0, None
+    if not _in_place(px, ldx, pw, din):
+        size = L.gbm_leaf_linear_workspace(n, e, din, dout, 0, 0)
+        ws = _workspace(size, device)
     _call(L.gbm_leaf_linear, device, px, ldx, pw, off, _TYPES[x.dtype], n, e, din, dout, y.data_ptr(), ldy, int(out is None),
           ws.data_ptr() if size else None, size)
     return y
 
 
-def leaf_linear_grad(x, w, offsets, dy, want_dx=True, want_dw=True):
+def leaf_linear_grad(x, w, offsets, dy, want_dx=True, want_dw=True, dw_out=None):
     """Gradients ``(dx, dw)`` of :func:`leaf_linear` in the operands' type:
     ``dx[r] = w[g].T @ dy[r]`` (0 in rows that no leaf has) and ``dw[g]`` the
-    sum of ``outer(dy[r], x[r])`` over leaf g's rows (0 for an empty leaf)."""
+    sum of ``outer(dy[r], x[r])`` over leaf g's rows (0 for an empty leaf).
+    ``dw_out`` (contiguous, of w's shape and type) takes dw."""
     n, ldx, e, dout, din, off = _leaf_args(x, w, offsets)
     rows, cols, lddy = _matrix(dy, "dy", x)
     if (rows, cols) != (n, dout):
@@ -193,7 +207,14 @@ def leaf_linear_grad(x, w, offsets, dy, want_dx=True, want_dw=True):
         raise ValueError("neither dx nor dw is wanted")
     px, pw, pg, device = x.data_ptr(), w.data_ptr(), dy.data_ptr(), x.device
     dx = x.new_empty((n, din)) if want_dx else None
-    dw = x.new_empty((e, dout, din)) if want_dw else None
+    if not want_dw:
+        dw = None
+    elif dw_out is None:
+        dw = x.new_empty((e, dout, din))
+    else:
+        dw = dw_out
+        if not isinstance(dw, torch.Tensor) or dw.shape != w.shape or dw.dtype is not w.dtype or dw.device != w.device or not dw.is_contiguous():
+            raise ValueError("dw_out must be contiguous and have w's shape, type and device")
     if n == 0 and not want_dw:
         return dx, dw
     L = lib()

@@ -646,6 +646,26 @@ def test_python_refusals_need_no_gpu(built_lib):
 
 
 @gpu
+def test_gradients_into_the_callers_buffers():
+    from bsscl_gbm_b200 import linear
+    s = _problem(5)
+    y = linear.leaf_linear(s["x"], s["w"], s["off"])
+    _, lse = linear.softmax_xent(y, s["head"], s["target"])
+    want = linear.softmax_xent_grad(y, s["head"], s["target"], lse, s["c"])
+    hold = torch.full((700, 80), 3.0, dtype=torch.bfloat16, device="cuda")
+    got = linear.softmax_xent_grad(y, s["head"], s["target"], lse, s["c"], dw_out=hold[:, 4:76])
+    assert torch.equal(got[0], want[0]) and torch.equal(hold[:, 4:76], want[1]) and (hold[:, :4] == 3).all() and (hold[:, 76:] == 3).all()
+    want = linear.leaf_linear_grad(s["x"], s["w"], s["off"], want[0])
+    dw = torch.empty_like(s["w"])
+    got = linear.leaf_linear_grad(s["x"], s["w"], s["off"], got[0], want_dx=False, dw_out=dw)
+    assert got[0] is None and got[1] is dw and torch.equal(dw, want[1])
+    with pytest.raises(ValueError, match="dw_out"):
+        linear.leaf_linear_grad(s["x"], s["w"], s["off"], y, dw_out=dw[:2])
+    with pytest.raises(ValueError, match="dw_out"):
+        linear.softmax_xent_grad(y, s["head"], s["target"], lse, s["c"], dw_out=hold)
+
+
+@gpu
 def test_python_refusals():
     from bsscl_gbm_b200 import linear
     t = torch.bfloat16
