@@ -87,6 +87,11 @@ def _in_place(p, ldp, q, ldq):
     return 0 if (p | q) & 15 or (ldp | ldq) & 7 else 1
 
 
+def _empty_like(a, contiguous):
+    """An uninitialised contiguous tensor of a's shape and type (empty_like takes half of empty's time)."""
+    return torch.empty_like(a) if contiguous else a.new_empty(a.shape)
+
+
 def _workspace(size, device):
     """Workspace of the current stream's pool, so that calls on two streams
     (and two captured graphs) never share one."""
@@ -107,7 +112,7 @@ def softmax_xent(x, w, target):
     y = _vector(target, "target", torch.int64, n, x)
     px, pw, device = x.data_ptr(), w.data_ptr(), x.device
     loss = torch.empty(n, dtype=torch.float32, device=device)
-    lse = loss.new_empty(n)
+    lse = torch.empty_like(loss)
     L = lib()
     size = L.gbm_softmax_xent_workspace(n, d, v, 0, _in_place(px, ldx, pw, ldw))
     ws = _workspace(size, device) if size else None
@@ -132,12 +137,12 @@ def softmax_xent_grad(x, w, target, lse, grad_loss, want_dx=True, want_dw=True, 
     if not (want_dx or want_dw):
         raise ValueError("neither dx nor dw is wanted")
     px, pw, device = x.data_ptr(), w.data_ptr(), x.device
-    dx = x.new_empty((n, d)) if want_dx else None
+    dx = _empty_like(x, ldx == d) if want_dx else None
     lddw = d
     if not want_dw:
         dw = None
     elif dw_out is None:
-        dw = x.new_empty((v, d))
+        dw = _empty_like(w, ldw == d)
     else:
         dw = dw_out
         rows, cols, lddw = _matrix(dw, "dw_out", x)
@@ -206,11 +211,11 @@ def leaf_linear_grad(x, w, offsets, dy, want_dx=True, want_dw=True, dw_out=None)
     if not (want_dx or want_dw):
         raise ValueError("neither dx nor dw is wanted")
     px, pw, pg, device = x.data_ptr(), w.data_ptr(), dy.data_ptr(), x.device
-    dx = x.new_empty((n, din)) if want_dx else None
+    dx = _empty_like(x, ldx == din) if want_dx else None
     if not want_dw:
         dw = None
     elif dw_out is None:
-        dw = x.new_empty((e, dout, din))
+        dw = torch.empty_like(w)
     else:
         dw = dw_out
         if not isinstance(dw, torch.Tensor) or dw.shape != w.shape or dw.dtype is not w.dtype or dw.device != w.device or not dw.is_contiguous():

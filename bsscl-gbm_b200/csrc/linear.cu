@@ -164,6 +164,31 @@ struct PackJob {
     int64_t chunks() const { return rows * (ldp / 8); }
 };
 
+// The 16 bytes at (r, c) of a packed copy.
+__device__ __forceinline__ void pack_chunk(const PackJob &j, int64_t r, int64_t c) {
+    uint4 q = make_uint4(0, 0, 0, 0);
+    bool has = true;
+    if (j.target) {
+        const int64_t y = j.target[r];
+        has = y >= 0 && y < j.v;
+    }
+    if (has) {
+        const uint16_t *s = j.src + r * j.ld + c;
+        if (j.vec && c + 8 <= j.cols) {
+            q = *(const uint4 *)s;
+        } else {
+            uint32_t h[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) h[e] = c + e < j.cols ? s[e] : 0;
+            q = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+        }
+    }
+    *(uint4 *)(j.dst + r * j.ldp + c) = q;
+}
+
+// The power of two that takes m to at most 2^14.
+__device__ __forceinline__ int scale_exponent(float m) { return m > 0.f && m < INFINITY ? min(max(14 - (ilogbf(m) + 1), -100), 100) : 0; }
+
 // What a call's other launches need first: copies of operands, tickets set to
 // 0, and the power of two that takes the largest |grad_loss| of the rows that
 // count to at most 2^14, half precision's range (scale[0], its inverse in
@@ -195,8 +220,7 @@ __global__ void __launch_bounds__(256) k_prep(const __grid_constant__ Prep p) {
         __syncthreads();
         if (threadIdx.x) return;
         for (int k = 1; k < 8; k++) m = fmaxf(m, red[k]);
-        int e = 0;
-        if (m > 0.f && m < INFINITY) e = min(max(14 - (ilogbf(m) + 1), -100), 100);
+        const int e = scale_exponent(m);
         p.scale[0] = ldexpf(1.f, e);
         p.scale[1] = ldexpf(1.f, -e);
         return;
@@ -209,24 +233,7 @@ __global__ void __launch_bounds__(256) k_prep(const __grid_constant__ Prep p) {
         for (int64_t i = first; i < total; i += step) {
             // 32 bits where they do: a 64-bit division costs more than the copy
             const int64_t r = total >> 31 ? i / per : (int64_t)((uint32_t)i / (uint32_t)per), c = (i - r * per) * 8;
-            uint4 q = make_uint4(0, 0, 0, 0);
-            bool has = true;
-            if (j.target) {
-                const int64_t y = j.target[r];
-                has = y >= 0 && y < j.v;
-            }
-            if (has) {
-                const uint16_t *s = j.src + r * j.ld + c;
-                if (j.vec && c + 8 <= j.cols) {
-                    q = *(const uint4 *)s;
-                } else {
-                    uint32_t h[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) h[e] = c + e < j.cols ? s[e] : 0;
-                    q = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-                }
-            }
-            *(uint4 *)(j.dst + r * j.ldp + c) = q;
+            pack_chunk(j, r, c);
         }
     }
 }
@@ -369,7 +376,7 @@ struct XentStats {
     const int64_t *target;
     float2 *part;
     float *ly, *loss, *lse;
-    __device__ void rest(int, int, int) const {}
+    template <class S> __device__ void rest(S &, int, int, int) const {}
     __device__ int64_t rows(const tc::Tile &t, const tc::Place &p) const { return t.m0 + p.row < t.mend ? target[t.m0 + p.row] : -1; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int64_t y, State &st, uint32_t addr, R release) const {
         const int row = t.m0 + p.row, c0 = p.half * 128, left = t.nend - t.n0 - c0;    // columns of this half that exist
@@ -474,22 +481,48 @@ template <class T> struct XentG {
     const float *lse, *grad_loss, *scale;
     T *g;
     int64_t ldg, part;  // row stride; from the leading to the trailing part (0: one part)
-    using State = tc::None;
+    // where no launch went before that did them: the copy of x with the
+    // ignored rows as zeros (rows 0: done), the tickets, and half precision's
+    // scale (find_scale)
+    PackJob copy;
+    uint32_t *tickets;
+    int n_tickets;
+    float *find_scale;
+    struct State {
+        float scale;
+    };
+    __device__ void rest(State &st, int warp, int warps, int lane) const {
+        st.scale = scale ? *scale : 1.f;
+        if (find_scale) {
+            float m = 0.f;
+#pragma unroll 8
+            for (int i = lane; i < dense.m; i += 32) {
+                const int64_t y = target[i];
+                m = fmaxf(m, y >= 0 && y < v ? fabsf(grad_loss[i]) : 0.f);
+            }
+            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+            const int e = scale_exponent(m);
+            st.scale = ldexpf(1.f, e);
+            if (warp == 0 && lane == 0) find_scale[0] = st.scale, find_scale[1] = ldexpf(1.f, -e);
+        }
+        for (int i = warp * 32 + lane; i < n_tickets; i += warps * 32) tickets[i] = 0;
+        for (int64_t r = warp; r < copy.rows; r += warps)
+            for (int64_t c = lane * 8; c < copy.ldp; c += 256) pack_chunk(copy, r, c);
+    }
     struct Rows {
         int64_t y;
         float c, z;
     };
-    __device__ void rest(int, int, int) const {}
     __device__ Rows rows(const tc::Tile &t, const tc::Place &p) const {
         const int row = t.m0 + p.row;
         Rows r{-1, 0.f, 0.f};
-        if (row < t.mend) r = {target[row], grad_loss[row] * (scale ? *scale : 1.f), lse[row] * kLog2e};
+        if (row < t.mend) r = {target[row], grad_loss[row], lse[row] * kLog2e};
         return r;
     }
-    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, Rows r, tc::None &, uint32_t addr, R release) const {
+    template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, Rows r, State &st, uint32_t addr, R release) const {
         const int h0 = p.half * 128;
         const int64_t y = r.y;
-        const float c = r.c, z = r.z;
+        const float c = r.c * st.scale, z = r.z;
         const bool has = y >= 0 && y < v, all = __all_sync(~0u, has);
         const int64_t off = y - c0 - t.n0 - h0;
         const int yc = has && off >= 0 && off < 128 ? (int)off : -1;
@@ -656,7 +689,7 @@ template <class T, int BN> struct XentPair {
     Dense dense[2];
     Sink<T> sink[2];
     int first, laps;
-    __device__ void rest(int, int, int) const {}
+    template <class S> __device__ void rest(S &, int, int, int) const {}
     using State = tc::None;
     __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, tc::None &, uint32_t addr, R release) const {
@@ -833,22 +866,41 @@ Err xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_
     constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
     const XentPlan pl(n, d, v);
     const XentGrad q(ws, n, d, v, tma_rows(x, ldx) && tma_rows(w, ldw));
-    Prep prep;
     // rows that count, zeros in the others': an ignored row's features must not reach dw
-    add_pack(prep, {x, d, n, ldx}, q.x, pl.dp, target, v);
-    const View xs{q.x, d, n, pl.dp}, wv = readable(prep, {w, d, v, ldw}, q.w);
-    if (pl.sx > 1 || pl.sw > 1) prep.tickets = q.tickets, prep.n_tickets = (int)pl.tickets();
-    if (!bf16) prep.grad_loss = grad_loss, prep.target = target, prep.n = n, prep.v = v, prep.scale = q.scale;
-    Err e = run_prep(prep, st);
-    const float *scale = prep.scale;
+    const View xs{q.x, d, n, pl.dp}, given{x, d, n, ldx};
+    const bool tickets = pl.sx > 1 || pl.sw > 1;
+    float *scale = bf16 ? nullptr : q.scale;
+    View xv = given, wv{w, d, v, ldw};
+    PackJob copy{};
+    Err e;
+    // G's own launch makes the copy under its first products, and finds
+    // half precision's scale where one warp reads all rows in about a microsecond
+    const bool own = tma_rows(x, ldx) && tma_rows(w, ldw) && (bf16 || n <= 1024);
+    if (own) {
+        if (dw) {
+            Prep one;
+            add_pack(one, given, q.x, pl.dp, target, v);
+            copy = one.job[0];
+        }
+    } else {
+        Prep prep;
+        add_pack(prep, given, q.x, pl.dp, target, v);
+        xv = xs;
+        wv = readable(prep, wv, q.w);
+        if (tickets) prep.tickets = q.tickets, prep.n_tickets = (int)pl.tickets();
+        if (!bf16) prep.grad_loss = grad_loss, prep.target = target, prep.n = n, prep.v = v, prep.scale = q.scale;
+        e = run_prep(prep, st);
+    }
     T *g = (T *)q.g;
     for (int64_t c = 0; c < v && !e.bad(); c += pl.pc) {
         const int64_t pc = std::min(pl.pc, v - c);
         View wp = wv;
         wp.p = (const char *)wv.p + c * wv.ld * 2;
         wp.rows = pc;
-        XentG<T> og{Dense(n, pc, d, 256), c, v, target, lse, grad_loss, scale, g, pl.ldg, pl.parts > 1 ? n * pl.ldg : 0};
-        const View xw[2] = {xs, wp};
+        const bool first = own && c == 0;
+        XentG<T> og{Dense(n, pc, d, 256), c, v, target, lse, grad_loss, first ? nullptr : scale, g, pl.ldg, pl.parts > 1 ? n * pl.ldg : 0,
+                    first ? copy : PackJob{}, q.tickets, first && tickets ? (int)pl.tickets() : 0, first ? scale : nullptr};
+        const View xw[2] = {xv, wp};
         e = launch(xw, og, bf16, og.dense.units(), st);
         if (e.bad()) break;
         e = pl.bn == 128 ? xent_pair<T, 128>(pl, q, xs, wp, scale, n, d, v, c, pc, target, dx, lddx, dw, lddw, st)
@@ -957,7 +1009,7 @@ template <class T> struct LeafRows {
     using Iter = LeafIter;
     Leaves leaves;
     LeafOut<T> y;
-    __device__ void rest(int warp, int warps, int lane) const {
+    __device__ void rest(tc::None &, int warp, int warps, int lane) const {
         if (y.rest) leaf_rest(leaves, y.out, y.ld, warp, warps, lane);
     }
     using State = tc::None;
@@ -1048,7 +1100,7 @@ template <class T> struct LeafPair {
     int dout, splits, mt, nt;
     tc::Div per, tiles, cols;    // units of one leaf's dw, its tiles, tiles side by side
     Sink<T> sink;          // of the (groups * dout) x din matrix of all leaves' dw; out null: not wanted
-    __device__ void rest(int warp, int warps, int lane) const {
+    __device__ void rest(tc::None &, int warp, int warps, int lane) const {
         if (dx.out && dx.rest) leaf_rest(leaves, dx.out, dx.ld, warp, warps, lane);
     }
     using State = tc::None;

@@ -527,7 +527,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         p.dead = dead;
         typename Op::State state{};
         // what no tile writes, while the first loads are on their way
-        op.rest((warp - 2) + kEpiWarps * (int)blockIdx.x, kEpiWarps * (int)gridDim.x, lane);
+        op.rest(state, (warp - 2) + kEpiWarps * (int)blockIdx.x, kEpiWarps * (int)gridDim.x, lane);
         int n = 0;
         typename Op::Iter it(op, cid, ncl);
         Tile t;
