@@ -29,6 +29,7 @@ from ._lib import ERRORS, GBM_OK, lib
 _TYPES = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}     # GBM_TYPE_*
 _local = threading.local()
 _stream_of = torch._C._cuda_getCurrentRawStream    # current_stream(i).cuda_stream without its wrapper object (3 us)
+_current = torch._C._cuda_getDevice
 
 
 def _call(fn, device, *args):
@@ -38,7 +39,7 @@ def _call(fn, device, *args):
     except AttributeError:
         err = _local.err = C.create_string_buffer(256)
     i = device.index
-    if i == torch.cuda.current_device():
+    if i == _current():
         rc = fn(*args, _stream_of(i), err, 256)
     else:
         with torch.cuda.device(i):

@@ -114,6 +114,17 @@ def test_xent_sizes(n, d, v, kind):
 
 
 @gpu
+@pytest.mark.parametrize("n,d,v", [(2100, 24, 131073), (19100, 16, 14849)])
+def test_xent_pieces(n, d, v):
+    """More than 512 MB of G: two pieces of classes, dx summed over them (the first case with split sums as well)."""
+    t = torch.bfloat16
+    x, w = _rand((n, d), t, 1), _rand((v, d), t, 2, 2.0 / d ** 0.5)
+    c = torch.rand(n, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda") + 0.25
+    _check_xent(x, w, _targets(n, v, 0.2, 5), c)
+    torch.cuda.empty_cache()
+
+
+@gpu
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 def test_xent_strides(kind):
     """Rows of a wider table, at offsets that are not 16-byte aligned."""
