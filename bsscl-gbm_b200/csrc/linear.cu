@@ -823,8 +823,10 @@ struct XentGrad {
     }
 };
 
+// Sizes whose products of two stay far from 64 bits in every count of bytes (and tiles within 31).
 bool sizes_ok(int64_t n, int64_t d, int64_t v) {
-    return n >= 0 && n <= kMaxDim && d >= 1 && d <= kMaxDim && v >= 1 && v <= kMaxDim;
+    constexpr int64_t kMost = 1LL << 46;
+    return n >= 0 && n <= kMaxDim && d >= 1 && d <= kMaxDim && v >= 1 && v <= kMaxDim && n * d <= kMost && v * d <= kMost && n * v <= kMost;
 }
 
 Err xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, bool bf16, int64_t n, int64_t d, int64_t v, const int64_t *target, float *loss,
@@ -940,12 +942,18 @@ struct Leaves {
 // through 32 leaves at a time: each lane counts one leaf's tiles.
 struct LeafIter {
     uint32_t at, step, base, total, upto;    // tiles before these 32 leaves, in them, in them up to this lane's
-    int first, lo, hi;
+    int first, lo, hi, next_lo, next_hi;     // rows of this lane's leaf, and of its one among the next 32
     template <class Op> __device__ LeafIter(const Op &, int cid, int ncl) : at(cid), step(ncl), base(0), total(0), first(-32) {}
+    template <class Op> __device__ void fetch(const Op &op, int g) {
+        next_lo = next_hi = 0;
+        if (g < op.leaves.groups) leaf_rows(op.leaves.off, g, op.leaves.t, next_lo, next_hi);
+    }
     template <class Op> __device__ void look(const Op &op) {
         const int lane = threadIdx.x % 32, g = first + lane;
-        lo = hi = 0;
-        if (g < op.leaves.groups) leaf_rows(op.leaves.off, g, op.leaves.t, lo, hi);
+        if (first == 0) fetch(op, g);
+        lo = next_lo;
+        hi = next_hi;
+        fetch(op, g + 32);
         upto = (uint32_t)((hi - lo + 255) / 256) * op.leaves.nt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -1493,8 +1501,12 @@ int gbm_softmax_xent_grad(const void *x, int64_t ldx, const void *w, int64_t ldw
     return finish(what, errbuf, errlen);
 }
 
+static bool leaf_ok(int64_t t, int32_t groups, int64_t din, int64_t dout) {
+    return sizes_ok(t, din, dout) && groups >= 1 && groups < 65536 && groups * dout <= kMaxDim && groups * dout * din <= 1LL << 46;
+}
+
 int64_t gbm_leaf_linear_workspace(int64_t t, int32_t groups, int64_t din, int64_t dout, int32_t grad, int32_t in_place) {
-    if (!sizes_ok(t, din, dout) || groups < 1 || groups >= 65536 || groups * dout > kMaxDim) return -1;
+    if (!leaf_ok(t, groups, din, dout)) return -1;
     return LeafWs(nullptr, t, groups, din, dout, grad != 0, in_place != 0).bytes;
 }
 
@@ -1502,7 +1514,7 @@ static int leaf_check(const char *what, const int32_t *offsets, int32_t dtype, i
                       int64_t dout, bool in_place, const void *ws, int64_t ws_bytes, int32_t grad, char *errbuf, int32_t errlen) {
     if (dtype != GBM_TYPE_BF16 && dtype != GBM_TYPE_F16)
         return fail(errbuf, errlen, GBM_ERR_UNSUPPORTED, "%s: type %d is neither bf16 nor f16", what, dtype);
-    if (!sizes_ok(t, din, dout) || groups < 1 || groups >= 65536 || groups * dout > kMaxDim)
+    if (!leaf_ok(t, groups, din, dout))
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: sizes t=%lld groups=%d din=%lld dout=%lld out of range", what,
                     (long long)t, groups, (long long)din, (long long)dout);
     if (!offsets || !aligned(offsets, 4)) return fail(errbuf, errlen, GBM_ERR_ARG, "%s: offsets null or not aligned", what);

@@ -402,7 +402,8 @@ enum {
  * in `dtype` (GBM_TYPE_BF16 or GBM_TYPE_F16); l_ik = x_i . w_k is summed in
  * 32 bits.  lse [n] f32 gets log sum_k exp l_ik, and loss [n] f32 gets
  * lse_i - l_i,target_i.  A row whose target is outside 0..v-1 is ignored: its loss is 0
- * (its lse is still computed).  n >= 0, d and v >= 1, each below 2^31 - 512.
+ * (its lse is still computed).  n >= 0, d and v >= 1, each below 2^31 - 512,
+ * the product of any two at most 2^46.
  * ws: gbm_softmax_xent_workspace(n, d, v, 0, in_place) bytes, 256-byte aligned. */
 int gbm_softmax_xent(const void *x, int64_t ldx, const void *w, int64_t ldw, int32_t dtype, int64_t n,
                      int64_t d, int64_t v, const int64_t *target, float *loss, float *lse, void *ws,
@@ -437,7 +438,8 @@ int64_t gbm_softmax_xent_workspace(int64_t n, int64_t d, int64_t v, int32_t grad
  * last one are set to 0 when zero_rest is not 0, else left as they were.
  * Offsets that break the rule are clamped into 0..t and a leaf with a
  * negative row count has no rows, so no access leaves the arrays.  t >= 0,
- * groups, din and dout >= 1, groups below 65536, the others below 2^31 - 512.
+ * groups, din and dout >= 1, groups below 65536, the others and groups * dout
+ * below 2^31 - 512, products of two sizes and the elements of w at most 2^46.
  * ws: gbm_leaf_linear_workspace(t, groups, din, dout, 0, in_place) bytes,
  * 256-byte aligned. */
 int gbm_leaf_linear(const void *x, int64_t ldx, const void *w, const int32_t *offsets, int32_t dtype,

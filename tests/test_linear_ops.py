@@ -328,6 +328,54 @@ def test_leaf_bad_offsets_stay_inside():
 
 
 @gpu
+def test_leaf_many_leaves():
+    """Thousands of leaves, most of them empty: more than one look at 32 of them, and than the 2048 that are sorted."""
+    for e in (100, 3000):
+        counts = np.random.default_rng(e).integers(0, 3, e) * (np.random.default_rng(1).random(e) < 0.3)
+        counts[-1] = 5
+        n = int(counts.sum())
+        x, dy, w = _rand((n, 40), torch.bfloat16, 1), _rand((n, 24), torch.bfloat16, 2), _rand((e, 24, 40), torch.bfloat16, 3, 0.2)
+        _check_leaf(x, w, _offsets(counts), dy)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements in one operand: the last rows are where they belong."""
+    from bsscl_gbm_b200 import linear
+    t, n, wide = torch.bfloat16, 140_000, 16_384
+    assert n * wide > 2 ** 31
+    x, w = _rand((n, 8), t, 1), _rand((2, wide, 8), t, 2)
+    off = _offsets([n - 300, 300])
+    y = linear.leaf_linear(x, w, off)
+    for lo, hi, k in ((0, 200, 0), (n - 400, n - 300, 0), (n - 300, n, 1)):
+        want = x[lo:hi].double() @ w[k].double().T
+        _near(y[lo:hi], want, 8 * 2.0 ** -23 * (x[lo:hi].double().abs() @ w[k].double().abs().T) + _u(t) * want.abs(), "y")
+    dx, dw = linear.leaf_linear_grad(x, w, off, y)
+    last = y[n - 300:].double()
+    want = last @ w[1].double()
+    _near(dx[n - 300:], want, wide * 2.0 ** -23 * (last.abs() @ w[1].double().abs()) + _u(t) * want.abs(), "dx")
+    want = last.T @ x[n - 300:].double()
+    _near(dw[1], want, 300 * 2.0 ** -23 * (last.abs().T @ x[n - 300:].double().abs()) + _u(t) * want.abs(), "dw")
+    head = _rand((50, wide), t, 4, 0.01)
+    target = _targets(n, 50, 0.0, 5)
+    loss, lse = linear.softmax_xent(y, head, target)
+    l = last @ head.double().T
+    el = wide * 2.0 ** -23 * (last.abs() @ head.double().abs().T).max(1).values
+    want = torch.logsumexp(l, 1)
+    _near(lse[n - 300:], want, el + 2.0 ** -18 + want.abs() * 2.0 ** -23, "lse")
+    dy, dhead = linear.softmax_xent_grad(y, head, target, lse, torch.ones(n, device="cuda"))
+    linear.status()
+    g = torch.exp(l - want[:, None])
+    g[torch.arange(300, device="cuda"), target[n - 300:]] -= 1.0
+    want = g @ head.double()
+    # G's error: its rounding, and the logits' and lse's
+    eg = g.abs() * (_u(t) + 2.0 ** -18) + (torch.expm1(2 * el) + 2.0 ** -17)[:, None]
+    _near(dy[n - 300:], want, eg @ head.double().abs() + _u(t) * want.abs() + 50 * 2.0 ** -23 * (g.abs() @ head.double().abs()), "dy")
+    del x, w, y, dx, dw, dy, last
+    torch.cuda.empty_cache()
+
+
+@gpu
 def test_leaf_partial_and_empty():
     from bsscl_gbm_b200 import linear
     t = torch.bfloat16
@@ -582,6 +630,8 @@ def test_xent_refusals(L):
     a = list(good)
     a[11] = a[13] = None
     assert _rc(L.gbm_softmax_xent_grad, *a)[0] == ARG
+    assert L.gbm_softmax_xent_workspace((1 << 31) - 600, 1, (1 << 31) - 600, 1, 1) == -1      # counts of bytes stay within 64 bits
+    assert L.gbm_leaf_linear_workspace(10, 65535, 1, 1 << 20, 1, 1) == -1
     assert L.gbm_softmax_xent_workspace(-1, 1, 1, 0, 0) == -1 and L.gbm_softmax_xent_workspace(1, 1, 1 << 31, 1, 1) == -1
 
 
