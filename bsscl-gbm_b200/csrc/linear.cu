@@ -125,13 +125,12 @@ template <class... P, class... A> Err start(void (*kernel)(P...), int64_t blocks
 // each, at most one CTA an SM.  views: A and B, for a launch of two products
 // twice.
 template <class Op> Err launch(const View *views, const Op &op, bool bf16, int64_t units, cudaStream_t st) {
-    using S = tc::Shape<Op::kBN>;
     if (units <= 0) return {};
     if (units > INT_MAX - 1024) return {GBM_ERR_ARG, "more than 2^31 tiles"};
     tc::Maps maps;
     for (int i = 0; i < (Op::kDual ? 4 : 2); i++) {
         const bool mn = i & 1 ? Op::kBMN : Op::kDual ? i == 2 : Op::kAMN;
-        Err e = encode(&maps.m[i], views[i], bf16, mn ? 64 : i & 1 ? Op::kBN / 2 : 128);
+        Err e = encode(&maps.m[i], views[i], bf16, mn ? 64 : 128);
         if (e.bad()) return e;
     }
     static std::atomic<uint64_t> ready;     // devices whose limit for this kernel is set
@@ -139,13 +138,13 @@ template <class Op> Err launch(const View *views, const Op &op, bool bf16, int64
     if (cudaGetDevice(&dev) != cudaSuccess) return {GBM_ERR_CUDA, "no current CUDA device"};
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;
     if (!(ready.load() & bit)) {
-        if (cudaFuncSetAttribute(tc::k_tc<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
+        if (cudaFuncSetAttribute(tc::k_tc<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, tc::kSmem) != cudaSuccess)
             return {GBM_ERR_CUDA, "the device does not have the kernel's shared memory"};
         ready.fetch_or(bit);
     }
     const int64_t clusters = std::min<int64_t>(units, sm_count() / 2);
     if (clusters < 1) return {GBM_ERR_CUDA, "no SMs"};
-    return start(tc::k_tc<Op>, 2 * clusters, tc::kThreads, S::kSmem, st, maps, op, tc::make_idesc(bf16, Op::kBMN, Op::kBN));
+    return start(tc::k_tc<Op>, 2 * clusters, tc::kThreads, tc::kSmem, st, maps, op, tc::make_idesc(bf16, Op::kBMN));
 }
 
 // Whether TMA can read the rows in place: 16-byte boundaries.
@@ -275,20 +274,20 @@ struct Dense {
     int per;           // stages of a part
     tc::Div all, band; // tiles in all, in 8 rows of tiles
     Dense() : m(0), n(0), nkb(0), splits(1), mt(0), nt(0), per(0) {}
-    Dense(int64_t m_, int64_t n_, int64_t k, int bn, int splits_ = 1, int laps = 1)
-        : m((int)m_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK) * laps), splits(splits_), mt((int)((m_ + 255) / 256)), nt((int)((n_ + bn - 1) / bn)),
+    Dense(int64_t m_, int64_t n_, int64_t k, int splits_ = 1, int laps = 1)
+        : m((int)m_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK) * laps), splits(splits_), mt((int)((m_ + 255) / 256)), nt((int)((n_ + 255) / 256)),
           per((nkb + splits_ - 1) / splits_), all((uint32_t)std::min<int64_t>(tiles(), INT_MAX)), band((uint32_t)std::min<int64_t>(8LL * nt, INT_MAX)) {}
     int64_t tiles() const { return (int64_t)mt * nt; }
     int64_t units() const { return tiles() * splits; }
     // A tile's place is found in 32 bits; launch() refuses more units.
-    template <int BN> __device__ void place(uint32_t at, tc::Tile &t) const {
+    __device__ void place(uint32_t at, tc::Tile &t) const {
         const uint32_t part = splits > 1 ? all(at) : 0, i = at - part * all.d;
         const uint32_t block = band(i), rest = i - block * band.d, wide = min(8u, mt - block * 8);
         const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
-        t.m0 = t.am = (int)(tm * 256);
-        t.n0 = (int)(tn * BN);
+        t.m0 = (int)(tm * 256);
+        t.n0 = (int)(tn * 256);
         t.mend = min(m - t.m0, 256) + t.m0;
-        t.nend = min(n - t.n0, BN) + t.n0;
+        t.nend = min(n - t.n0, 256) + t.n0;
         t.k0 = 0;
         t.q0 = min((int)part * per, nkb);
         t.nkb = min(per, nkb - t.q0);
@@ -304,7 +303,7 @@ struct DenseIter {
     template <class Op> __device__ DenseIter(const Op &, int cid, int ncl) : at(cid), step(ncl) {}
     template <class Op> __device__ bool next(const Op &op, tc::Tile &t) {
         if (at >= (uint32_t)(op.dense.mt * op.dense.nt) * op.dense.splits) return false;
-        op.dense.template place<Op::kBN>(at, t);
+        op.dense.place(at, t);
         at += step;
         return true;
     }
@@ -342,7 +341,6 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 // rows' loss and lse at once.  One lane of the epilogue has one row, so no
 // exchange between lanes is needed.
 struct XentStats {
-    static constexpr int kBN = 256;
     static constexpr bool kAMN = false, kBMN = false, kTail = false, kDual = false;
     static constexpr int laps = 1;
     struct Iter {
@@ -352,15 +350,15 @@ struct XentStats {
             const Dense &g = op.dense;
             if (!op.whole) {
                 if (at >= (uint32_t)(g.mt * g.nt)) return false;
-                g.place<kBN>(at, t);
+                g.place(at, t);
                 at += step;
                 return true;
             }
             if (at >= (uint32_t)g.mt) return false;
-            t.m0 = t.am = (int)at * 256;
-            t.n0 = (int)c * kBN;
+            t.m0 = (int)at * 256;
+            t.n0 = (int)c * 256;
             t.mend = min(g.m - t.m0, 256) + t.m0;
-            t.nend = min(g.n - t.n0, kBN) + t.n0;
+            t.nend = min(g.n - t.n0, 256) + t.n0;
             t.k0 = t.q0 = t.bz = t.tail = t.kind = t.aux = 0;
             t.nkb = g.nkb;
             if (++c == (uint32_t)g.nt) c = 0, at += step;
@@ -379,19 +377,20 @@ struct XentStats {
     template <class S> __device__ void rest(S &, int, int, int) const {}
     __device__ int64_t rows(const tc::Tile &t, const tc::Place &p) const { return t.m0 + p.row < t.mend ? target[t.m0 + p.row] : -1; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int64_t y, State &st, uint32_t addr, R release) const {
-        const int row = t.m0 + p.row, c0 = p.half * 128, left = t.nend - t.n0 - c0;    // columns of this half that exist
+        const int row = t.m0 + p.row, c0 = p.first(), left = min(t.nend - t.n0 - c0, p.wide);    // columns of this half that exist
         const bool in = row < t.mend;
         const int64_t off = y - t.n0 - c0;
-        const int yc = off >= 0 && off < min(128, left) ? (int)off : -1;
+        const int yc = off >= 0 && off < left ? (int)off : -1;
         const tc::F2 log2e = tc::f2(kLog2e, kLog2e);
         const bool fresh = !whole || t.n0 == 0;
         float m = fresh ? -INFINITY : st.m, s = fresh ? 0.f : st.s, z = fresh ? 0.f : st.ly;
+        if (t.mend - t.m0 <= p.row - p.lane || left <= 0) release();      // no rows, or no columns, of this warp's
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
+        for (int c = 0; c < left && t.mend - t.m0 > p.row - p.lane; c += 32) {
             float v[32];
             tc::tmem_ld32(addr + c, v);
             tc::tmem_wait(v);
-            if (c == 96) release();
+            if (c + 32 >= left) release();
             if (__any_sync(~0u, yc >= c && yc < c + 32)) {
 #pragma unroll
                 for (int i = 0; i < 32; i++) z = yc == c + i ? v[i] : z;
@@ -421,7 +420,7 @@ struct XentStats {
         }
         if (!whole) {
             if (yc >= 0) ly[row] = z;
-            if (in) part[((int64_t)(t.n0 / kBN) * 2 + p.half) * dense.m + row] = make_float2(m, s);
+            if (in) part[((int64_t)(t.n0 / 256) * 2 + p.half) * dense.m + row] = make_float2(m, s);
             return;
         }
         st.m = m;
@@ -471,7 +470,6 @@ __global__ void __launch_bounds__(256) k_xent_join(const float2 *__restrict__ pa
 // times the scale, rounded to the products' type.  With two parts what the
 // rounding leaves is rounded too and follows in a second matrix.
 template <class T> struct XentG {
-    static constexpr int kBN = 256;
     static constexpr bool kAMN = false, kBMN = false, kTail = false, kDual = false;
     static constexpr int laps = 1;
     using Iter = DenseIter;
@@ -520,12 +518,12 @@ template <class T> struct XentG {
         return r;
     }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, Rows r, State &st, uint32_t addr, R release) const {
-        const int h0 = p.half * 128;
+        const int h0 = p.first();
         const int64_t y = r.y;
         const float c = r.c * st.scale, z = r.z;
         const bool has = y >= 0 && y < v, all = __all_sync(~0u, has);
         const int64_t off = y - c0 - t.n0 - h0;
-        const int yc = has && off >= 0 && off < 128 ? (int)off : -1;
+        const int yc = has && off >= 0 && off < p.wide ? (int)off : -1;
         const int row0 = t.m0 + p.row - p.lane;
         auto value = [&](float (&x)[32], int col) {
             const bool here = __any_sync(~0u, yc >= col && yc < col + 32);
@@ -549,8 +547,8 @@ template <class T> struct XentG {
         T *out = g + (int64_t)row0 * ldg + t.n0 + h0;
         const int rows = t.mend - row0, cols = t.nend - t.n0 - h0;
         if (part) {
-            tc::store_tile<T, 128>(p, addr, out, ldg, rows, cols, 8, false, value, [] {});
-            tc::store_tile<T, 128>(
+            tc::store_tile<T>(p, addr, out, ldg, rows, cols, 8, false, value, [] {});
+            tc::store_tile<T>(
                 p, addr, out + part, ldg, rows, cols, 8, false,
                 [&](float (&x)[32], int col) {
                     value(x, col);
@@ -559,7 +557,7 @@ template <class T> struct XentG {
                 },
                 release);
         } else {
-            tc::store_tile<T, 128>(p, addr, out, ldg, rows, cols, 8, false, value, release);
+            tc::store_tile<T>(p, addr, out, ldg, rows, cols, 8, false, value, release);
         }
     }
 };
@@ -583,9 +581,9 @@ template <class T> struct Sink {
 };
 
 // f32 sums of a warp's 32 x COLS block: its place in acc.
-template <int COLS, class T, class R>
+template <class T, class R>
 __device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, const tc::Tile &t, const tc::Place &p, uint32_t addr, R release, int tile) {
-    const int row = t.m0 + p.row, row0 = row - p.lane, h0 = p.half * COLS, cols = t.nend - t.n0 - h0;
+    const int row = t.m0 + p.row, row0 = row - p.lane, h0 = p.first(), cols = t.nend - t.n0 - h0;
     const float scale = k.scale ? k.scale[1] : 1.f;
     bool has = row < t.mend;
     if (k.target && has) {
@@ -597,8 +595,12 @@ __device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, c
     float *q = k.acc ? k.acc + ((int64_t)t.aux * m + row) * k.ldacc + t.n0 + h0 : nullptr;
     // ldacc is a multiple of 64: whole groups of 32 columns fit
     const auto mine = [&](int c) { return row < t.mend && c < cols; };
+    if (row0 >= t.mend) {
+        release();
+        return;
+    }
     if (!k.acc || (one && k.last)) {
-        tc::store_tile<T, COLS>(
+        tc::store_tile<T>(
             p, addr, out, k.ld, t.mend - row0, cols, k.width, t.nkb == 0,
             [&](float (&x)[32], int c) {
                 if (k.acc && k.add && mine(c)) {
@@ -615,7 +617,7 @@ __device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, c
         return;
     }
 #pragma unroll 1
-    for (int c = 0; c < COLS; c += 32) {
+    for (int c = 0; c < p.wide; c += 32) {
         float x[32];
         if (t.nkb) {
             tc::tmem_ld32(addr + c, x);
@@ -624,7 +626,7 @@ __device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, c
 #pragma unroll
             for (int i = 0; i < 32; i++) x[i] = 0.f;
         }
-        if (c == COLS - 32) release();
+        if (c == p.wide - 32) release();
         if (mine(c)) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -649,7 +651,7 @@ __device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, c
     __threadfence();
     const float *first = k.acc + (int64_t)row * k.ldacc + t.n0 + h0;
     const int64_t step = (int64_t)m * k.ldacc;
-    tc::store_tile<T, COLS>(
+    tc::store_tile<T>(
         p, addr, out, k.ld, t.mend - row0, cols, k.width, true,
         [&](float (&x)[32], int c) {
             if (!mine(c)) return;
@@ -669,8 +671,7 @@ __device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, c
 // dx = G w (A K-major) and dw = G^T x (A's m axis contiguous), B's n axis
 // contiguous in both, as one pool of tiles: neither alone fills its last wave.
 // The product with the longer k axis goes first.
-template <class T, int BN> struct XentPair {
-    static constexpr int kBN = BN;
+template <class T> struct XentPair {
     static constexpr bool kAMN = false, kBMN = true, kTail = false, kDual = true;
     struct Iter : tc::Snake {
         __device__ Iter(const XentPair &, int cid, int ncl) : tc::Snake(cid, ncl) {}
@@ -680,7 +681,7 @@ template <class T, int BN> struct XentPair {
             if (at >= u0 + u1) return false;
             const int kind = op.first ? at < u1 : at >= u0;
             const uint32_t i = op.first ? (kind ? at : at - u1) : (kind ? at - u0 : at);
-            op.dense[kind].template place<BN>(i, t);
+            op.dense[kind].place(i, t);
             t.kind = kind;
             step();
             return true;
@@ -694,7 +695,7 @@ template <class T, int BN> struct XentPair {
     __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, tc::None &, uint32_t addr, R release) const {
         const Dense &g = dense[t.kind];
-        sink_tile<BN / 2>(sink[t.kind], g.m, g.splits, t, p, addr, release, (t.m0 / 256) * g.nt + t.n0 / BN);
+        sink_tile(sink[t.kind], g.m, g.splits, t, p, addr, release, (t.m0 / 256) * g.nt + t.n0 / 256);
     }
 };
 
@@ -710,6 +711,9 @@ double chain(int64_t u0, int64_t l0, int64_t u1, int64_t l1) {
     // at least the mean; a cluster of the fullest wave, which holds as many long units as fit
     return (double)std::max(all, std::min(r0, waves) * l0 + (waves - std::min(r0, waves)) * l1);
 }
+
+// A stage's time against a 256 x 256 tile's, for results of d columns.
+double stage_cost(int64_t d) { return d > 128 ? 1.0 : d > 64 ? 0.5 : 0.3; }
 
 // Parts of both products' k axes (tx tiles of kx stages, tw of kw): those that
 // end first.  Split sums cost some 5 us of fences, tickets and reading back,
@@ -741,7 +745,6 @@ struct XentPlan {
     int64_t pc;        // classes of a piece, a multiple of 256 unless there is one piece
     int64_t ldg;       // row stride of G
     int64_t ldacc;
-    int bn;            // columns of the products' tiles
     int parts;         // of G: see below
     int pieces, sx, sw;
     int64_t tx, tw;    // tiles
@@ -751,7 +754,6 @@ struct XentPlan {
         // and few rounded values of G weigh in a result (with one row a
         // single one), whose rounding does not average out: keep G in two parts.
         parts = n <= 256 ? 2 : 1;
-        bn = d <= 128 ? 128 : 256;
         constexpr int64_t kMost = 512 << 20;
         pieces = (int)std::min<int64_t>((n * v * 2 * parts + kMost - 1) / kMost, (v + 255) / 256);
         pieces = std::max(pieces, 1);
@@ -759,10 +761,10 @@ struct XentPlan {
         pieces = (int)((v + pc - 1) / pc);
         ldg = round_up(pc, 64);
         ldacc = round_up(d, 64);
-        const int64_t dt = (d + bn - 1) / bn;
+        const int64_t dt = (d + 255) / 256;
         tx = (n + 255) / 256 * dt;
         tw = (pc + 255) / 256 * dt;
-        choose_splits(tx, (pc + 63) / 64 * parts, tw, (n + 63) / 64 * parts, bn / 256.0, sx, sw);
+        choose_splits(tx, (pc + 63) / 64 * parts, tw, (n + 63) / 64 * parts, stage_cost(d), sx, sw);
     }
     bool dx_acc() const { return pieces > 1 || sx > 1; }
     int64_t tickets() const { return 16 * (tx + tw * pieces); }
@@ -836,7 +838,7 @@ Err xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, bool bf
     const View a = readable(prep, {x, d, n, ldx}, q.x), b = readable(prep, {w, d, v, ldw}, q.w);
     Err e = run_prep(prep, st);
     if (e.bad()) return e;
-    const Dense g(n, v, d, 256);
+    const Dense g(n, v, d);
     XentStats op{g, xent_whole(n, d, v), target, q.part, q.ly, loss, lse};
     const View ab[2] = {a, b};
     e = launch(ab, op, bf16, op.whole ? g.mt : g.units(), st);
@@ -844,19 +846,19 @@ Err xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, bool bf
     return start(k_xent_join, (n + 7) / 8, 256, 0, st, q.part, n, (v + 255) / 256 * 2, v, target, q.ly, loss, lse);
 }
 
-template <class T, int BN>
+template <class T>
 Err xent_pair(const XentPlan &pl, const XentGrad &q, const View &xs, const View &wp, const float *scale, int64_t n, int64_t d, int64_t v, int64_t c, int64_t pc,
               const int64_t *target, T *dx, int64_t lddx, T *dw, int64_t lddw, cudaStream_t st) {
     const View gv{q.g, pc, n, pl.ldg, pl.parts};
     const View views[4] = {gv, wp, gv, xs};
-    XentPair<T, BN> op{};
+    XentPair<T> op{};
     if (dx) {
-        op.dense[0] = Dense(n, d, pc, BN, pl.sx, pl.parts);
+        op.dense[0] = Dense(n, d, pc, pl.sx, pl.parts);
         op.sink[0] = {target, v, scale, dx, lddx, tc::store_width(dx, lddx), pl.dx_acc() ? q.accx : nullptr, pl.ldacc, c > 0, c + pc == v, q.tickets};
     }
     if (dw) {
         T *o = dw + c * lddw;
-        op.dense[1] = Dense(pc, d, n, BN, pl.sw, pl.parts);
+        op.dense[1] = Dense(pc, d, n, pl.sw, pl.parts);
         op.sink[1] = {nullptr, 0, scale, o, lddw, tc::store_width(o, lddw), pl.sw > 1 ? q.accw : nullptr, pl.ldacc, false, true,
                       q.tickets + 16 * (pl.tx + pl.tw * (c / pl.pc))};
     }
@@ -903,13 +905,12 @@ Err xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_
         wp.p = (const char *)wv.p + c * wv.ld * 2;
         wp.rows = pc;
         const bool first = own && c == 0;
-        XentG<T> og{Dense(n, pc, d, 256), c, v, target, lse, grad_loss, first ? nullptr : scale, g, pl.ldg, pl.parts > 1 ? n * pl.ldg : 0,
+        XentG<T> og{Dense(n, pc, d), c, v, target, lse, grad_loss, first ? nullptr : scale, g, pl.ldg, pl.parts > 1 ? n * pl.ldg : 0,
                     first ? copy : PackJob{}, q.tickets, first && tickets ? (int)pl.tickets() : 0, first ? scale : nullptr};
         const View xw[2] = {xv, wp};
         e = launch(xw, og, bf16, og.dense.units(), st);
         if (e.bad()) break;
-        e = pl.bn == 128 ? xent_pair<T, 128>(pl, q, xs, wp, scale, n, d, v, c, pc, target, dx, lddx, dw, lddw, st)
-                         : xent_pair<T, 256>(pl, q, xs, wp, scale, n, d, v, c, pc, target, dx, lddx, dw, lddw, st);
+        e = xent_pair<T>(pl, q, xs, wp, scale, n, d, v, c, pc, target, dx, lddx, dw, lddw, st);
     }
     return e;
 }
@@ -976,7 +977,7 @@ struct LeafIter {
         // 8 row tiles beside one another, as in Dense
         const uint32_t block = op.leaves.band(i), rest = i - block * op.leaves.band.d, wide = min(8u, rt - block * 8);
         const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
-        t.m0 = t.am = a + (int)tm * 256;
+        t.m0 = a + (int)tm * 256;
         t.n0 = (int)(tn * 256);
         t.mend = min(b - t.m0, 256) + t.m0;
         t.nend = min(op.leaves.n - t.n0, 256) + t.n0;
@@ -1007,14 +1008,13 @@ template <class T> struct LeafOut {
     int64_t ld;
     int width, rest;
     template <class R> __device__ void store(const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) const {
-        const int row0 = t.m0 + p.row - p.lane, h0 = p.half * 128;
-        tc::store_tile<T, 128>(p, addr, out + (int64_t)row0 * ld + t.n0 + h0, ld, t.mend - row0, t.nend - t.n0 - h0, width, false, [](float (&)[32], int) {}, release);
+        const int row0 = t.m0 + p.row - p.lane, h0 = p.first();
+        tc::store_tile<T>(p, addr, out + (int64_t)row0 * ld + t.n0 + h0, ld, t.mend - row0, t.nend - t.n0 - h0, width, false, [](float (&)[32], int) {}, release);
     }
 };
 
 // y = x w^T, leaf by leaf.
 template <class T> struct LeafRows {
-    static constexpr int kBN = 256;
     static constexpr bool kAMN = false, kBMN = false, kTail = false, kDual = false;
     static constexpr int laps = 1;
     using Iter = LeafIter;
@@ -1054,7 +1054,6 @@ __global__ void __launch_bounds__(1024) k_leaf_order(const int32_t *__restrict__
 // tiles (of one leaf and one part of its rows, the k axis; longest leaf
 // first), then dx's, all of the same short k axis.
 template <class T> struct LeafPair {
-    static constexpr int kBN = 256;
     static constexpr bool kAMN = false, kBMN = true, kTail = true, kDual = true;
     static constexpr int laps = 1;
     struct Iter : tc::Snake {
@@ -1090,7 +1089,7 @@ template <class T> struct LeafPair {
             look(op);
             const int nkb = (hi - lo + 63) / 64, each = op.splits > 1 ? (nkb + op.splits - 1) / op.splits : nkb, k0 = min((int)part * each, nkb),
                       k1 = min(k0 + each, nkb);
-            t.m0 = t.am = (int)tm * 256;
+            t.m0 = (int)tm * 256;
             t.n0 = (int)tn * 256;
             t.mend = min(op.dout - t.m0, 256) + t.m0;
             t.nend = min(op.leaves.n - t.n0, 256) + t.n0;
@@ -1127,14 +1126,14 @@ template <class T> struct LeafPair {
         all.m0 += base;
         all.mend += base;
         all.aux = t.aux / leaves.groups;
-        sink_tile<128>(sink, leaves.groups * dout, splits, all, p, addr, release, (g * mt + t.m0 / 256) * nt + t.n0 / 256);
+        sink_tile(sink, leaves.groups * dout, splits, all, p, addr, release, (g * mt + t.m0 / 256) * nt + t.n0 / 256);
     }
 };
 
 // Parts of dw's k axis, as if all leaves were alike.
 int leaf_splits(int64_t t, int32_t groups, int64_t din, int64_t dout) {
     int none = 1, s = 1;
-    choose_splits(0, 0, (int64_t)groups * ((din + 255) / 256) * ((dout + 255) / 256), (t / groups + 63) / 64, 1.0, none, s);
+    choose_splits(0, 0, (int64_t)groups * ((din + 255) / 256) * ((dout + 255) / 256), (t / groups + 63) / 64, stage_cost(din), none, s);
     return s;
 }
 

@@ -2,13 +2,16 @@
 // frame for the operators of linear.cu, which differ in how a tile is found
 // (Op::Iter) and in what happens to its sums (Op::epilogue).
 //
-// A cluster of two CTAs works on one 256 x BN tile.  Each CTA keeps 128 rows
-// of A and BN/2 rows of B in shared memory, 64 values of k a stage, fetched
+// A cluster of two CTAs works on one 256 x 256 tile.  Each CTA keeps 128 rows
+// of A and 128 rows of B in shared memory, 64 values of k a stage, fetched
 // by TMA with the 128-byte swizzle; one tcgen05.mma of the pair reads both
-// halves, so each SM fetches half of B: 32 KB a stage at BN = 256, 64 bytes a
+// halves, so each SM fetches half of B: 32 KB a stage, 64 bytes a
 // clock and SM against the 512 clocks of the stage's products.  The sums lie
-// in tensor memory (128 lanes x BN columns in each CTA), twice, so that one
-// tile's epilogue runs under the next one's products.
+// in tensor memory (128 lanes x 256 columns in each CTA), twice, so that one
+// tile's epilogue runs under the next one's products.  A tile whose result
+// has at most 128 or 64 columns multiplies that many, and boxes of which
+// no row or column is wanted are not fetched: what lies in their place ends in
+// sums that nobody stores.
 //
 // Warp 0 fetches, warp 1 of the leading CTA issues the products, warps 2..9
 // run the epilogue (warp w reads the tensor memory lanes 32 (w % 4) .. +31,
@@ -40,12 +43,11 @@ constexpr long long kWaitClocks = 4000000000ll;   // about 2 s
 
 static __device__ int g_ops_timeout;
 
-template <int BN> struct Shape {
-    static constexpr int kBBytes = BN / 2 * kBK * 2;
-    static constexpr int kStage = kABytes + kBBytes;
-    static constexpr int kStages = (227 * 1024 - kStaging - 2048) / kStage > 8 ? 8 : (227 * 1024 - kStaging - 2048) / kStage;
-    static constexpr int kSmem = kStages * kStage + kStaging + 2048;   // 1024 of alignment, 1024 of barriers and exchange
-};
+constexpr int kBN = 256;
+constexpr int kStageBytes = kABytes + kBN / 2 * kBK * 2;
+constexpr int kStages = (227 * 1024 - kStaging - 2048) / kStageBytes;
+constexpr int kSmem = kStages * kStageBytes + kStaging + 2048;   // 1024 of alignment, 1024 of barriers
+static_assert(kStages == 6, "");
 
 // ---- shared memory, barriers ------------------------------------------------
 
@@ -224,11 +226,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// kind::f16: sums in f32; A and B bf16 (1) or f16 (0); M = 256, N = BN;
-// bit 15 (A's m axis contiguous) is set tile by tile
-inline uint32_t make_idesc(bool bf16, bool b_mn, int bn) {
+// kind::f16: sums in f32; A and B bf16 (1) or f16 (0); M = 256;
+// bit 15 (A's m axis contiguous) and N (from bit 17) are set tile by tile
+inline uint32_t make_idesc(bool bf16, bool b_mn) {
     return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10  | (b_mn ? 1u : 0u) << 16 |
-           (uint32_t)(bn >> 3) << 17 | (uint32_t)(256 >> 4) << 24;
+           (uint32_t)(256 >> 4) << 24;
 }
 
 // A launch may start before the one in front of it has ended (its set-up
@@ -240,7 +242,7 @@ __device__ __forceinline__ void depend() {
 
 // ---- the frame --------------------------------------------------------------
 
-// One unit of work: C[m0 .. mend) x [n0 .. nend) (256 x BN at most), the
+// One unit of work: C[m0 .. mend) x [n0 .. nend) (256 x 256 at most), the
 // stages q0 .. q0 + nkb - 1 of its k axis, which starts at k0 in the maps.
 // With two parts of A (batches 0 and 1 of its map: a value's leading and
 // trailing bits), the stages take both parts of one block of k in turn.
@@ -248,7 +250,8 @@ __device__ __forceinline__ void depend() {
 // behind the k axis' end (0: the maps end there, TMA fills zeros).
 struct Tile {
     int m0, n0, mend, nend;
-    int am;           // A's first row in its map (m0 but for a piece of a longer axis)
+    // columns multiplied: each CTA brings half of them
+    __device__ int cols() const { return nend - n0 > 128 ? 256 : nend - n0 > 64 ? 128 : 64; }
     int k0, q0, nkb;
     int bz;           // B's batch
     int tail;
@@ -292,13 +295,16 @@ struct None {};
 struct Place {
     int sub, half, lane, rank;
     int row;             // row of the tile (0..255) of this lane
+    int wide;            // columns of one half
+    __device__ int first() const { return half * wide; }
     uint8_t *staging;    // 4096 bytes of this warp's own
     uint32_t swap;       // 4 barriers of the two warps of these rows (left and right columns)
     volatile int *dead;
 };
 
 // A place among the stages, and its barriers' parity.
-template <int N> struct Ring {
+struct Ring {
+    static constexpr int N = kStages;
     int s = 0;
     uint32_t ph = 0;
     __device__ void step() {
@@ -311,43 +317,57 @@ template <int N> struct Ring {
     }
 };
 
-// One stage of both operands into shared memory at `a`: boxes of 64 values of
-// k x 128 (BN/2) rows, or where the m (n) axis is contiguous 64 of its values x 64 of k.
+// What one CTA of the pair fetches of a tile: boxes of 64 values of k x 128
+// rows, or where the m (n) axis is contiguous 64 of its values x 64 of k.
+struct Boxes {
+    int am, bn, a, b;      // first row of A and B, boxes of each
+    __device__ static int count(bool mn, int from, int end) { return end <= from ? 0 : mn && end - from > 64 ? 2 : 1; }
+    __device__ Boxes(const Tile &t, bool amn, bool bmn, int rank) {
+        const int half = t.cols() / 2;
+        am = t.m0 + rank * 128;
+        bn = t.n0 + rank * half;
+        a = count(amn, am, min(t.mend, am + 128));
+        b = count(bmn, bn, min(t.nend, bn + half));
+    }
+    __device__ uint32_t bytes(bool amn, bool bmn) const { return a * (amn ? 8192 : kABytes) + b * (bmn ? 8192 : kABytes); }
+};
+
+// One stage of both operands into shared memory at `a`, counted on the
+// leading CTA's barrier (PAIR) or this one's.
 template <class Op, bool AMN, bool PAIR>
-__device__ __forceinline__ void load_stage(const CUtensorMap *maps, uint32_t a, uint32_t bar, int am, int bn, int at, int az, int bz) {
-    constexpr int BN = Op::kBN;
+__device__ __forceinline__ void load_stage(const CUtensorMap *maps, uint32_t a, uint32_t bar, const Boxes &x, int at, int az, int bz) {
     auto load = [&](uint32_t dst, const CUtensorMap *m, int x, int y, int z) {
         if (PAIR)
             tma_pair(dst, m, bar, x, y, z);
         else
             tma_own(dst, m, bar, x, y, z);
     };
-    if (AMN) {
-        load(a, maps, am, at, az);
-        load(a + 8192, maps, am + 64, at, az);
-    } else {
-        load(a, maps, at, am, az);
-    }
     const uint32_t b = a + kABytes;
+    if (AMN) {
+        if (x.a > 0) load(a, maps, x.am, at, az);
+        if (x.a > 1) load(a + 8192, maps, x.am + 64, at, az);
+    } else if (x.a) {
+        load(a, maps, at, x.am, az);
+    }
     if (Op::kBMN) {
-#pragma unroll
-        for (int j = 0; j < BN / 2; j += 64) load(b + j * 128, maps + 1, bn + j, at, bz);
-    } else {
-        load(b, maps + 1, at, bn, bz);
+        if (x.b > 0) load(b, maps + 1, x.bn, at, bz);
+        if (x.b > 1) load(b + 8192, maps + 1, x.bn + 64, at, bz);
+    } else if (x.b) {
+        load(b, maps + 1, at, x.bn, bz);
     }
 }
 
 template <class Op, bool AMN>
-__device__ __forceinline__ bool fetch(const Op &op, const CUtensorMap *maps, const Tile &t, int n, Ring<Shape<Op::kBN>::kStages> r, uint32_t stages, uint32_t full,
-                                      uint32_t empty, uint32_t rank, volatile int *dead) {
-    using S = Shape<Op::kBN>;
-    const int am = t.am + (int)rank * 128, bn = t.n0 + (int)rank * (Op::kBN / 2);
+__device__ __forceinline__ bool fetch(const Op &op, const CUtensorMap *maps, const Tile &t, int n, Ring r, uint32_t stages, uint32_t full, uint32_t empty,
+                                      uint32_t rank, volatile int *dead) {
+    const Boxes mine(t, AMN, Op::kBMN, (int)rank), other(t, AMN, Op::kBMN, (int)rank ^ 1);
+    const uint32_t bytes = mine.bytes(AMN, Op::kBMN) + other.bytes(AMN, Op::kBMN);
     const bool two = op.laps == 2;
     for (int q = t.q0; q < t.q0 + n; q++) {
         if (!mbar_wait(empty + 8 * r.s, r.ph ^ 1, dead)) return false;
         const uint32_t bar = full + 8 * r.s;
-        if (rank == 0) mbar_expect(bar, 2 * S::kStage);
-        load_stage<Op, AMN, true>(maps, stages + r.s * S::kStage, bar, am, bn, t.k0 + (two ? q >> 1 : q) * kBK, two ? q & 1 : 0, t.bz);
+        if (rank == 0) mbar_expect(bar, bytes);
+        load_stage<Op, AMN, true>(maps, stages + r.s * kStageBytes, bar, mine, t.k0 + (two ? q >> 1 : q) * kBK, two ? q & 1 : 0, t.bz);
         r.step();
     }
     return true;
@@ -364,12 +384,11 @@ template <class Op, bool AMN> __device__ __forceinline__ void multiply_stage(uin
 }
 
 template <class Op, bool AMN>
-__device__ __forceinline__ bool multiply(uint32_t d, int n, Ring<Shape<Op::kBN>::kStages> &r, uint32_t stages, uint32_t full, uint32_t empty, uint32_t idesc,
-                                         volatile int *dead) {
+__device__ __forceinline__ bool multiply(uint32_t d, int n, Ring &r, uint32_t stages, uint32_t full, uint32_t empty, uint32_t idesc, volatile int *dead) {
     for (int k = 0; k < n; k++) {
         if (!mbar_wait(full + 8 * r.s, r.ph, dead)) return false;
         fence_after();
-        multiply_stage<Op, AMN>(d, stages + r.s * Shape<Op::kBN>::kStage, idesc, k > 0);
+        multiply_stage<Op, AMN>(d, stages + r.s * kStageBytes, idesc, k > 0);
         commit_pair(empty + 8 * r.s);
         r.step();
     }
@@ -379,18 +398,16 @@ __device__ __forceinline__ bool multiply(uint32_t d, int n, Ring<Shape<Op::kBN>:
 template <class Op>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uint32_t idesc) {
-    constexpr int BN = Op::kBN;
-    using S = Shape<BN>;
-    constexpr int kCols = 2 * BN < 32 ? 32 : 2 * BN;    // tensor memory columns: a power of two
+    constexpr int kCols = 2 * kBN;      // of tensor memory
     extern __shared__ uint8_t raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    uint8_t *staging = base + S::kStages * S::kStage;
+    uint8_t *staging = base + kStages * kStageBytes;
     uint64_t *bars = (uint64_t *)(staging + kStaging);
     const uint32_t stages = smem_u32(base);
-    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, tfull = empty + 8 * S::kStages, tempty = tfull + 16,
-                   fixed = tempty + 16, tailbar = fixed + 8 * S::kStages;
-    const uint32_t swap = tailbar + 8 * S::kStages;
-    uint32_t *tmem_slot = (uint32_t *)(bars + 4 * S::kStages + 20);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16,
+                   fixed = tempty + 16, tailbar = fixed + 8 * kStages;
+    const uint32_t swap = tailbar + 8 * kStages;
+    uint32_t *tmem_slot = (uint32_t *)(bars + 4 * kStages + 20);
     volatile int *dead = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cluster_rank();
@@ -398,7 +415,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
 
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < (Op::kDual ? 4 : 2); i++) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.m[i]) : "memory");
-        for (int s = 0; s < S::kStages; s++) {
+        for (int s = 0; s < kStages; s++) {
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
             // one a stage: a CTA ahead of the other by a whole short tile must not count for both
@@ -426,7 +443,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
 
     if (warp == 0) {
         // ---- fetch: one thread runs a tile's stages (a stage has 512 clocks)
-        Ring<S::kStages> r;
+        Ring r;
         typename Op::Iter it(op, cid, ncl);
         Tile t;
         while (it.next(op, t)) {
@@ -438,14 +455,15 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                                                    : fetch<Op, Op::kAMN>(op, maps.m, t, n, r, stages, full, empty, rank, dead);
                 if (ok && tail) {
                     // the last stage's bytes count for warp 10, not for the products
-                    Ring<S::kStages> q = r;
+                    Ring q = r;
                     q.skip(n);
                     ok = mbar_wait(empty + 8 * q.s, q.ph ^ 1, dead);
                     if (ok) {
-                        mbar_expect(tailbar + 8 * q.s, S::kStage);
+                        const Boxes mine(t, true, Op::kBMN, (int)rank);
+                        mbar_expect(tailbar + 8 * q.s, mine.bytes(true, Op::kBMN));
                         if (rank == 0) mbar_arrive(full + 8 * q.s);
-                        load_stage<Op, true, false>(Op::kDual ? maps.m + 2 : maps.m, stages + q.s * S::kStage, tailbar + 8 * q.s, t.am + (int)rank * 128,
-                                                    t.n0 + (int)rank * (BN / 2), t.k0 + (t.q0 + n) * kBK, 0, t.bz);
+                        load_stage<Op, true, false>(Op::kDual ? maps.m + 2 : maps.m, stages + q.s * kStageBytes, tailbar + 8 * q.s, mine,
+                                                    t.k0 + (t.q0 + n) * kBK, 0, t.bz);
                     }
                 }
             }
@@ -456,7 +474,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     } else if (warp == 1) {
         // ---- products, issued by one thread too
         if (rank == 0) {
-            Ring<S::kStages> r;
+            Ring r;
             int n = 0;
             uint32_t fixed_ph = 0;
             typename Op::Iter it(op, cid, ncl);
@@ -464,21 +482,21 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
             while (it.next(op, t)) {
                 const int buf = n & 1;
                 const bool tail = Op::kTail && t.tail && t.nkb, second = Op::kDual && t.kind == 1;
-                const int last = (r.s + t.nkb - 1) % S::kStages;     // the tail's stage
+                const int last = (r.s + t.nkb - 1) % kStages;     // the tail's stage
                 __syncwarp();
                 if (elect_one()) {
                     bool ok = mbar_wait(tempty + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
                     fence_after();
-                    const uint32_t d = tmem + buf * BN;
-                    Ring<S::kStages> q = r;
+                    const uint32_t d = tmem + buf * kBN, id = idesc | (uint32_t)(t.cols() >> 3) << 17;
+                    Ring q = r;
                     if (ok)
-                        ok = second ? multiply<Op, true>(d, t.nkb - tail, q, stages, full, empty, idesc, dead)
-                                    : multiply<Op, Op::kAMN>(d, t.nkb - tail, q, stages, full, empty, idesc, dead);
+                        ok = second ? multiply<Op, true>(d, t.nkb - tail, q, stages, full, empty, id, dead)
+                                    : multiply<Op, Op::kAMN>(d, t.nkb - tail, q, stages, full, empty, id, dead);
                     if (ok && tail) {
                         ok = mbar_wait(full + 8 * q.s, q.ph, dead) && mbar_wait<true>(fixed + 8 * q.s, fixed_ph >> q.s & 1, dead);
                         fence_after();
                         if (ok) {
-                            multiply_stage<Op, true>(d, stages + q.s * S::kStage, idesc, t.nkb > 1);
+                            multiply_stage<Op, true>(d, stages + q.s * kStageBytes, id, t.nkb > 1);
                             commit_pair(empty + 8 * q.s);
                         }
                     }
@@ -496,18 +514,18 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         // end belong to the next leaf; zeros take their place before the
         // products see them
         if (Op::kTail) {
-            Ring<S::kStages> r;
+            Ring r;
             uint32_t ph = 0;
             typename Op::Iter it(op, cid, ncl);
             Tile t;
             while (it.next(op, t)) {
                 r.skip(t.nkb);
                 if (!t.tail || !t.nkb) continue;
-                const int s = r.s == 0 ? S::kStages - 1 : r.s - 1;
+                const int s = r.s == 0 ? kStages - 1 : r.s - 1;
                 if (!mbar_wait_warp(tailbar + 8 * s, ph >> s & 1, dead)) break;
                 ph ^= 1u << s;
-                uint8_t *st = base + s * S::kStage;
-                for (int box = 0; box < S::kStage / 8192; box++)
+                uint8_t *st = base + s * kStageBytes;
+                for (int box = 0; box < kStageBytes / 8192; box++)
                     for (int i = t.tail * 8 + lane; i < 64 * 8; i += 32) *(uint4 *)(st + box * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -537,7 +555,8 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
             if (!mbar_wait_warp(tfull + 8 * buf, (n >> 1) & 1, dead)) break;
             n++;
             fence_after();
-            op.epilogue(t, p, rows, state, tmem + buf * BN + ((uint32_t)(p.sub * 32) << 16) + p.half * (BN / 2), [&] {
+            p.wide = t.cols() / 2;
+            op.epilogue(t, p, rows, state, tmem + buf * kBN + ((uint32_t)(p.sub * 32) << 16) + p.half * p.wide, [&] {
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_at<false>(tempty + 8 * buf, 0);
@@ -590,20 +609,24 @@ template <class T> __device__ __forceinline__ void store8(T *dst, uint4 q, int n
     }
 }
 
-// The sums of this warp's 32 rows, COLS columns from `addr` on, through f(v,
-// col) (32 columns at a time, col from the tile's first), rounded to T and
+// The sums of this warp's 32 rows, p.wide columns from `addr` on, through f(v,
+// col) (32 columns at a time, col from the half's first), rounded to T and
 // stored at out[r * ld + c] for r < rows, c < cols: 64 columns at a time pass
 // through the warp's staging memory, so that eight lanes store one row's 128
 // bytes.  width: store_width of the rows.  empty: no products, the sums are
 // 0.  release() hands the tensor memory back once it is read.
-template <class T, int COLS, class F, class R>
+template <class T, class F, class R>
 __device__ __forceinline__ void store_tile(const Place &p, uint32_t addr, T *out, int64_t ld, int rows, int cols, int width, bool empty, F f, R release) {
-    static_assert(COLS % 64 == 0, "");
+    if (rows <= 0) {
+        release();
+        return;
+    }
 #pragma unroll 1
-    for (int c = 0; c < COLS; c += 64) {
+    for (int c = 0; c < p.wide; c += 64) {
         __syncwarp();
 #pragma unroll
         for (int h = 0; h < 64; h += 32) {
+            if (c + h >= p.wide) break;
             float v[32];
             if (empty) {
 #pragma unroll
@@ -623,13 +646,13 @@ __device__ __forceinline__ void store_tile(const Place &p, uint32_t addr, T *out
                 *(uint4 *)(p.staging + p.lane * 128 + (((h / 8 + i) ^ (p.lane & 7)) * 16)) = q;
             }
         }
-        if (c + 64 >= COLS) release();
+        if (c + 64 >= p.wide) release();
         __syncwarp();
         if (c >= cols) continue;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int r = i * 4 + p.lane / 8, ch = p.lane % 8, col = c + ch * 8;
-            if (r < rows && col < cols)
+            if (r < rows && col < min(cols, p.wide))
                 store8(out + (int64_t)r * ld + col, *(const uint4 *)(p.staging + r * 128 + ((ch ^ (r & 7)) * 16)), min(cols - col, 8), width);
         }
     }
