@@ -188,15 +188,12 @@ __device__ __forceinline__ void pack_chunk(const PackJob &j, int64_t r, int64_t 
 // The power of two that takes m to at most 2^14.
 __device__ __forceinline__ int scale_exponent(float m) { return m > 0.f && m < INFINITY ? min(max(14 - (ilogbf(m) + 1), -100), 100) : 0; }
 
-// What a call's other launches need first: copies of operands, tickets set to
-// 0, and the power of two that takes the largest |grad_loss| of the rows that
+// What a call's other launches need first: copies of operands, and the power of two that takes the largest |grad_loss| of the rows that
 // count to at most 2^14, half precision's range (scale[0], its inverse in
 // scale[1]; by the last block).
 struct Prep {
     PackJob job[3];
     int jobs = 0;
-    uint32_t *tickets = nullptr;
-    int n_tickets = 0;
     const float *grad_loss = nullptr;
     const int64_t *target = nullptr;
     int64_t n = 0, v = 0;
@@ -225,7 +222,6 @@ __global__ void __launch_bounds__(256) k_prep(const __grid_constant__ Prep p) {
         return;
     }
     const int64_t first = blockIdx.x * 256LL + threadIdx.x, step = work * 256LL;
-    for (int64_t i = first; i < p.n_tickets; i += step) p.tickets[i] = 0;
     for (int k = 0; k < p.jobs; k++) {
         const PackJob &j = p.job[k];
         const int64_t per = j.ldp / 8, total = j.rows * per;
@@ -238,9 +234,9 @@ __global__ void __launch_bounds__(256) k_prep(const __grid_constant__ Prep p) {
 }
 
 Err run_prep(const Prep &p, cudaStream_t st) {
-    int64_t most = p.n_tickets / 4;
+    int64_t most = 0;
     for (int k = 0; k < p.jobs; k++) most = std::max(most, p.job[k].chunks());
-    if (!p.jobs && !p.n_tickets && !p.scale) return {};
+    if (!p.jobs && !p.scale) return {};
     const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((most + 255) / 256, sm_count() * 8LL));
     return start(k_prep, blocks + (p.scale ? 1 : 0), 256, 0, st, p);
 }
@@ -480,11 +476,10 @@ template <class T> struct XentG {
     T *g;
     int64_t ldg, part;  // row stride; from the leading to the trailing part (0: one part)
     // where no launch went before that did them: the copy of x with the
-    // ignored rows as zeros (rows 0: done), the tickets, and half precision's
-    // scale (find_scale)
+    // ignored rows as zeros (rows 0: done) and half precision's scale
+    // (find_scale)
     PackJob copy;
-    uint32_t *tickets;
-    int n_tickets;
+    tc::Div per;        // 16-byte pieces of a row
     float *find_scale;
     struct State {
         float scale;
@@ -503,9 +498,12 @@ template <class T> struct XentG {
             st.scale = ldexpf(1.f, e);
             if (warp == 0 && lane == 0) find_scale[0] = st.scale, find_scale[1] = ldexpf(1.f, -e);
         }
-        for (int i = warp * 32 + lane; i < n_tickets; i += warps * 32) tickets[i] = 0;
-        for (int64_t r = warp; r < copy.rows; r += warps)
-            for (int64_t c = lane * 8; c < copy.ldp; c += 256) pack_chunk(copy, r, c);
+        const uint32_t all = (uint32_t)copy.rows * per.d;
+#pragma unroll 4
+        for (uint32_t i = warp * 32 + lane; i < all; i += warps * 32) {
+            const uint32_t r = per(i);
+            pack_chunk(copy, r, (i - r * per.d) * 8);
+        }
     }
     struct Rows {
         int64_t y;
@@ -562,11 +560,12 @@ template <class T> struct XentG {
     }
 };
 
-// Where a product's sums go.  One unit makes all of a tile where acc is null
-// or (with add) `last` says so; else the units leave f32 sums in acc
-// [split][m][ldacc], on top of an earlier piece's (add), and the last unit of
-// a tile to arrive (by a ticket a warp) adds the splits up, always in the
-// same order, so that the result does not depend on who came last.
+// Where a product's sums go: rounded to out where one launch's one unit has
+// all of them (one split, and the last piece), else as f32 sums to acc
+// [split][m][ldacc], on top of an earlier piece's (add); a launch of
+// k_sum adds the splits up, always in the same order.  (The last of a tile's
+// units to arrive, told by a ticket, adding them up instead took 84 us for
+// 2 tiles of 32 splits: one warp's serial reads.)
 template <class T> struct Sink {
     const int64_t *target;     // rows whose target is ignored are 0 (null: none)
     int64_t v;
@@ -577,12 +576,11 @@ template <class T> struct Sink {
     float *acc;
     int64_t ldacc;
     bool add, last;
-    uint32_t *tickets;         // [tile][16 warps of the pair]
 };
 
 // f32 sums of a warp's 32 x COLS block: its place in acc.
 template <class T, class R>
-__device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, const tc::Tile &t, const tc::Place &p, uint32_t addr, R release, int tile) {
+__device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, const tc::Tile &t, const tc::Place &p, uint32_t addr, R release) {
     const int row = t.m0 + p.row, row0 = row - p.lane, h0 = p.first(), cols = t.nend - t.n0 - h0;
     const float scale = k.scale ? k.scale[1] : 1.f;
     bool has = row < t.mend;
@@ -640,32 +638,60 @@ __device__ __forceinline__ void sink_tile(const Sink<T> &k, int m, int splits, c
             }
         }
     }
-    if (!k.last || one) return;
-    const int warp = p.rank * 8 + p.half * 4 + p.sub;
-    uint32_t n = 0;
-    __threadfence();
-    __syncwarp();
-    if (p.lane == 0) n = atomicAdd(k.tickets + (int64_t)tile * 16 + warp, 1u);
-    n = __shfl_sync(~0u, n, 0);
-    if (n != (uint32_t)splits - 1) return;
-    __threadfence();
-    const float *first = k.acc + (int64_t)row * k.ldacc + t.n0 + h0;
-    const int64_t step = (int64_t)m * k.ldacc;
-    tc::store_tile<T>(
-        p, addr, out, k.ld, t.mend - row0, cols, k.width, true,
-        [&](float (&x)[32], int c) {
-            if (!mine(c)) return;
-            for (int s = 0; s < splits; s++) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float4 o = __ldcg((const float4 *)(first + s * step + c) + i);
-                    x[4 * i] += o.x, x[4 * i + 1] += o.y, x[4 * i + 2] += o.z, x[4 * i + 3] += o.w;
-                }
+}
+
+// out = the splits' sums, scaled back and rounded; ignored rows 0.
+struct SumJob {
+    const float *acc;
+    int64_t ldacc, m, n;
+    int splits;
+    const float *scale;
+    const int64_t *target;
+    int64_t v;
+    void *out;
+    int64_t ld;
+    tc::Div per;       // groups of 4 columns of a row
+};
+
+template <class T> __global__ void __launch_bounds__(256) k_sum(const __grid_constant__ SumJob a, const __grid_constant__ SumJob b) {
+    tc::depend();
+    for (int k = 0; k < 2; k++) {
+        const SumJob &j = k ? b : a;
+        const uint32_t total = (uint32_t)j.m * j.per.d;
+        const float c = j.scale ? j.scale[1] : 1.f;
+        for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
+            const uint32_t r = j.per(i), col = (i - r * j.per.d) * 4;
+            const float *p = j.acc + r * j.ldacc + col;
+            float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+            for (int q = 0; q < j.splits; q++) {
+                const float4 o = *(const float4 *)(p + q * j.m * j.ldacc);
+                s.x += o.x, s.y += o.y, s.z += o.z, s.w += o.w;
             }
+            bool has = true;
+            if (j.target) {
+                const int64_t y = j.target[r];
+                has = y >= 0 && y < j.v;
+            }
+            const float x[4] = {s.x, s.y, s.z, s.w};
+            T *out = (T *)j.out + r * j.ld + col;
 #pragma unroll
-            for (int i = 0; i < 32; i++) x[i] = has ? x[i] * scale : 0.f;
-        },
-        [] {});
+            for (int e = 0; e < 4; e++)
+                if (col + e < j.n) out[e] = from_f<T>(has ? x[e] * c : 0.f);
+        }
+    }
+}
+
+// The sums of up to two products of which parts lie in acc.
+template <class T> Err run_sum(SumJob a, SumJob b, cudaStream_t st) {
+    for (SumJob *j : {&a, &b}) {
+        if (!j->m) continue;
+        const int64_t per = (j->n + 3) / 4;
+        if (j->m * per > INT_MAX - (1 << 20)) return {GBM_ERR_ARG, "split sums of more than 2^31 pieces"};
+        j->per = tc::Div((uint32_t)per);
+    }
+    const int64_t most = std::max(a.m * (int64_t)a.per.d, b.m * (int64_t)b.per.d);
+    return start(k_sum<T>, std::min<int64_t>((most + 255) / 256, sm_count() * 8LL), 256, 0, st, a, b);
 }
 
 // dx = G w (A K-major) and dw = G^T x (A's m axis contiguous), B's n axis
@@ -694,8 +720,7 @@ template <class T> struct XentPair {
     using State = tc::None;
     __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, tc::None &, uint32_t addr, R release) const {
-        const Dense &g = dense[t.kind];
-        sink_tile(sink[t.kind], g.m, g.splits, t, p, addr, release, (t.m0 / 256) * g.nt + t.n0 / 256);
+        sink_tile(sink[t.kind], dense[t.kind].m, dense[t.kind].splits, t, p, addr, release);
     }
 };
 
@@ -716,9 +741,9 @@ double chain(int64_t u0, int64_t l0, int64_t u1, int64_t l1) {
 double stage_cost(int64_t d) { return d > 128 ? 1.0 : d > 64 ? 0.5 : 0.3; }
 
 // Parts of both products' k axes (tx tiles of kx stages, tw of kw): those that
-// end first.  Split sums cost some 5 us of fences, tickets and reading back,
-// and the time the f32 sums take to be written and read again (512 KB a tile,
-// 0.08 us at the memory's rate: 0.3 of a stage).  cost: a stage's time against
+// end first.  Split sums cost a launch, some 5 us, and the time the f32 sums
+// take to be written and read again (512 KB a tile, 0.08 us at the memory's
+// rate: 0.3 of a stage).  cost: a stage's time against
 // that of a 256 x 256 tile.
 void choose_splits(int64_t tx, int64_t kx, int64_t tw, int64_t kw, double cost, int &sx, int &sw) {
     static constexpr int kTry[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
@@ -767,7 +792,6 @@ struct XentPlan {
         choose_splits(tx, (pc + 63) / 64 * parts, tw, (n + 63) / 64 * parts, stage_cost(d), sx, sw);
     }
     bool dx_acc() const { return pieces > 1 || sx > 1; }
-    int64_t tickets() const { return 16 * (tx + tw * pieces); }
 };
 
 struct Room {
@@ -809,13 +833,11 @@ struct XentLoss {
 struct XentGrad {
     uint16_t *x, *w, *g;
     float *accx, *accw, *scale;
-    uint32_t *tickets;
     int64_t bytes;
     XentGrad(void *ws, int64_t n, int64_t d, int64_t v, bool in_place) {
         Room r(ws);
         const XentPlan pl(n, d, v);
         scale = r.take<float>(2);
-        tickets = r.take<uint32_t>(pl.tickets());
         x = r.take<uint16_t>(n * pl.dp);
         w = r.take<uint16_t>(in_place ? 0 : v * pl.dp);
         g = r.take<uint16_t>(n * pl.ldg * pl.parts);
@@ -854,17 +876,20 @@ Err xent_pair(const XentPlan &pl, const XentGrad &q, const View &xs, const View 
     XentPair<T> op{};
     if (dx) {
         op.dense[0] = Dense(n, d, pc, pl.sx, pl.parts);
-        op.sink[0] = {target, v, scale, dx, lddx, tc::store_width(dx, lddx), pl.dx_acc() ? q.accx : nullptr, pl.ldacc, c > 0, c + pc == v, q.tickets};
+        op.sink[0] = {target, v, scale, dx, lddx, tc::store_width(dx, lddx), pl.dx_acc() ? q.accx : nullptr, pl.ldacc, c > 0, c + pc == v};
     }
     if (dw) {
         T *o = dw + c * lddw;
         op.dense[1] = Dense(pc, d, n, pl.sw, pl.parts);
-        op.sink[1] = {nullptr, 0, scale, o, lddw, tc::store_width(o, lddw), pl.sw > 1 ? q.accw : nullptr, pl.ldacc, false, true,
-                      q.tickets + 16 * (pl.tx + pl.tw * (c / pl.pc))};
+        op.sink[1] = {nullptr, 0, scale, o, lddw, tc::store_width(o, lddw), pl.sw > 1 ? q.accw : nullptr, pl.ldacc, false, true};
     }
     op.first = op.dense[1].per > op.dense[0].per;
     op.laps = pl.parts;
-    return launch(views, op, std::is_same<T, __nv_bfloat16>::value, op.dense[0].units() + op.dense[1].units(), st);
+    Err e = launch(views, op, std::is_same<T, __nv_bfloat16>::value, op.dense[0].units() + op.dense[1].units(), st);
+    SumJob a{}, b{};
+    if (dx && pl.sx > 1 && c + pc == v) a = {q.accx, pl.ldacc, n, d, pl.sx, scale, target, v, dx, lddx, {}};
+    if (dw && pl.sw > 1) b = {q.accw, pl.ldacc, pc, d, pl.sw, scale, nullptr, 0, dw + c * lddw, lddw, {}};
+    return e.bad() || !(a.m || b.m) ? e : run_sum<T>(a, b, st);
 }
 
 template <class T>
@@ -875,14 +900,16 @@ Err xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_
     const XentGrad q(ws, n, d, v, tma_rows(x, ldx) && tma_rows(w, ldw));
     // rows that count, zeros in the others': an ignored row's features must not reach dw
     const View xs{q.x, d, n, pl.dp}, given{x, d, n, ldx};
-    const bool tickets = pl.sx > 1 || pl.sw > 1;
     float *scale = bf16 ? nullptr : q.scale;
     View xv = given, wv{w, d, v, ldw};
     PackJob copy{};
     Err e;
-    // G's own launch makes the copy under its first products, and finds
-    // half precision's scale where one warp reads all rows in about a microsecond
-    const bool own = tma_rows(x, ldx) && tma_rows(w, ldw) && (bf16 || n <= 1024);
+    // G's own launch makes the copy under its first products where that is a few
+    // 16-byte pieces a thread of its epilogue (9472 x 1024, some 32 of them:
+    // G 170 -> 194K clocks, against 7 us for a launch), and finds half
+    // precision's scale where a warp reads all rows in about a microsecond
+    const int64_t threads = std::min<int64_t>(74, (n + 255) / 256 * ((pl.pc + 255) / 256)) * 2 * tc::kEpiWarps * 32;
+    const bool own = tma_rows(x, ldx) && tma_rows(w, ldw) && (bf16 || n <= 1024) && (!dw || n * (pl.dp / 8) <= 4 * threads);
     if (own) {
         if (dw) {
             Prep one;
@@ -894,7 +921,6 @@ Err xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_
         add_pack(prep, given, q.x, pl.dp, target, v);
         xv = xs;
         wv = readable(prep, wv, q.w);
-        if (tickets) prep.tickets = q.tickets, prep.n_tickets = (int)pl.tickets();
         if (!bf16) prep.grad_loss = grad_loss, prep.target = target, prep.n = n, prep.v = v, prep.scale = q.scale;
         e = run_prep(prep, st);
     }
@@ -906,7 +932,7 @@ Err xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_
         wp.rows = pc;
         const bool first = own && c == 0;
         XentG<T> og{Dense(n, pc, d), c, v, target, lse, grad_loss, first ? nullptr : scale, g, pl.ldg, pl.parts > 1 ? n * pl.ldg : 0,
-                    first ? copy : PackJob{}, q.tickets, first && tickets ? (int)pl.tickets() : 0, first ? scale : nullptr};
+                    first ? copy : PackJob{}, tc::Div((uint32_t)(pl.dp / 8)), first ? scale : nullptr};
         const View xw[2] = {xv, wp};
         e = launch(xw, og, bf16, og.dense.units(), st);
         if (e.bad()) break;
@@ -1126,7 +1152,7 @@ template <class T> struct LeafPair {
         all.m0 += base;
         all.mend += base;
         all.aux = t.aux / leaves.groups;
-        sink_tile(sink, leaves.groups * dout, splits, all, p, addr, release, (g * mt + t.m0 / 256) * nt + t.n0 / 256);
+        sink_tile(sink, leaves.groups * dout, splits, all, p, addr, release);
     }
 };
 
@@ -1140,9 +1166,8 @@ int leaf_splits(int64_t t, int32_t groups, int64_t din, int64_t dout) {
 struct LeafWs {
     uint16_t *x, *w, *dy;
     float *acc;
-    uint32_t *tickets;
     int4 *order;
-    int64_t ldacc, n_tickets, bytes;
+    int64_t ldacc, bytes;
     LeafWs(void *ws, int64_t t, int32_t groups, int64_t din, int64_t dout, bool grad, bool in_place) {
         Room r(ws);
         const int64_t ip = round_up(din, 8), op = round_up(dout, 8);
@@ -1152,8 +1177,6 @@ struct LeafWs {
         ldacc = round_up(din, 64);
         const int s = grad ? leaf_splits(t, groups, din, dout) : 1;
         acc = r.take<float>(s > 1 ? s * groups * dout * ldacc : 0);
-        n_tickets = s > 1 ? 16 * groups * ((din + 255) / 256) * ((dout + 255) / 256) : 0;
-        tickets = r.take<uint32_t>(n_tickets);
         order = r.take<int4>(grad ? groups : 0);
         bytes = r.bytes();
     }
@@ -1187,11 +1210,7 @@ Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off,
     const View g = readable(prep, {dy, dout, t, lddy}, q.dy);
     View a{}, b{};
     if (dx) b = readable(prep, {w, din, dout, din, groups}, q.w);
-    if (dw) {
-        a = readable(prep, {x, din, t, ldx}, q.x);
-        prep.tickets = q.tickets;
-        prep.n_tickets = (int)q.n_tickets;
-    }
+    if (dw) a = readable(prep, {x, din, t, ldx}, q.x);
     Err e = run_prep(prep, st);
     const int s = leaf_splits(t, groups, din, dout), mt = (int)((dout + 255) / 256), nt = (int)((din + 255) / 256);
     LeafPair<T> op{Leaves(off, t, groups, dout, din), {}, nullptr, (int)dout, s, mt, nt, {}, {}, {}, {}};
@@ -1211,12 +1230,14 @@ Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off,
             e = start(k_leaf_order, 1, 1024, 0, st, off, groups, t, q.order);
             op.order = q.order;
         }
-        op.sink = {nullptr, 0, nullptr, dw, din, tc::store_width(dw, din), s > 1 ? q.acc : nullptr, q.ldacc, false, true, q.tickets};
+        op.sink = {nullptr, 0, nullptr, dw, din, tc::store_width(dw, din), s > 1 ? q.acc : nullptr, q.ldacc, false, true};
         units += own;
     }
     if (e.bad()) return e;
     const View views[4] = {g, dx ? b : a, g, dw ? a : b};
-    return launch(views, op, bf16, units, st);
+    e = launch(views, op, bf16, units, st);
+    if (e.bad() || !dw || s == 1) return e;
+    return run_sum<T>({q.acc, q.ldacc, groups * dout, din, s, nullptr, nullptr, 0, dw, din, {}}, {}, st);
 }
 
 // ---------------------------------------------------------------------------
