@@ -589,23 +589,27 @@ __host__ __device__ inline int store_width(const void *p, int64_t ld) {
     return a & 15 ? a & 7 ? a & 3 ? 1 : 2 : 4 : 8;
 }
 
-// Stores elements [0, n) (n <= 8) of the 16 bytes q.
-template <class T> __device__ __forceinline__ void store8(T *dst, uint4 q, int n, int width) {
-    if (width == 8 && n >= 8) {
-        *(uint4 *)dst = q;
-    } else if (width >= 4 && (n & 3) == 0) {
-        *(uint2 *)dst = make_uint2(q.x, q.y);
-        if (n == 8) *(uint2 *)(dst + 4) = make_uint2(q.z, q.w);
-    } else if (width >= 2 && (n & 1) == 0) {
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// Rows of 64 columns in a warp's staging memory (16-byte piece i of row r at
+// piece i ^ (r % 8)) to out[r * ld + c] for r < rows, c < cols, W elements a
+// lane: 64 / W lanes have one row, so that a store of the warp covers runs of
+// a row whatever W is (with 8 elements a lane stored one by one, rows of odd
+// length took 32 places a store).
+template <int W, class V, class T>
+__device__ __forceinline__ void store_rows(const uint8_t *staging, int lane, T *out, int64_t ld, int rows, int cols) {
+    constexpr int kLanes = 64 / W;      // of a row
+#pragma unroll(W == 8 ? 4 : 2)
+    for (int i = lane; i < 32 * kLanes; i += 32) {
+        const int r = i / kLanes, c = i % kLanes * W;
+        if (r >= rows || c >= cols) continue;
+        const uint8_t *from = staging + r * 128 + ((c / 8 ^ (r & 7)) * 16) + c % 8 * 2;
+        T *to = out + (int64_t)r * ld + c;
+        if (c + W <= cols) {
+            *(V *)to = *(const V *)from;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (2 * j < n) *(uint32_t *)(dst + 2 * j) = w[j];
-    } else {
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < n) *(uint16_t *)(dst + j) = (uint16_t)(w[j / 2] >> (j & 1) * 16);
+            for (int k = 0; k < W - 1; k++)
+                if (c + k < cols) ((uint16_t *)to)[k] = ((const uint16_t *)from)[k];
+        }
     }
 }
 
@@ -648,13 +652,16 @@ __device__ __forceinline__ void store_tile(const Place &p, uint32_t addr, T *out
         }
         if (c + 64 >= p.wide) release();
         __syncwarp();
-        if (c >= cols) continue;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int r = i * 4 + p.lane / 8, ch = p.lane % 8, col = c + ch * 8;
-            if (r < rows && col < min(cols, p.wide))
-                store8(out + (int64_t)r * ld + col, *(const uint4 *)(p.staging + r * 128 + ((ch ^ (r & 7)) * 16)), min(cols - col, 8), width);
-        }
+        const int lim = min(cols, p.wide) - c;
+        if (lim <= 0) continue;
+        if (width == 8)
+            store_rows<8, uint4>(p.staging, p.lane, out + c, ld, rows, lim);
+        else if (width == 4)
+            store_rows<4, uint2>(p.staging, p.lane, out + c, ld, rows, lim);
+        else if (width == 2)
+            store_rows<2, uint32_t>(p.staging, p.lane, out + c, ld, rows, lim);
+        else
+            store_rows<1, uint16_t>(p.staging, p.lane, out + c, ld, rows, lim);
     }
 }
 
