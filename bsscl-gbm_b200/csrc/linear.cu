@@ -268,22 +268,23 @@ struct Dense {
     int splits;        // parts of the k axis
     int mt, nt;        // tiles
     int per;           // stages of a part
+    int wide;          // columns of a tile
     tc::Div all, band; // tiles in all, in 8 rows of tiles
-    Dense() : m(0), n(0), nkb(0), splits(1), mt(0), nt(0), per(0) {}
-    Dense(int64_t m_, int64_t n_, int64_t k, int splits_ = 1, int laps = 1)
-        : m((int)m_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK) * laps), splits(splits_), mt((int)((m_ + 255) / 256)), nt((int)((n_ + 255) / 256)),
-          per((nkb + splits_ - 1) / splits_), all((uint32_t)std::min<int64_t>(tiles(), INT_MAX)), band((uint32_t)std::min<int64_t>(8LL * nt, INT_MAX)) {}
+    Dense() : m(0), n(0), nkb(0), splits(1), mt(0), nt(0), per(0), wide(256) {}
+    Dense(int64_t m_, int64_t n_, int64_t k, int splits_ = 1, int laps = 1, int wide_ = 256)
+        : m((int)m_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK) * laps), splits(splits_), mt((int)((m_ + 255) / 256)), nt((int)((n_ + wide_ - 1) / wide_)),
+          per((nkb + splits_ - 1) / splits_), wide(wide_), all((uint32_t)std::min<int64_t>(tiles(), INT_MAX)), band((uint32_t)std::min<int64_t>(8LL * nt, INT_MAX)) {}
     int64_t tiles() const { return (int64_t)mt * nt; }
     int64_t units() const { return tiles() * splits; }
     // A tile's place is found in 32 bits; launch() refuses more units.
     __device__ void place(uint32_t at, tc::Tile &t) const {
         const uint32_t part = splits > 1 ? all(at) : 0, i = at - part * all.d;
-        const uint32_t block = band(i), rest = i - block * band.d, wide = min(8u, mt - block * 8);
-        const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
+        const uint32_t block = band(i), rest = i - block * band.d, tall = min(8u, mt - block * 8);
+        const uint32_t tn = tall == 8 ? rest >> 3 : rest / tall, tm = block * 8 + (rest - tn * tall);
         t.m0 = (int)(tm * 256);
-        t.n0 = (int)(tn * 256);
+        t.n0 = (int)tn * wide;
         t.mend = min(m - t.m0, 256) + t.m0;
-        t.nend = min(n - t.n0, 256) + t.n0;
+        t.nend = min(n - t.n0, wide) + t.n0;
         t.k0 = 0;
         t.q0 = min((int)part * per, nkb);
         t.nkb = min(per, nkb - t.q0);
@@ -416,7 +417,7 @@ struct XentStats {
         }
         if (!whole) {
             if (yc >= 0) ly[row] = z;
-            if (in) part[((int64_t)(t.n0 / 256) * 2 + p.half) * dense.m + row] = make_float2(m, s);
+            if (in) part[((int64_t)(t.n0 / dense.wide) * 2 + p.half) * dense.m + row] = make_float2(m, s);
             return;
         }
         st.m = m;
@@ -545,15 +546,7 @@ template <class T> struct XentG {
         T *out = g + (int64_t)row0 * ldg + t.n0 + h0;
         const int rows = t.mend - row0, cols = t.nend - t.n0 - h0;
         if (part) {
-            tc::store_tile<T>(p, addr, out, ldg, rows, cols, 8, false, value, [] {});
-            tc::store_tile<T>(
-                p, addr, out + part, ldg, rows, cols, 8, false,
-                [&](float (&x)[32], int col) {
-                    value(x, col);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) x[i] -= to_f(from_f<T>(x[i]));
-                },
-                release);
+            tc::store_parts<T>(p, addr, out, part, ldg, rows, cols, value, release);
         } else {
             tc::store_tile<T>(p, addr, out, ldg, rows, cols, 8, false, value, release);
         }
@@ -805,6 +798,15 @@ struct Room {
     int64_t bytes() const { return at - base; }
 };
 
+// Columns of the softmax's tiles: 256, or with so few of those that half the
+// clusters or more would stay idle 128 or 64, whose epilogues are as much shorter
+// (of a tile of two stages the epilogue is the longest part: 3300 clocks of
+// the loss's 256 columns, 6000 of G's).
+int xent_wide(int64_t n, int64_t v) {
+    const int64_t tiles = (n + 255) / 256 * ((v + 255) / 256);
+    return tiles <= 18 ? 64 : tiles <= 37 ? 128 : 256;
+}
+
 // Whether one cluster takes all classes of its rows: where that takes no
 // longer than tiles for all clusters and a second launch that joins their
 // parts (about 16 stages' time; a tile 4 stages on top of its own).
@@ -824,7 +826,8 @@ struct XentLoss {
         x = r.take<uint16_t>(in_place ? 0 : n * dp);
         w = r.take<uint16_t>(in_place ? 0 : v * dp);
         const bool parts = !xent_whole(n, d, v);
-        part = r.take<float2>(parts ? (v + 255) / 256 * 2 * n : 0);
+        const int64_t wide = xent_wide(n, v);
+        part = r.take<float2>(parts ? (v + wide - 1) / wide * 2 * n : 0);
         ly = r.take<float>(parts ? n : 0);
         bytes = r.bytes();
     }
@@ -860,12 +863,13 @@ Err xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, bool bf
     const View a = readable(prep, {x, d, n, ldx}, q.x), b = readable(prep, {w, d, v, ldw}, q.w);
     Err e = run_prep(prep, st);
     if (e.bad()) return e;
-    const Dense g(n, v, d);
-    XentStats op{g, xent_whole(n, d, v), target, q.part, q.ly, loss, lse};
+    const bool whole = xent_whole(n, d, v);
+    const Dense g(n, v, d, 1, 1, whole ? 256 : xent_wide(n, v));
+    XentStats op{g, whole, target, q.part, q.ly, loss, lse};
     const View ab[2] = {a, b};
     e = launch(ab, op, bf16, op.whole ? g.mt : g.units(), st);
     if (e.bad() || op.whole) return e;
-    return start(k_xent_join, (n + 7) / 8, 256, 0, st, q.part, n, (v + 255) / 256 * 2, v, target, q.ly, loss, lse);
+    return start(k_xent_join, (n + 7) / 8, 256, 0, st, q.part, n, g.nt * 2LL, v, target, q.ly, loss, lse);
 }
 
 template <class T>
@@ -931,7 +935,7 @@ Err xent_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_
         wp.p = (const char *)wv.p + c * wv.ld * 2;
         wp.rows = pc;
         const bool first = own && c == 0;
-        XentG<T> og{Dense(n, pc, d), c, v, target, lse, grad_loss, first ? nullptr : scale, g, pl.ldg, pl.parts > 1 ? n * pl.ldg : 0,
+        XentG<T> og{Dense(n, pc, d, 1, 1, xent_wide(n, pc)), c, v, target, lse, grad_loss, first ? nullptr : scale, g, pl.ldg, pl.parts > 1 ? n * pl.ldg : 0,
                     first ? copy : PackJob{}, tc::Div((uint32_t)(pl.dp / 8)), first ? scale : nullptr};
         const View xw[2] = {xv, wp};
         e = launch(xw, og, bf16, og.dense.units(), st);

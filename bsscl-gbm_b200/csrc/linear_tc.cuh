@@ -413,21 +413,22 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     const uint32_t rank = cluster_rank();
     const int cid = blockIdx.x / 2, ncl = gridDim.x / 2;
 
-    if (warp == 0 && lane == 0) {
-        for (int i = 0; i < (Op::kDual ? 4 : 2); i++) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.m[i]) : "memory");
-        for (int s = 0; s < kStages; s++) {
-            mbar_init(full + 8 * s, 1);
-            mbar_init(empty + 8 * s, 1);
+    if (warp == 0) {
+        // a lane a barrier: one lane for all 44 took 400 clocks
+        if (lane < (Op::kDual ? 4 : 2)) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.m[lane]) : "memory");
+        if (lane < kStages) {
+            mbar_init(full + 8 * lane, 1);
+            mbar_init(empty + 8 * lane, 1);
             // one a stage: a CTA ahead of the other by a whole short tile must not count for both
-            mbar_init(fixed + 8 * s, 2);
-            mbar_init(tailbar + 8 * s, 1);
+            mbar_init(fixed + 8 * lane, 2);
+            mbar_init(tailbar + 8 * lane, 1);
         }
-        for (int s = 0; s < 2; s++) {
-            mbar_init(tfull + 8 * s, 1);
-            mbar_init(tempty + 8 * s, 2 * kEpiWarps);
+        if (lane < 2) {
+            mbar_init(tfull + 8 * lane, 1);
+            mbar_init(tempty + 8 * lane, 2 * kEpiWarps);
         }
-        for (int s = 0; s < 16; s++) mbar_init(swap + 8 * s, 1);
-        *dead = 0;
+        if (lane < 16) mbar_init(swap + 8 * lane, 1);
+        if (lane == 0) *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -583,6 +584,10 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
     return *reinterpret_cast<uint32_t *>(&v);
 }
 
+template <class T> __device__ __forceinline__ float unpack(uint32_t bits);
+template <> __device__ __forceinline__ float unpack<__nv_bfloat16>(uint32_t bits) { return __uint_as_float(bits << 16); }
+template <> __device__ __forceinline__ float unpack<__half>(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
+
 // Elements of one store that rows at `p`, `ld` apart, allow: 8, 4, 2 or 1.
 __host__ __device__ inline int store_width(const void *p, int64_t ld) {
     const uint64_t a = (uint64_t)(uintptr_t)p | (uint64_t)ld * 2;
@@ -609,6 +614,56 @@ __device__ __forceinline__ void store_rows(const uint8_t *staging, int lane, T *
 #pragma unroll
             for (int k = 0; k < W - 1; k++)
                 if (c + k < cols) ((uint16_t *)to)[k] = ((const uint16_t *)from)[k];
+        }
+    }
+}
+
+// The same sums in two parts: rounded to T at out, and what the rounding left,
+// rounded too, at out + part; 32 columns of each at a time.  Rows start on
+// 16-byte boundaries.
+template <class T, class F, class R>
+__device__ __forceinline__ void store_parts(const Place &p, uint32_t addr, T *out, int64_t part, int64_t ld, int rows, int cols, F f, R release) {
+    if (rows <= 0) {
+        release();
+        return;
+    }
+#pragma unroll 1
+    for (int c = 0; c < p.wide; c += 32) {
+        __syncwarp();
+        float v[32];
+        tmem_ld32(addr + c, v);
+        tmem_wait(v);
+        if (c + 32 >= p.wide) release();
+        f(v, c);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t a[4], b[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float x = v[8 * i + 2 * k], y = v[8 * i + 2 * k + 1];
+                a[k] = pack2<T>(x, y);
+                b[k] = pack2<T>(x - unpack<T>(a[k] & 0xFFFF), y - unpack<T>(a[k] >> 16));
+            }
+            *(uint4 *)(p.staging + p.lane * 128 + ((i ^ (p.lane & 7)) * 16)) = make_uint4(a[0], a[1], a[2], a[3]);
+            *(uint4 *)(p.staging + p.lane * 128 + (((i + 4) ^ (p.lane & 7)) * 16)) = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+        __syncwarp();
+        const int lim = min(cols, p.wide) - c;
+        if (lim <= 0) continue;
+#pragma unroll 4
+        for (int i = p.lane; i < 32 * 8; i += 32) {
+            const int r = i / 8, ch = i % 8, col = ch % 4 * 8;
+            if (r >= rows || col >= lim) continue;
+            const uint4 q = *(const uint4 *)(p.staging + r * 128 + ((ch ^ (r & 7)) * 16));
+            T *to = out + (ch / 4) * part + (int64_t)r * ld + c + col;
+            if (col + 8 <= lim) {
+                *(uint4 *)to = q;
+            } else {
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int k = 0; k < 7; k++)
+                    if (col + k < lim) ((uint16_t *)to)[k] = (uint16_t)(w[k / 2] >> (k & 1) * 16);
+            }
         }
     }
 }
