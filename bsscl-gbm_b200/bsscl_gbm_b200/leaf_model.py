@@ -53,7 +53,8 @@ class LeafLinearClassifier:
     regression) whose tree ``tree`` routes the rows; None = one leaf.  Trained
     by stochastic gradient descent on the class-weighted log-loss
     (class_weight as the estimator's), the gradients clipped to ``max_norm``.
-    Weights are kept in float32 and multiplied in ``dtype``.  Features are standardised; a missing value counts as the mean.
+    Weights are kept in float32 and multiplied in ``dtype``.  Features are
+    standardised; a missing or infinite value counts as the mean.
     """
 
     def __init__(self, router=None, tree=0, n_hidden=64, learning_rate=0.5, max_norm=1.0, n_epochs=10, batch_size=8192,

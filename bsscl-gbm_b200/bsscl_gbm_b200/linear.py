@@ -74,8 +74,10 @@ class GradClip:
     """The global 2-norm of many gradients, and clipping to it.
 
     Made once for the gradients of a model (a list of CUDA tensors of one
-    device; float32, bfloat16 or float16, each dense), whose buffers it keeps; ``out`` (default: the gradients themselves) takes the
-    clipped values.  No two buffers may overlap, but out[i] may be grads[i].
+    device; float32, bfloat16 or float16, each dense), whose buffers it keeps;
+    ``out`` (default: the gradients themselves) takes the clipped values.  No
+    two buffers may overlap, but out[i] may be grads[i], and calls on two
+    streams at once would write the same outputs: wait between them.
     """
 
     def __init__(self, grads, out=None):

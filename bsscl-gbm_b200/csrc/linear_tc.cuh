@@ -468,8 +468,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                     }
                 }
             }
-            __syncwarp();
-            if (*dead) break;
+            if (__any_sync(~0u, *dead)) break;
             r.skip(t.nkb);
         }
     } else if (warp == 1) {
@@ -503,8 +502,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                     }
                     if (ok) commit_pair(tfull + 8 * buf);
                 }
-                __syncwarp();
-                if (*dead) break;
+                if (__any_sync(~0u, *dead)) break;
                 if (tail) fixed_ph ^= 1u << last;
                 r.skip(t.nkb);
                 n++;
