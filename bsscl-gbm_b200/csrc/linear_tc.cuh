@@ -16,7 +16,9 @@
 // Warp 0 fetches, warp 1 of the leading CTA issues the products, warps 2..9
 // run the epilogue (warp w reads the tensor memory lanes 32 (w % 4) .. +31,
 // warps 2..5 the tile's left columns, warps 6..9 its right ones), warp 10
-// puts zeros behind a k axis that ends inside a stage.  The thread that
+// tells the products' thread of its tiles and puts zeros behind a k axis that
+// ends inside a stage.  (Few products wait in the tensor core's queue: looking for the
+// next tile, 500 clocks, 1500 among leaves, by the products' own warp idled it.)  The thread that
 // fetches and the one that issues products are chosen by elect.sync: under a
 // plain test of the lane the compiler does not know that one thread runs, and
 // the loops took up to 20 % more clocks than the products.
@@ -44,6 +46,7 @@ constexpr long long kWaitClocks = 4000000000ll;   // about 2 s
 static __device__ int g_ops_timeout;
 
 constexpr int kBN = 256;
+constexpr int kTold = 4;                      // tiles the products' thread may know of ahead
 constexpr int kStageBytes = kABytes + kBN / 2 * kBK * 2;
 constexpr int kStages = (227 * 1024 - kStaging - 2048) / kStageBytes;
 constexpr int kSmem = kStages * kStageBytes + kStaging + 2048;   // 1024 of alignment, 1024 of barriers
@@ -406,15 +409,17 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     const uint32_t stages = smem_u32(base);
     const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16,
                    fixed = tempty + 16, tailbar = fixed + 8 * kStages;
-    const uint32_t swap = tailbar + 8 * kStages;
-    uint32_t *tmem_slot = (uint32_t *)(bars + 4 * kStages + 20);
+    const uint32_t swap = tailbar + 8 * kStages, told = swap + 8 * 16, heard = told + 8 * kTold;
+    int4 *tiles = (int4 *)(bars + 4 * kStages + 20 + 2 * kTold);     // told: stages, columns, tail, kind
+    static_assert((4 * kStages + 20 + 2 * kTold) % 2 == 0, "");
+    uint32_t *tmem_slot = (uint32_t *)(tiles + kTold);
     volatile int *dead = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cluster_rank();
     const int cid = blockIdx.x / 2, ncl = gridDim.x / 2;
 
     if (warp == 0) {
-        // a lane a barrier: one lane for all 44 took 400 clocks
+        // a lane a barrier: one lane for all took 400 clocks
         if (lane < (Op::kDual ? 4 : 2)) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.m[lane]) : "memory");
         if (lane < kStages) {
             mbar_init(full + 8 * lane, 1);
@@ -428,6 +433,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
             mbar_init(tempty + 8 * lane, 2 * kEpiWarps);
         }
         if (lane < 16) mbar_init(swap + 8 * lane, 1);
+        if (lane < 2 * kTold) mbar_init(told + 8 * lane, 1);
         if (lane == 0) *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -473,51 +479,62 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         }
     } else if (warp == 1) {
         // ---- products, issued by one thread too
-        if (rank == 0) {
+        if (rank == 0 && elect_one()) {
             Ring r;
-            int n = 0;
             uint32_t fixed_ph = 0;
-            typename Op::Iter it(op, cid, ncl);
-            Tile t;
-            while (it.next(op, t)) {
-                const int buf = n & 1;
-                const bool tail = Op::kTail && t.tail && t.nkb, second = Op::kDual && t.kind == 1;
-                const int last = (r.s + t.nkb - 1) % kStages;     // the tail's stage
-                __syncwarp();
-                if (elect_one()) {
-                    bool ok = mbar_wait(tempty + 8 * buf, ((n >> 1) & 1) ^ 1, dead);
+            for (int n = 0;; n++) {
+                const int buf = n & 1, slot = n % kTold;
+                if (!mbar_wait(told + 8 * slot, n / kTold & 1, dead)) break;
+                const int4 t = tiles[slot];
+                mbar_arrive(heard + 8 * slot);
+                if (t.x < 0) break;
+                const bool tail = Op::kTail && t.z, second = Op::kDual && t.w;
+                if (!mbar_wait(tempty + 8 * buf, ((n >> 1) & 1) ^ 1, dead)) break;
+                fence_after();
+                const uint32_t d = tmem + buf * kBN, id = idesc | (uint32_t)(t.y >> 3) << 17;
+                if (!(second ? multiply<Op, true>(d, t.x - tail, r, stages, full, empty, id, dead)
+                             : multiply<Op, Op::kAMN>(d, t.x - tail, r, stages, full, empty, id, dead)))
+                    break;
+                if (tail) {
+                    if (!mbar_wait(full + 8 * r.s, r.ph, dead) || !mbar_wait<true>(fixed + 8 * r.s, fixed_ph >> r.s & 1, dead)) break;
                     fence_after();
-                    const uint32_t d = tmem + buf * kBN, id = idesc | (uint32_t)(t.cols() >> 3) << 17;
-                    Ring q = r;
-                    if (ok)
-                        ok = second ? multiply<Op, true>(d, t.nkb - tail, q, stages, full, empty, id, dead)
-                                    : multiply<Op, Op::kAMN>(d, t.nkb - tail, q, stages, full, empty, id, dead);
-                    if (ok && tail) {
-                        ok = mbar_wait(full + 8 * q.s, q.ph, dead) && mbar_wait<true>(fixed + 8 * q.s, fixed_ph >> q.s & 1, dead);
-                        fence_after();
-                        if (ok) {
-                            multiply_stage<Op, true>(d, stages + q.s * kStageBytes, id, t.nkb > 1);
-                            commit_pair(empty + 8 * q.s);
-                        }
-                    }
-                    if (ok) commit_pair(tfull + 8 * buf);
+                    multiply_stage<Op, true>(d, stages + r.s * kStageBytes, id, t.x > 1);
+                    commit_pair(empty + 8 * r.s);
+                    fixed_ph ^= 1u << r.s;
+                    r.step();
                 }
-                if (__any_sync(~0u, *dead)) break;
-                if (tail) fixed_ph ^= 1u << last;
-                r.skip(t.nkb);
-                n++;
+                commit_pair(tfull + 8 * buf);
             }
         }
     } else if (warp == 2 + kEpiWarps) {
-        // ---- the last stage of a k axis that ends inside it: rows behind the
-        // end belong to the next leaf; zeros take their place before the
-        // products see them
-        if (Op::kTail) {
-            Ring r;
-            uint32_t ph = 0;
-            typename Op::Iter it(op, cid, ncl);
-            Tile t;
-            while (it.next(op, t)) {
+        // ---- tells the products' thread of the next tile, then sees to the
+        // current one's last stage where its k axis ends inside it: rows
+        // behind the end belong to the next leaf; zeros take their place
+        // before the products see them
+        Ring r;
+        uint32_t ph = 0;
+        typename Op::Iter it(op, cid, ncl);
+        Tile t, next{};
+        int n = 0;
+        auto tell = [&](bool more) {
+            if (rank) return true;
+            const int slot = n % kTold;
+            if (!mbar_wait_warp(heard + 8 * slot, (n / kTold & 1) ^ 1, dead)) return false;
+            if (lane == 0) {
+                tiles[slot] = make_int4(more ? next.nkb : -1, next.cols(), next.tail && next.nkb, next.kind);
+                mbar_arrive(told + 8 * slot);
+            }
+            __syncwarp();
+            n++;
+            return true;
+        };
+        bool more = it.next(op, next);
+        if (tell(more))
+            while (more) {
+                t = next;
+                more = it.next(op, next);
+                if (!tell(more)) break;
+                if (!Op::kTail) continue;
                 r.skip(t.nkb);
                 if (!t.tail || !t.nkb) continue;
                 const int s = r.s == 0 ? kStages - 1 : r.s - 1;
@@ -530,7 +547,6 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                 __syncwarp();
                 if (lane == 0) mbar_arrive_at<true>(fixed + 8 * s, 0);
             }
-        }
     } else {
         // ---- epilogue
         Place p;
