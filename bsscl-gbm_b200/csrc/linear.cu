@@ -1385,8 +1385,12 @@ __global__ void __launch_bounds__(256, kClipBlocks) k_clip(const ClipPlan *__res
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, shares = plan->shares;
     for (int b = blockIdx.x; b < shares; b += gridDim.x) {
         double s[4] = {0, 0, 0, 0};
-        for (int i = plan->start[b]; i < plan->start[b + 1]; i++) {
-            const ClipItem it = items[i];
+        const int end = plan->start[b + 1];
+        int i = plan->start[b];
+        ClipItem next = items[min(i, end - 1)];      // a piece's place is on its way while the one before it is read
+        for (; i < end; i++) {
+            const ClipItem it = next;
+            next = items[min(i + 1, end - 1)];
             if (it.dtype == GBM_TYPE_F32)
                 sum_sq((const float *)it.src, it.n, s);
             else if (it.dtype == GBM_TYPE_BF16)
@@ -1415,9 +1419,13 @@ __global__ void __launch_bounds__(256, kClipBlocks) k_clip(const ClipPlan *__res
     const double r = sqrt(t), f = max_norm / (r + 1e-6);
     const float c = (float)(f > 1.0 ? 1.0 : f);
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)r;
-    for (int b = blockIdx.x; b < shares; b += gridDim.x)
-        for (int i = plan->start[b + 1] - 1; i >= plan->start[b]; i--) {
-            const ClipItem it = items[i];
+    for (int b = blockIdx.x; b < shares; b += gridDim.x) {
+        const int begin = plan->start[b];
+        int i = plan->start[b + 1] - 1;
+        ClipItem next = items[max(i, begin)];
+        for (; i >= begin; i--) {
+            const ClipItem it = next;
+            next = items[max(i - 1, begin)];
             if (c == 1.f && it.src == it.dst) continue;
             if (it.dtype == GBM_TYPE_F32)
                 scale_to((const float *)it.src, (float *)it.dst, it.n, c);
@@ -1426,6 +1434,7 @@ __global__ void __launch_bounds__(256, kClipBlocks) k_clip(const ClipPlan *__res
             else
                 scale_to((const __half *)it.src, (__half *)it.dst, it.n, c);
         }
+    }
 }
 
 // Calls item(gradient, first element, elements, share) for the pieces of all
@@ -1684,6 +1693,13 @@ int gbm_grad_clip(const void *plan_host, const void *plan_dev, double max_norm, 
     cudaError_t e = cudaLaunchCooperativeKernel((const void *)k_clip, dim3((unsigned)blocks), dim3(256), args, 0, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return fail(errbuf, errlen, GBM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
     return GBM_OK;
+}
+
+int gbm_test_ops_wait(int32_t timeout_ms, void *stream, char *errbuf, int32_t errlen) {
+    if (timeout_ms < 1 || timeout_ms > 10000) return fail(errbuf, errlen, GBM_ERR_ARG, "gbm_test_ops_wait: %d ms", timeout_ms);
+    Err e = start(tc::k_wait, 1, 32, 0, static_cast<cudaStream_t>(stream), timeout_ms * 2000000ll);
+    if (e.bad()) return fail(errbuf, errlen, e.code, "gbm_test_ops_wait: %s", e.what);
+    return gbm_ops_status(stream, errbuf, errlen);
 }
 
 int gbm_ops_status(void *stream, char *errbuf, int32_t errlen) {

@@ -98,14 +98,14 @@ template <bool DATA> __device__ __forceinline__ bool mbar_try(uint32_t bar, uint
     return ok;
 }
 // Waits for the phase of this parity; false when the wait ran out here or in another warp of the CTA.
-template <bool DATA = false> __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead) {
+template <bool DATA = false> __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead, long long limit = kWaitClocks) {
     if (mbar_try<DATA>(bar, parity)) return true;
     const long long t0 = clock64();
     for (uint32_t i = 1;; i++) {
         if (mbar_try<DATA>(bar, parity)) return true;
         if ((i & 31) == 0) {
             if (*dead) return false;
-            if (clock64() - t0 > kWaitClocks) {
+            if (clock64() - t0 > limit) {
                 *dead = 1;
                 g_ops_timeout = 1;
                 return false;
@@ -584,6 +584,19 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     __syncthreads();
     cluster_sync();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+}
+
+// A wait that nothing ends, for the test of what a wait that runs out does.
+__global__ void k_wait(long long clocks) {
+    depend();
+    __shared__ uint64_t bar;
+    __shared__ int dead;
+    if (threadIdx.x == 0) {
+        dead = 0;
+        mbar_init(smem_u32(&bar), 1);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) mbar_wait(smem_u32(&bar), 0, &dead, clocks);
 }
 
 // ---- epilogues --------------------------------------------------------------

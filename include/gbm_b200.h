@@ -489,6 +489,12 @@ int64_t gbm_grad_clip_workspace(const void *plan_host);
  * asynchronous error (GBM_ERR_CUDA). */
 int gbm_ops_status(void *stream, char *errbuf, int32_t errlen);
 
+/* Failure-detection self test: on the current device, the operators' bounded
+ * wait for a signal that nothing sends, limited to about `timeout_ms`
+ * (1..10000) at 2 GHz, then gbm_ops_status: GBM_ERR_TIMEOUT when the wait ran
+ * out and said so.  Nothing is left waiting. */
+int gbm_test_ops_wait(int32_t timeout_ms, void *stream, char *errbuf, int32_t errlen);
+
 /* Synchronise the context's stream; returns the first asynchronous error
  * (no reference counterpart). */
 int gbm_sync(gbm_ctx *ctx);

@@ -52,6 +52,22 @@ def test_leaf_of_rows_follows_the_tree():
 
 
 @pytest.mark.gpu
+def test_routers_of_other_kinds():
+    """A multi-class, a regression and a NaN-direction model's trees route rows too."""
+    from bsscl_gbm_b200 import HybridHistGBMNumbaV1_0_1, HybridHistGBMRegressorV1_0_1, LeafLinearClassifier, leaf_of_rows
+    X, y = _data(n=1200, classes=70)
+    z = np.nan_to_num(X[:, 0]) + np.nan_to_num(X[:, 1])
+    kw = dict(n_estimators=2, max_depth=3, random_state=0, verbose=False)
+    for model, labels in ((HybridHistGBMNumbaV1_0_1(**kw), np.digitize(z, [-0.5, 0.5])), (HybridHistGBMRegressorV1_0_1(**kw), z),
+                          (HybridHistGBMNumbaV1_0_1(nan_direction='learn', **kw), (z > 0).astype(int))):
+        model.fit(X, labels)
+        leaf, count = leaf_of_rows(model, X, 1)
+        assert count > 1 and set(np.unique(leaf)) <= set(range(count)) and len(np.unique(leaf)) > 1
+        m = LeafLinearClassifier(model, tree=1, n_hidden=8, n_epochs=1).fit(X, y)
+        assert m.n_leaves_ == count and np.isfinite(m.predict_proba(X[:50])).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("routed", [False, True])
 def test_fit_and_answers(routed, dtype):

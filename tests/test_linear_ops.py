@@ -584,6 +584,54 @@ def test_captured_clip_follows_its_gradients():
         _near(norm, want, want * (2.0 ** -24 + 1e-12), "norm")
 
 
+@gpu
+def test_two_threads_at_once():
+    """Calls from two host threads on streams of their own."""
+    import threading
+    problems, want, got = [_problem(21), _problem(22, n=700, v=2500)], [], [None, None]
+    for p in problems:
+        want.append(_step(p, clip=False))
+    torch.cuda.synchronize()
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[k] = _step(problems[k], clip=False)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g[:6], w[:6]))
+
+
+@gpu
+def test_a_wait_that_runs_out_is_reported_once():
+    from bsscl_gbm_b200 import lib, linear
+    linear.status()
+    err = C.create_string_buffer(256)
+    assert lib().gbm_test_ops_wait(20, None, err, 256) == 6 and b"ran out" in err.value
+    linear.status()                                    # told once, and the context is usable
+    assert lib().gbm_test_ops_wait(0, None, err, 256) == ARG
+    s = _problem(1)
+    assert torch.isfinite(_step(s)[1]).all()
+
+
+@gpu
+def test_leaves_of_a_graph_and_long_features():
+    """Parameters that require gradients, and more features than a product has stages many times over."""
+    from bsscl_gbm_b200 import linear
+    s = _problem(9)
+    w = s["w"].clone().requires_grad_()
+    y = linear.leaf_linear(s["x"], w, s["off"])
+    assert not y.requires_grad and torch.equal(y, linear.leaf_linear(s["x"], s["w"], s["off"]))
+    x, head = _rand((5, 70_001), torch.bfloat16, 1), _rand((9, 70_001), torch.bfloat16, 2, 0.005)
+    _check_xent(x, head, _targets(5, 9, 0.0, 3), torch.ones(5, device="cuda"))
+
+
 # ---------------------------------------------------------------------------
 # refusals (no GPU: nothing is launched)
 # ---------------------------------------------------------------------------
