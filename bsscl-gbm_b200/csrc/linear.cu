@@ -206,10 +206,17 @@ __global__ void __launch_bounds__(256) k_prep(const __grid_constant__ Prep p) {
     if ((int)blockIdx.x == work) {
         __shared__ float red[8];
         float m = 0.f;
-#pragma unroll 8
-        for (int64_t i = threadIdx.x; i < p.n; i += 256) {
-            const int64_t y = p.target[i];
-            m = fmaxf(m, y >= 0 && y < p.v ? fabsf(p.grad_loss[i]) : 0.f);
+        for (int64_t i = threadIdx.x; i < p.n; i += 256 * 16) {     // 16 rows of a thread on their way at a time
+            int64_t y[16];
+            float g[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const int64_t r = min(i + 256 * k, p.n - 1);
+                y[k] = p.target[r];
+                g[k] = p.grad_loss[r];
+            }
+#pragma unroll
+            for (int k = 0; k < 16; k++) m = fmaxf(m, y[k] >= 0 && y[k] < p.v ? fabsf(g[k]) : 0.f);
         }
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
         if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
@@ -452,7 +459,13 @@ __global__ void __launch_bounds__(256) k_xent_join(const float2 *__restrict__ pa
     const int64_t row = blockIdx.x * 8LL + r;
     float2 a = make_float2(-INFINITY, 0.f);
     if (row < n)
-        for (int64_t k = q; k < nt; k += 32) a = join(a, part[k * n + row]);
+        for (int64_t k = q; k < nt; k += 32 * 8) {      // eight parts on their way at a time
+            float2 b[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) b[j] = k + 32 * j < nt ? part[(k + 32 * j) * n + row] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) a = join(a, b[j]);
+        }
     sh[q][r] = a;
     __syncthreads();
     for (int o = 16; o; o >>= 1) {
@@ -1229,8 +1242,9 @@ Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off,
     }
     if (dw) {
         const int64_t own = (int64_t)groups * s * mt * nt;
-        // more units than clusters: their order decides how evenly the clusters end
-        if (own > sm_count() / 2 && groups > 1 && groups <= kSortLeaves && !e.bad()) {
+        // more units than clusters: their order decides how evenly the
+        // clusters end, which is worth a launch (3 us) from some 64 stages (17 us) a cluster on
+        if (own > sm_count() / 2 && (t / 64) * mt * nt >= 64LL * 74 && groups > 1 && groups <= kSortLeaves && !e.bad()) {
             e = start(k_leaf_order, 1, 1024, 0, st, off, groups, t, q.order);
             op.order = q.order;
         }
@@ -1258,7 +1272,7 @@ Err leaf_backward(const void *x, int64_t ldx, const void *w, const int32_t *off,
 constexpr uint64_t kClipMagic = 0x47424d434c495031ull;
 constexpr int kClipBlocks = 4;                // blocks of 256 threads an SM
 constexpr int kClipShares = 148 * kClipBlocks;
-constexpr int64_t kClipLeast = 2048;          // elements of a share: a thread's 8
+constexpr int64_t kClipLeast = 512;           // elements of a share: a thread's 2, so that many small gradients are not read one behind the other
 
 struct ClipItem {
     const void *src;

@@ -629,7 +629,7 @@ __host__ __device__ inline int store_width(const void *p, int64_t ld) {
 template <int W, class V, class T>
 __device__ __forceinline__ void store_rows(const uint8_t *staging, int lane, T *out, int64_t ld, int rows, int cols) {
     constexpr int kLanes = 64 / W;      // of a row
-#pragma unroll(W == 8 ? 4 : 2)
+#pragma unroll 4
     for (int i = lane; i < 32 * kLanes; i += 32) {
         const int r = i / kLanes, c = i % kLanes * W;
         if (r >= rows || c >= cols) continue;
