@@ -314,6 +314,66 @@ struct DenseIter {
 };
 
 // ---------------------------------------------------------------------------
+// few rows
+// ---------------------------------------------------------------------------
+
+// With a few rows a product is a read of the weights, which a 256-row tile's
+// loads (128 bytes of each of 128 rows at a time) take at 5 TB/s at
+// most.  Here a warp takes 16 rows of weights as the m16 of mma.m16n8k16 and
+// reads 512 bytes of each at a time, straight into the operand's registers: a lane's
+// 16 bytes are 8 values of k of one row, and as both operands are read alike,
+// it does not matter that the instruction counts these k's in another order.
+
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __half) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// acc[i][h + 2 j] = w row (g + 8 j) . x row (8 i + 2 c + h), for lane 4 g + c;
+// wrows <= 16 and xrows <= 8 NT rows exist (others repeat the last one), K is
+// a multiple of 8 and rows start on 16-byte boundaries.
+template <class T, int NT>
+__device__ __forceinline__ void dot_few(const T *w, int64_t ldw, int wrows, const T *x, int64_t ldx, int xrows, int K, float (&acc)[NT][4]) {
+    constexpr int kDeep = NT == 1 ? 8 : 4;      // steps of 32 values of k on their way
+    const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4 * 8;
+    const T *w0 = w + min(g, wrows - 1) * ldw + c, *w1 = w + min(g + 8, wrows - 1) * ldw + c;
+    const T *xr[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        xr[i] = x + min(8 * i + g, xrows - 1) * ldx + c;
+        acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    }
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    for (int k0 = 0; k0 < K; k0 += 32 * kDeep) {
+        uint4 a[kDeep], b[kDeep], q[NT][kDeep];
+#pragma unroll
+        for (int u = 0; u < kDeep; u++) {
+            const int k = k0 + 32 * u;
+            const bool in = k + c < K;
+            a[u] = in ? __ldcs((const uint4 *)(w0 + k)) : none;
+            b[u] = in ? __ldcs((const uint4 *)(w1 + k)) : none;
+#pragma unroll
+            for (int i = 0; i < NT; i++) q[i][u] = in ? __ldg((const uint4 *)(xr[i] + k)) : none;
+        }
+#pragma unroll
+        for (int u = 0; u < kDeep; u++)
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                mma16(acc[i], a[u].x, b[u].x, a[u].y, b[u].y, q[i][u].x, q[i][u].y, T{});
+                mma16(acc[i], a[u].z, b[u].z, a[u].w, b[u].w, q[i][u].z, q[i][u].w, T{});
+            }
+    }
+}
+
+constexpr int kFewBlocks = 2;     // blocks of 8 warps an SM
+
+// ---------------------------------------------------------------------------
 // softmax cross entropy
 // ---------------------------------------------------------------------------
 
@@ -811,6 +871,65 @@ struct Room {
     int64_t bytes() const { return at - base; }
 };
 
+// The loss's parts for up to 8 NT rows: a warp takes 16 classes at a time and
+// keeps each row's maximum and sum of exponentials over them; part [block][row].
+template <class T, int NT>
+__global__ void __launch_bounds__(256, kFewBlocks) k_xent_few(const T *x, int64_t ldx, const T *w, int64_t ldw, int n, int d, int v,
+                                                             const int64_t *__restrict__ target, float2 *__restrict__ part, float *__restrict__ ly) {
+    tc::depend();
+    __shared__ float2 red[8][8 * NT];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+    float2 st[NT][2];
+    int y[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int row = 8 * i + 2 * c + h;
+            const int64_t t = row < n ? target[row] : -1;
+            y[i][h] = t >= 0 && t < v ? (int)t : -1;
+            st[i][h] = make_float2(-INFINITY, 0.f);
+        }
+    for (int64_t k0 = (blockIdx.x * 8LL + warp) * 16; k0 < v; k0 += gridDim.x * 128LL) {
+        float acc[NT][4];
+        dot_few<T, NT>(w + k0 * ldw, ldw, (int)min(v - k0, (int64_t)16), x, ldx, n, d, acc);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int64_t k = k0 + g + 8 * j;
+            if (k >= v) continue;
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float l = acc[i][h + 2 * j];
+                    if (y[i][h] == k) ly[8 * i + 2 * c + h] = l;
+                    // a NaN is no maximum, but stays in the sum
+                    st[i][h] = join(st[i][h], make_float2(isnan(l) ? -INFINITY : l, isnan(l) ? l : 1.f));
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float2 a = st[i][h];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) a = join(a, make_float2(__shfl_xor_sync(~0u, a.x, o), __shfl_xor_sync(~0u, a.y, o)));
+            if (g == 0) red[warp][8 * i + 2 * c + h] = a;
+        }
+    __syncthreads();
+    const int row = threadIdx.x;
+    if (row >= n) return;
+    float2 a = red[0][row];
+#pragma unroll
+    for (int k = 1; k < 8; k++) a = join(a, red[k][row]);
+    part[(int64_t)blockIdx.x * n + row] = a;
+}
+
+// Up to this many rows the loss reads the weights at the memory's rate in k_xent_few.
+constexpr int kFewRows = 32;
+int64_t few_blocks(int64_t v) { return std::min<int64_t>((v + 127) / 128, 148 * kFewBlocks); }
+
 // Columns of the softmax's tiles: 256, or with so few of those that half the
 // clusters or more would stay idle 128 or 64, whose epilogues are as much shorter
 // (of a tile of two stages the epilogue is the longest part: 3300 clocks of
@@ -840,7 +959,7 @@ struct XentLoss {
         w = r.take<uint16_t>(in_place ? 0 : v * dp);
         const bool parts = !xent_whole(n, d, v);
         const int64_t wide = xent_wide(n, v);
-        part = r.take<float2>(parts ? (v + wide - 1) / wide * 2 * n : 0);
+        part = r.take<float2>(parts ? std::max((v + wide - 1) / wide * 2, few_blocks(v)) * n : 0);
         ly = r.take<float>(parts ? n : 0);
         bytes = r.bytes();
     }
@@ -877,6 +996,21 @@ Err xent_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, bool bf
     Err e = run_prep(prep, st);
     if (e.bad()) return e;
     const bool whole = xent_whole(n, d, v);
+    if (!whole && n <= kFewRows && tma_rows(x, ldx) && tma_rows(w, ldw) && d % 8 == 0) {
+        const int64_t blocks = few_blocks(v);
+        auto run = [&](auto type, auto rows) {
+            using T = decltype(type);
+            return start(k_xent_few<T, decltype(rows)::value>, blocks, 256, 0, st, (const T *)x, ldx, (const T *)w, ldw, (int)n, (int)d, (int)v, target, q.part,
+                         q.ly);
+        };
+        auto go = [&](auto type) {
+            return n <= 8 ? run(type, std::integral_constant<int, 1>{})
+                          : n <= 16 ? run(type, std::integral_constant<int, 2>{}) : run(type, std::integral_constant<int, 4>{});
+        };
+        Err f = bf16 ? go(__nv_bfloat16{}) : go(__half{});
+        if (f.bad()) return f;
+        return start(k_xent_join, (n + 7) / 8, 256, 0, st, q.part, n, blocks, v, target, q.ly, loss, lse);
+    }
     const Dense g(n, v, d, 1, 1, whole ? 256 : xent_wide(n, v));
     XentStats op{g, whole, target, q.part, q.ly, loss, lse};
     const View ab[2] = {a, b};
@@ -974,15 +1108,16 @@ struct Leaves {
     int32_t groups;
     int n;              // columns of the result
     int nkb, nt;
+    int tall, wide;     // rows and columns of a tile
     tc::Div band;       // tiles in 8 rows of tiles
-    Leaves(const int32_t *off_, int64_t t_, int32_t groups_, int64_t k, int64_t n_)
-        : off(off_), t(t_), groups(groups_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK)), nt((int)((n_ + 255) / 256)),
-          band((uint32_t)std::min<int64_t>(8LL * nt, INT_MAX)) {}
+    Leaves(const int32_t *off_, int64_t t_, int32_t groups_, int64_t k, int64_t n_, int tall_ = 256, int wide_ = 256)
+        : off(off_), t(t_), groups(groups_), n((int)n_), nkb((int)((k + tc::kBK - 1) / tc::kBK)), nt((int)((n_ + wide_ - 1) / wide_)), tall(tall_),
+          wide(wide_), band((uint32_t)std::min<int64_t>(8LL * nt, INT_MAX)) {}
     // tiles at most: each leaf may end in a part of one
-    int64_t units() const { return ((t + 255) / 256 + groups) * nt; }
+    int64_t units() const { return ((t + tall - 1) / tall + groups) * nt; }
 };
 
-// The 256 x 256 tiles of all leaves' rows, leaf after leaf.  A warp looks
+// The tiles of all leaves' rows, leaf after leaf.  A warp looks
 // through 32 leaves at a time: each lane counts one leaf's tiles.
 struct LeafIter {
     uint32_t at, step, base, total, upto;    // tiles before these 32 leaves, in them, in them up to this lane's
@@ -998,7 +1133,7 @@ struct LeafIter {
         lo = next_lo;
         hi = next_hi;
         fetch(op, g + 32);
-        upto = (uint32_t)((hi - lo + 255) / 256) * op.leaves.nt;
+        upto = (uint32_t)((hi - lo + op.leaves.tall - 1) / op.leaves.tall) * op.leaves.nt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t u = __shfl_up_sync(~0u, upto, o);
@@ -1016,14 +1151,14 @@ struct LeafIter {
         const uint32_t rel = at - base, nt = op.leaves.nt;
         const int l = __ffs(__ballot_sync(~0u, upto > rel)) - 1;
         const int a = __shfl_sync(~0u, lo, l), b = __shfl_sync(~0u, hi, l);
-        const uint32_t end = __shfl_sync(~0u, upto, l), rt = (b - a + 255) / 256, i = rel - (end - rt * nt);
+        const uint32_t end = __shfl_sync(~0u, upto, l), rt = (b - a + op.leaves.tall - 1) / op.leaves.tall, i = rel - (end - rt * nt);
         // 8 row tiles beside one another, as in Dense
-        const uint32_t block = op.leaves.band(i), rest = i - block * op.leaves.band.d, wide = min(8u, rt - block * 8);
-        const uint32_t tn = wide == 8 ? rest >> 3 : rest / wide, tm = block * 8 + (rest - tn * wide);
-        t.m0 = a + (int)tm * 256;
-        t.n0 = (int)(tn * 256);
-        t.mend = min(b - t.m0, 256) + t.m0;
-        t.nend = min(op.leaves.n - t.n0, 256) + t.n0;
+        const uint32_t block = op.leaves.band(i), rest = i - block * op.leaves.band.d, tall = min(8u, rt - block * 8);
+        const uint32_t tn = tall == 8 ? rest >> 3 : rest / tall, tm = block * 8 + (rest - tn * tall);
+        t.m0 = a + (int)tm * op.leaves.tall;
+        t.n0 = (int)tn * op.leaves.wide;
+        t.mend = min(b - t.m0, op.leaves.tall) + t.m0;
+        t.nend = min(op.leaves.n - t.n0, op.leaves.wide) + t.n0;
         t.k0 = t.q0 = 0;
         t.nkb = op.leaves.nkb;
         t.bz = first + l;
@@ -1070,6 +1205,33 @@ template <class T> struct LeafRows {
     __device__ int rows(const tc::Tile &, const tc::Place &) const { return 0; }
     template <class R> __device__ void epilogue(const tc::Tile &t, const tc::Place &p, int, tc::None &, uint32_t addr, R release) const { y.store(t, p, addr, release); }
 };
+
+// y = x w^T for leaves of a few rows: a warp takes 8 rows of a leaf and 16 of
+// its columns at a time.
+template <class T> struct LeafFew {
+    Leaves leaves;
+    LeafOut<T> y;
+    const T *x, *w;
+    int64_t ldx;
+    int din;
+};
+
+template <class T> __global__ void __launch_bounds__(256, kFewBlocks) k_leaf_few(const __grid_constant__ LeafFew<T> op) {
+    tc::depend();
+    const int lane = threadIdx.x % 32, warp = blockIdx.x * 8 + threadIdx.x / 32, warps = gridDim.x * 8, g = lane / 4, c = lane % 4;
+    if (op.y.rest) leaf_rest(op.leaves, op.y.out, op.y.ld, warp, warps, lane);
+    LeafIter it(op, warp, warps);
+    tc::Tile t;
+    while (it.next(op, t)) {
+        float acc[1][4];
+        dot_few<T, 1>(op.w + ((int64_t)t.bz * op.leaves.n + t.n0) * op.din, op.din, t.nend - t.n0, op.x + t.m0 * op.ldx, op.ldx, t.mend - t.m0, op.din, acc);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int row = t.m0 + 2 * c + (k & 1), col = t.n0 + g + k / 2 * 8;
+            if (row < t.mend && col < t.nend) op.y.out[(int64_t)row * op.y.ld + col] = from_f<T>(acc[0][k]);
+        }
+    }
+}
 
 // The leaves in order of their rows, longest first, for the tiles of dw.
 constexpr int kSortLeaves = 2048;
@@ -1207,6 +1369,13 @@ Err leaf_forward(const void *x, int64_t ldx, const void *w, const int32_t *off, 
     const View a = readable(prep, {x, din, t, ldx}, q.x), b = readable(prep, {w, din, dout, din, groups}, q.w);
     Err e = run_prep(prep, st);
     if (e.bad()) return e;
+    // At most 8 rows a leaf on average: bound by reading the weights.  (Row
+    // blocks of a leaf that has many more are spread over the warps too.)
+    if (t <= 8LL * groups && din % 8 == 0 && tma_rows(x, ldx) && tma_rows(w, din)) {
+        LeafFew<T> few{Leaves(off, t, groups, din, dout, 8, 16), {y, ldy, 1, zero_rest}, (const T *)x, (const T *)w, ldx, (int)din};
+        if (few.leaves.units() > INT_MAX - (1 << 20)) return {GBM_ERR_ARG, "more than 2^31 tiles"};
+        return start(k_leaf_few<T>, std::min<int64_t>((few.leaves.units() + 7) / 8, sm_count() * kFewBlocks), 256, 0, st, few);
+    }
     LeafRows<T> op{Leaves(off, t, groups, din, dout), {y, ldy, tc::store_width(y, ldy), zero_rest}};
     const View views[2] = {a, b};
     // a cluster at least for the rows outside the leaves

@@ -99,7 +99,9 @@ def _check_xent(x, w, y, c):
 
 XENT = [(1, 1, 1), (1, 8, 2), (1, 64, 1000), (2, 30, 3), (3, 100, 64), (7, 64, 65), (64, 64, 64), (65, 100, 129),
         (127, 200, 255), (128, 256, 256), (129, 72, 257), (255, 1024, 300), (256, 65, 1000), (300, 128, 5000),
-        (1000, 100, 1501), (33, 2048, 70), (513, 264, 513), (2000, 40, 2000)]
+        (1000, 100, 1501), (33, 2048, 70), (513, 264, 513), (2000, 40, 2000),
+        # few rows against many classes, features that end inside a step
+        (1, 72, 9001), (5, 1000, 20011), (8, 264, 9000), (9, 520, 30000), (16, 104, 20000), (17, 1024, 9999), (32, 8, 40001)]
 
 
 @gpu
@@ -161,6 +163,10 @@ def test_xent_rows_without_a_target(kind):
     _near(lse[keep], want[1][keep], tol[1][keep], "lse")
     _near(dx, want[2], tol[2], "dx")
     _near(dw, want[3], tol[3], "dw")
+    # with few rows too, against classes enough for many blocks
+    few, many = x[:8].contiguous(), _rand((9000, 64), t, 7, 0.25)
+    z = linear.softmax_xent(few, many, y[:8])[1]
+    assert torch.isnan(z[5]) and torch.isfinite(z[[0, 1, 2, 3, 4, 6, 7]]).all()
     # NaN in a row that counts stays in that row's loss
     y[5] = 3
     loss = linear.softmax_xent(x, w, y)[0]
@@ -254,8 +260,9 @@ def _check_leaf(x, w, off, dy, t_rows=None):
     return y, dx, dw
 
 
+# a few rows in most leaves, a block of them in one; then
 # many short leaves: one stage of rows a tile, each with its tail, many tiles a cluster
-LEAF = [([3, 1, 7, 63, 2, 65] * 40, 264, 520), ([1], 1, 1), ([1], 8, 8), ([0, 3, 0], 30, 20), ([5, 0, 64, 1], 64, 64), ([63, 65, 127, 129], 100, 61),
+LEAF = [([1, 0, 2] * 20 + [70], 1032, 40), ([0] * 9 + [40], 264, 17), ([3, 1, 7, 63, 2, 65] * 40, 264, 520), ([1], 1, 1), ([1], 8, 8), ([0, 3, 0], 30, 20), ([5, 0, 64, 1], 64, 64), ([63, 65, 127, 129], 100, 61),
         ([0, 0, 0], 16, 24), ([256, 255, 257, 1, 0, 2], 128, 256), ([700], 264, 136), ([1] * 40, 72, 300),
         ([33, 0, 500, 7], 1000, 50), ([64] * 8, 256, 512), ([3, 1000, 0, 20], 40, 520)]
 
