@@ -17,8 +17,9 @@
 // run the epilogue (warp w reads the tensor memory lanes 32 (w % 4) .. +31,
 // warps 2..5 the tile's left columns, warps 6..9 its right ones), warp 10
 // tells the products' thread of its tiles and puts zeros behind a k axis that
-// ends inside a stage.  (Few products wait in the tensor core's queue: looking for the
-// next tile, 500 clocks, 1500 among leaves, by the products' own warp idled it.)  The thread that
+// ends inside a stage.  (Few products wait in the tensor core's queue: looking
+// for the next tile, 500 clocks, 1500 among leaves, by the products' own warp
+// idled it.)  The thread that
 // fetches and the one that issues products are chosen by elect.sync: under a
 // plain test of the lane the compiler does not know that one thread runs, and
 // the loops took up to 20 % more clocks than the products.
