@@ -188,7 +188,8 @@ class LeafLinearClassifier:
         return out
 
     def predict(self, X):
-        return self.classes_[np.argmax(self.predict_proba(X), axis=1)]
+        best = np.argmax(self.predict_proba(X), axis=1)
+        return self.classes_[best]
 
     def log_loss(self, X, y):
         """Mean log-loss of the labels, without the n x classes matrix of

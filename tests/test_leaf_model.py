@@ -35,6 +35,14 @@ def test_refusals_need_no_gpu():
         m.predict_proba(np.zeros((4, 2)))
 
 
+def test_every_answer_of_an_unfitted_model_says_so(built_lib):
+    from bsscl_gbm_b200 import LeafLinearClassifier
+    X = np.zeros((3, 2))
+    for ask in (LeafLinearClassifier().predict, LeafLinearClassifier().predict_proba):
+        with pytest.raises(ValueError, match="not fitted"):
+            ask(X)
+
+
 @pytest.mark.gpu
 def test_leaf_of_rows_follows_the_tree():
     from bsscl_gbm_b200 import leaf_of_rows
