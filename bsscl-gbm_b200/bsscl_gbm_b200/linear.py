@@ -13,8 +13,9 @@ model whose leaves hold linear maps under a softmax head of many classes:
 
 Every call runs on the current stream of its tensors' device, whatever the
 current device is, waits for nothing, and may be captured into a CUDA graph.
-There is no CPU path.  Wrong types, shapes, strides and devices raise
-ValueError before anything is launched.
+There is no CPU path.  Wrong types, shapes, strides and devices, and a given
+output that overlaps what its call reads, raise ValueError before anything is
+launched.
 """
 
 from __future__ import annotations

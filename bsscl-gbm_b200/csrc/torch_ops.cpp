@@ -11,6 +11,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <initializer_list>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -69,6 +70,29 @@ struct Matrix {
     }
     bool ready() const { return in_place(p, ld); }
 };
+
+// An output that the caller gave shares no memory with what the call reads: its
+// kernels read on while they write.  Rows of one stride may lie beside one
+// another, as columns of one matrix do; other areas are taken from end to end.
+struct Area {
+    uintptr_t at, row, step;      // bytes of a row, and from row to row
+    int64_t rows;
+    Area(const Matrix &m) : at(reinterpret_cast<uintptr_t>(m.p)), row(m.cols * 2), step(m.ld * 2), rows(m.rows) {}
+    Area(const Tensor &a) : at(reinterpret_cast<uintptr_t>(a.data_ptr())), row(a.nbytes()), step(row), rows(row > 0) {}
+    Area(const void *p, int64_t bytes) : at(reinterpret_cast<uintptr_t>(p)), row(bytes), step(row), rows(bytes > 0) {}
+    uintptr_t end() const { return at + (rows - 1) * step + row; }
+    bool meets(const Area &o) const {
+        if (!rows || !o.rows || end() <= o.at || o.end() <= at) return false;
+        if (step != o.step) return true;
+        const uintptr_t off = o.at >= at ? (o.at - at) % step : (step - (at - o.at) % step) % step;
+        return off < row || off + o.row > step;
+    }
+};
+
+void apart(const Area &out, const char *name, std::initializer_list<Area> read) {
+    for (const Area &a : read)
+        if (out.meets(a)) refuse(name, " overlaps a tensor that the call reads");
+}
 
 int32_t code(const Tensor &a) { return a.scalar_type() == at::kBFloat16 ? GBM_TYPE_BF16 : GBM_TYPE_F16; }
 
@@ -186,6 +210,7 @@ PyObject *softmax_xent_grad(PyObject *, PyObject *const *args, Py_ssize_t nargs)
             dw = tensor(args[7], "dw_out");
             const Matrix m(dw, "dw_out", &h.x);
             if (m.rows != h.v || m.cols != h.d) refuse("dw_out must have shape (", h.v, ", ", h.d, "), got ", shape_of(dw));
+            apart(m, "dw_out", {h.a, h.b, {h.y, h.n * 8}, {lse, h.n * 4}, {g, h.n * 4}});
             lddw = m.ld;
         }
         Call c(h.x, h.bytes(1));
@@ -226,6 +251,7 @@ PyObject *leaf_linear(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
             y = tensor(args[3], "out");
             const Matrix m(y, "out", &l.x);
             if (m.rows != l.n || m.cols != l.dout) refuse("out must have shape (", l.n, ", ", l.dout, "), got ", shape_of(y));
+            apart(m, "out", {l.a, l.w, {l.off, (l.e + 1) * 4}});
             ldy = m.ld;
         }
         Call c(l.x, gbm_leaf_linear_workspace(l.n, (int32_t)l.e, l.din, l.dout, 0, l.a.ready() && in_place(l.w.data_ptr(), l.din)));
@@ -250,6 +276,7 @@ PyObject *leaf_linear_grad(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
             dw = tensor(args[6], "dw_out");
             if (dw.sizes() != l.w.sizes() || dw.scalar_type() != l.w.scalar_type() || dw.device() != l.w.device() || !dw.is_contiguous())
                 refuse("dw_out must be contiguous and have w's shape, type and device");
+            apart(dw, "dw_out", {l.a, l.w, g, {l.off, (l.e + 1) * 4}});
         }
         const bool ready = g.ready() && (!want_dw || l.a.ready()) && (!want_dx || in_place(l.w.data_ptr(), l.din));
         Call c(l.x, gbm_leaf_linear_workspace(l.n, (int32_t)l.e, l.din, l.dout, 1, ready));

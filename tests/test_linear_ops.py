@@ -808,3 +808,36 @@ def test_python_refusals():
     for a in ((x, lw, off, dy[:5]), (x, lw, off, dy[:, :4]), (x, lw, off, dy.half())):
         with pytest.raises(ValueError):
             linear.leaf_linear_grad(*a)
+
+
+@gpu
+def test_outputs_that_overlap_inputs():
+    """The caller's output may lie beside an operand, never on it."""
+    from bsscl_gbm_b200 import linear
+    t = torch.bfloat16
+    hold = _rand((40, 48), t, 1)
+    lw, off = _rand((2, 16, 16), t, 2), _offsets([19, 20])
+    x = hold[:, :16]
+    want = linear.leaf_linear(x, lw, off)
+    for out in (x, hold[:, 8:24], hold[:, 15:31], hold.view(-1)[:640].view(40, 16)):
+        with pytest.raises(ValueError, match="overlaps"):
+            linear.leaf_linear(x, lw, off, out=out)
+    with pytest.raises(ValueError, match="overlaps"):
+        linear.leaf_linear(hold[:, 32:], lw, off, out=hold[:, 24:40])
+    with pytest.raises(ValueError, match="overlaps"):
+        linear.leaf_linear(x[:16], lw, _offsets([9, 7]), out=lw[1])
+    before = hold[:, 32:].clone()
+    got = linear.leaf_linear(x, lw, off, out=hold[:, 16:32])
+    assert torch.equal(got[:39], want[:39]) and torch.equal(hold[:, 32:], before)
+    got = linear.leaf_linear(hold[:, 32:], lw, off, out=hold[:, 16:32])      # to the left of what it reads
+    assert torch.equal(got[:39], linear.leaf_linear(before, lw, off)[:39])
+    dy = _rand((40, 16), t, 3)
+    for dw in (lw, dy[:32].view(2, 16, 16)):
+        with pytest.raises(ValueError, match="overlaps"):
+            linear.leaf_linear_grad(x, lw, off, dy, dw_out=dw)
+    head, target = _rand((9, 16), t, 4), torch.arange(40, device="cuda") % 9
+    c = torch.ones(40, device="cuda")
+    _, lse = linear.softmax_xent(dy, head, target)
+    for dw in (head, dy[3:12], dy[31:]):
+        with pytest.raises(ValueError, match="overlaps"):
+            linear.softmax_xent_grad(dy, head, target, lse, c, dw_out=dw)
