@@ -24,9 +24,21 @@
 // plain test of the lane the compiler does not know that one thread runs, and
 // the loops took up to 20 % more clocks than the products.
 //
-// Every wait is bounded: when one runs out, the kernel notes it in
-// g_ops_timeout, all roles leave their loops, the copies in flight get time
-// to land, tensor memory is freed and the kernel returns.
+// Every wait for a barrier in shared memory is bounded: when one runs out, the
+// kernel notes it in g_ops_timeout, all roles leave their loops, the copies in
+// flight get time to land, tensor memory is freed and the kernel returns.  What
+// the hardware waits for by itself ends with that: a barrier of the cluster is
+// reached by every warp of both CTAs on every path, the launch in front
+// (griddepcontrol.wait) ends as this one does, and tcgen05.alloc finds all of
+// the pair's tensor memory free, for
+// - both CTAs run (the cluster has met) before either allocates, and neither
+//   leaves before both have freed: allocating and freeing are operations of
+//   the pair on both SMs;
+// - the launch in front, whose CTAs may have left these SMs a moment ago, is
+//   over altogether, its tensor memory freed;
+// - a CTA's shared memory keeps a second one of this frame off its SM.
+// (With the allocation before the CTAs had met, under the launch in front, a
+// training loop twice did not come back.)
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -438,16 +450,16 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         if (lane == 0) *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    cluster_sync();     // both CTAs run, their barriers stand
+    depend();
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
         fence_before();
     }
-    __syncthreads();
-    cluster_sync();
+    cluster_sync();     // both have their tensor memory
     fence_after();
     const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
-    depend();
 
     if (warp == 0) {
         // ---- fetch: one thread runs a tile's stages (a stage has 512 clocks)
@@ -478,6 +490,8 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
             if (__any_sync(~0u, *dead)) break;
             r.skip(t.nkb);
         }
+        // every product's end has reached this CTA's barriers before it leaves
+        for (int i = 0; i < kStages && mbar_wait_warp(empty + 8 * r.s, r.ph ^ 1, dead); i++) r.step();
     } else if (warp == 1) {
         // ---- products, issued by one thread too
         if (rank == 0 && elect_one()) {
@@ -582,9 +596,10 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     __syncwarp();
     if (*dead)
         for (int i = 0; i < 1000; i++) __nanosleep(1000);    // copies in flight land meanwhile
-    __syncthreads();
-    cluster_sync();
+    cluster_sync();     // nobody reads tensor memory any more
+    fence_after();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+    cluster_sync();     // both have freed theirs
 }
 
 // A wait that nothing ends, for the test of what a wait that runs out does.
