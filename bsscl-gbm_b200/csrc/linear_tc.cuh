@@ -334,7 +334,12 @@ struct Ring {
 };
 
 // What one CTA of the pair fetches of a tile: boxes of 64 values of k x 128
-// rows, or where the m (n) axis is contiguous 64 of its values x 64 of k.
+// rows, or where the m (n) axis is contiguous 64 of its values x 64 of k.  The
+// second CTA may have none of either operand (up to 128 rows and 32 columns).
+// It arrives on the leading CTA's barrier of every stage all the same: without
+// that the leading one could run a lap of the ring ahead, and the second one's
+// wait by parity would take the lap after for the one that it is in.  So no
+// stage is full before both have come to it.
 struct Boxes {
     int am, bn, a, b;      // first row of A and B, boxes of each
     __device__ static int count(bool mn, int from, int end) { return end <= from ? 0 : mn && end - from > 64 ? 2 : 1; }
@@ -382,7 +387,10 @@ __device__ __forceinline__ bool fetch(const Op &op, const CUtensorMap *maps, con
     for (int q = t.q0; q < t.q0 + n; q++) {
         if (!mbar_wait(empty + 8 * r.s, r.ph ^ 1, dead)) return false;
         const uint32_t bar = full + 8 * r.s;
-        if (rank == 0) mbar_expect(bar, bytes);
+        if (rank == 0)
+            mbar_expect(bar, bytes);
+        else
+            mbar_arrive_at<false>(bar, 0);
         load_stage<Op, AMN, true>(maps, stages + r.s * kStageBytes, bar, mine, t.k0 + (two ? q >> 1 : q) * kBK, two ? q & 1 : 0, t.bz);
         r.step();
     }
@@ -435,7 +443,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         // a lane a barrier: one lane for all took 400 clocks
         if (lane < (Op::kDual ? 4 : 2)) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.m[lane]) : "memory");
         if (lane < kStages) {
-            mbar_init(full + 8 * lane, 1);
+            mbar_init(full + 8 * lane, 2);      // both CTAs' fetching threads
             mbar_init(empty + 8 * lane, 1);
             // one a stage: a CTA ahead of the other by a whole short tile must not count for both
             mbar_init(fixed + 8 * lane, 2);
@@ -481,7 +489,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                     if (ok) {
                         const Boxes mine(t, true, Op::kBMN, (int)rank);
                         mbar_expect(tailbar + 8 * q.s, mine.bytes(true, Op::kBMN));
-                        if (rank == 0) mbar_arrive(full + 8 * q.s);
+                        mbar_arrive_at<false>(full + 8 * q.s, 0);
                         load_stage<Op, true, false>(Op::kDual ? maps.m + 2 : maps.m, stages + q.s * kStageBytes, tailbar + 8 * q.s, mine,
                                                     t.k0 + (t.q0 + n) * kBK, 0, t.bz);
                     }

@@ -2,6 +2,7 @@
 its roles wait for.  Its protocol is read from the source and run on the CPU;
 on the GPU the launches that follow one another run many times over."""
 import os
+import random
 import re
 
 import pytest
@@ -14,9 +15,13 @@ from conftest import ROOT
 gpu = pytest.mark.gpu
 
 
-def _frame():
+def _source():
     with open(os.path.join(ROOT, "bsscl-gbm_b200", "csrc", "linear_tc.cuh")) as f:
-        text = re.sub(r"//[^\n]*", "", f.read())
+        return re.sub(r"//[^\n]*", "", f.read())
+
+
+def _frame():
+    text = _source()
     return text[text.index("k_tc(const"):text.index("k_wait(")]
 
 
@@ -26,6 +31,79 @@ def test_tensor_memory_is_taken_and_freed_while_both_ctas_are_there():
     order = re.findall(r"cluster_sync\(\)|depend\(\)|tcgen05\.alloc|tcgen05\.dealloc|op\.epilogue", _frame())
     assert order == ["cluster_sync()", "depend()", "tcgen05.alloc", "cluster_sync()", "op.epilogue",
                      "cluster_sync()", "tcgen05.dealloc", "cluster_sync()"]
+
+
+class _Bar:
+    """An mbarrier: phases that end with `count` arrivals and all expected bytes."""
+
+    def __init__(self, count):
+        self.count, self.left, self.bytes, self.phase = count, count, 0, 0
+
+    def move(self, arrive=0, bytes_=0):
+        self.left -= arrive
+        self.bytes += bytes_
+        if self.left == 0 and self.bytes == 0:
+            self.left, self.phase = self.count, self.phase + 1
+
+    def passed(self, parity):
+        return self.phase % 2 != parity
+
+
+def _run_ring(count, second_arrives, boxes, laps, rng):
+    """Both CTAs' fetching threads and the products over `laps` rounds of six stages, in a random order of their steps (the
+    second CTA a slow one); boxes = what the second CTA brings of a stage.  None, or what went wrong."""
+    n = 6
+    full, empty = [_Bar(count) for _ in range(n)], [[_Bar(1) for _ in range(n)] for _ in range(2)]
+    at, total = {"first": 0, "second": 0, "products": 0}, n * laps
+    late = []                                     # bytes and arrivals on their way
+    pace = {"first": 1.0, "second": rng.choice([0.02, 0.2, 1.0]), "products": 1.0}
+    while at["second"] < total or at["products"] < total:
+        moved = False
+        for who in ("first", "second", "products"):
+            k = at[who]
+            if k == total or rng.random() > pace[who]:
+                moved |= k < total and pace[who] < 1.0
+                continue
+            s, lap = k % n, k // n
+            if who == "products":
+                if full[s].passed(lap % 2):
+                    late += [(empty[0][s], 1, 0), (empty[1][s], 1, 0)]
+                    at[who], moved = k + 1, True
+                continue
+            cta = who == "second"
+            if not empty[cta][s].passed(lap % 2 ^ 1):
+                continue
+            if empty[cta][s].phase != lap:
+                return f"the {who} CTA's wait stands for lap {empty[cta][s].phase}, not {lap}"
+            if cta:
+                full[s].move(arrive=int(second_arrives))
+                late += [(full[s], 0, -1)] * boxes
+            else:
+                full[s].move(arrive=1, bytes_=1 + boxes)
+                late += [(full[s], 0, -1)]
+            at[who], moved = k + 1, True
+        if late and rng.random() < 0.8:
+            bar, arrive, bytes_ = late.pop(0)
+            bar.move(arrive, bytes_)
+            moved = True
+        if not moved and not late:
+            return f"stuck at {at}"
+    return None
+
+
+def test_a_cta_that_fetches_nothing_is_held_in_step():
+    """The barriers of the ring as the source has them, in random orders: no wait ever stands for another lap's phase."""
+    text = _source()
+    count = int(re.search(r"mbar_init\(full \+ 8 \* lane, (\d)\)", text).group(1))
+    fetch = re.sub(r"\s+", " ", text[text.index("bool fetch("):text.index("void multiply_stage")])
+    arrives = "if (rank == 0) mbar_expect(bar, bytes); else mbar_arrive_at<false>(bar, 0);" in fetch
+    rng = random.Random(1)
+    for _ in range(300):
+        for boxes in (0, 1, 2):
+            assert _run_ring(count, arrives, boxes, 8, rng) is None
+    # the model tells: without the second CTA's arrival it is lapped where it fetches nothing
+    assert any(_run_ring(1, False, 0, 8, rng) for _ in range(300))
+    assert not any(_run_ring(1, False, 1, 8, rng) for _ in range(300))
 
 
 def _rand(shape, t, seed, scale=1.0):
@@ -68,3 +146,46 @@ def test_leaf_products_that_follow_one_another():
     linear.status()
     for a, b in zip(got + grad, (want[0],) + want):
         assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("classes,hidden", [(128, 32), (100, 32), (65, 24), (128, 8), (20, 30), (1, 1)])
+def test_tiles_of_which_the_second_cta_has_nothing(classes, hidden):
+    """At most 128 rows and 32 columns of a result, over 64 and more stages: every product of the frame."""
+    from bsscl_gbm_b200 import linear
+    t, n = torch.bfloat16, 6000                       # dw's k axis: 94 stages of rows
+    x, w = _rand((n, hidden), t, 1), _rand((classes, hidden), t, 2, 0.2)
+    y, c = torch.arange(n, device="cuda") % classes, torch.ones(n, device="cuda")
+    l = x.double() @ w.double().T
+    lse64 = torch.logsumexp(l, 1)
+    for _ in range(20):
+        loss, lse = linear.softmax_xent(x, w, y)
+        dx, dw = linear.softmax_xent_grad(x, w, y, lse, c)
+    # logits and few rows: the k axis is the features'
+    wide, rows = _rand((classes, 5000), t, 3, 0.02), _rand((hidden, 5000), t, 4)
+    for _ in range(20):
+        few = linear.softmax_xent(rows, wide, y[:hidden] * 0)[1]
+        fx, fw = linear.softmax_xent_grad(rows, wide, y[:hidden] * 0, few, c[:hidden])
+    off = torch.tensor([0, n - 100, n], dtype=torch.int32, device="cuda")
+    dy, lw = _rand((n, classes), t, 5), _rand((2, classes, hidden), t, 6, 0.2)
+    for _ in range(20):
+        ly = linear.leaf_linear(x, lw, off)
+        lx, ldw = linear.leaf_linear_grad(x, lw, off, dy)
+    linear.status()
+    u = 2.0 ** -8
+    g = torch.exp(l - lse64[:, None])
+    g[torch.arange(n, device="cuda"), y] -= 1.0
+    # norm-wise: G's rounding and the result's, and 32-bit sums.  G itself is off by the logits' and lse's errors,
+    # 2 hidden 2^-23 sum |x w| + 2^-20 < 2^-15 here, which is all there is of it with one class.
+    for got, want, size in ((dx, g @ w.double(), w.double().abs().sum(0).expand(n, -1)),
+                            (dw, g.T @ x.double(), x.double().abs().sum(0).expand(classes, -1))):
+        assert float((got.double() - want).norm()) <= 2 * u * float(want.norm()) + 2.0 ** -15 * float(size.norm())
+    for got, want in ((lse, lse64), (few, torch.logsumexp(rows.double() @ wide.double().T, 1)),
+                      (ly[:n - 100], x[:n - 100].double() @ lw[0].double().T), (lx[n - 100:], dy[n - 100:].double() @ lw[1].double()),
+                      (ldw[0], dy[:n - 100].double().T @ x[:n - 100].double()), (ldw[1], dy[n - 100:].double().T @ x[n - 100:].double())):
+        assert float((got.double() - want).norm()) <= 2 * u * float(want.norm()) + 1e-5
+    if classes > 1:
+        p = torch.softmax(rows.double() @ wide.double().T, 1)
+        p[:, 0] -= 1.0
+        for got, want in ((fx, p @ wide.double()), (fw, p.T @ rows.double())):
+            assert float((got.double() - want).norm()) <= 2 * u * float(want.norm()) + 1e-5
