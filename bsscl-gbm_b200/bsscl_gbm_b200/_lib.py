@@ -38,6 +38,7 @@ EXPORTS = (
     "gbm_round_reg_sampled", "gbm_softmax_xent", "gbm_softmax_xent_grad", "gbm_softmax_xent_workspace",
     "gbm_leaf_linear", "gbm_leaf_linear_grad", "gbm_leaf_linear_workspace", "gbm_grad_clip_plan_bytes",
     "gbm_grad_clip_plan", "gbm_grad_clip", "gbm_grad_clip_workspace", "gbm_ops_status", "gbm_test_ops_wait",
+    "gbm_test_ops_expire",
 )
 
 
@@ -187,6 +188,7 @@ def lib():
     L.gbm_grad_clip_workspace.restype = i64
     L.gbm_ops_status.argtypes = [P, C.c_char_p, i32]
     L.gbm_test_ops_wait.argtypes = [i32, P, C.c_char_p, i32]
+    L.gbm_test_ops_expire.argtypes = [i32, P, C.c_char_p, i32]
     _lib = L
     return L
 

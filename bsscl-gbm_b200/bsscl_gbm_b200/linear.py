@@ -138,7 +138,9 @@ def _dense(a):
 def status(device=None):
     """Waits for the current stream and raises RuntimeError when a bounded
     wait inside one of these operators ran out on `device` since the last
-    call, or an asynchronous error occurred."""
+    call, or an asynchronous error occurred.  After a wait that ran out the
+    products do nothing until this has told it.  There is one answer a device:
+    with several streams at work, wait for all of them and ask once."""
     err = C.create_string_buffer(256)
     with torch.cuda.device(device):
         rc = lib().gbm_ops_status(torch.cuda.current_stream().cuda_stream, err, 256)

@@ -1887,11 +1887,15 @@ int gbm_grad_clip(const void *plan_host, const void *plan_dev, double max_norm, 
     return GBM_OK;
 }
 
-int gbm_test_ops_wait(int32_t timeout_ms, void *stream, char *errbuf, int32_t errlen) {
-    if (timeout_ms < 1 || timeout_ms > 10000) return fail(errbuf, errlen, GBM_ERR_ARG, "gbm_test_ops_wait: %d ms", timeout_ms);
+int gbm_test_ops_expire(int32_t timeout_ms, void *stream, char *errbuf, int32_t errlen) {
+    if (timeout_ms < 1 || timeout_ms > 10000) return fail(errbuf, errlen, GBM_ERR_ARG, "gbm_test_ops_expire: %d ms", timeout_ms);
     Err e = start(tc::k_wait, 1, 32, 0, static_cast<cudaStream_t>(stream), timeout_ms * 2000000ll);
-    if (e.bad()) return fail(errbuf, errlen, e.code, "gbm_test_ops_wait: %s", e.what);
-    return gbm_ops_status(stream, errbuf, errlen);
+    return e.bad() ? fail(errbuf, errlen, e.code, "gbm_test_ops_expire: %s", e.what) : GBM_OK;
+}
+
+int gbm_test_ops_wait(int32_t timeout_ms, void *stream, char *errbuf, int32_t errlen) {
+    const int rc = gbm_test_ops_expire(timeout_ms, stream, errbuf, errlen);
+    return rc == GBM_OK ? gbm_ops_status(stream, errbuf, errlen) : rc;
 }
 
 int gbm_ops_status(void *stream, char *errbuf, int32_t errlen) {

@@ -26,7 +26,9 @@
 //
 // Every wait for a barrier in shared memory is bounded: when one runs out, the
 // kernel notes it in g_ops_timeout, all roles leave their loops, the copies in
-// flight get time to land, tensor memory is freed and the kernel returns.  What
+// flight get time to land, tensor memory is freed and the kernel returns; the
+// launches behind it, whose inputs it did not make, do nothing until the host
+// has asked (so that a long run of them does not wait each its own 2 s).  What
 // the hardware waits for by itself ends with that: a barrier of the cluster is
 // reached by every warp of both CTAs on every path, the launch in front
 // (griddepcontrol.wait) ends as this one does, and tcgen05.alloc finds all of
@@ -77,6 +79,10 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// A word of the cluster's CTA `rank`, at this address in its shared memory.
+__device__ __forceinline__ void store_at(uint32_t addr, uint32_t rank, int v) {
+    asm volatile("{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n st.shared::cluster.b32 [r], %2;\n}" ::"r"(addr), "r"(rank), "r"(v) : "memory");
 }
 // Arrive on the same barrier of the cluster's CTA `rank`.  DATA: with writes
 // to shared memory that the other side is to see; tensor memory has its own fences.
@@ -143,6 +149,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -458,8 +465,14 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         if (lane == 0) *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // whether a launch before this one has run out; the one directly in front may not have ended yet
+    const bool late = threadIdx.x == kThreads - 1 && *(volatile int *)&g_ops_timeout;
     cluster_sync();     // both CTAs run, their barriers stand
     depend();
+    if (late) {
+        store_at(smem_u32((const void *)dead), 0, 1);
+        store_at(smem_u32((const void *)dead), 1, 1);
+    }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -468,8 +481,10 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
     cluster_sync();     // both have their tensor memory
     fence_after();
     const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
+    const bool none = *dead;      // the same in both CTAs
 
-    if (warp == 0) {
+    if (none) {
+    } else if (warp == 0) {
         // ---- fetch: one thread runs a tile's stages (a stage has 512 clocks)
         Ring r;
         typename Op::Iter it(op, cid, ncl);
@@ -602,7 +617,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         }
     }
     __syncwarp();
-    if (*dead)
+    if (*dead && !none)
         for (int i = 0; i < 1000; i++) __nanosleep(1000);    // copies in flight land meanwhile
     cluster_sync();     // nobody reads tensor memory any more
     fence_after();

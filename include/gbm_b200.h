@@ -485,8 +485,10 @@ int64_t gbm_grad_clip_workspace(const void *plan_host);
 
 /* Waits for `stream` and tells whether a bounded wait inside one of the
  * operators ran out on the current device since the last time it was asked
- * (GBM_ERR_TIMEOUT: their outputs are not valid); also the first
- * asynchronous error (GBM_ERR_CUDA). */
+ * (GBM_ERR_TIMEOUT: outputs of the calls since then are not valid; the products
+ * launched behind such a call do nothing until this one has told); also the
+ * first asynchronous error (GBM_ERR_CUDA).  There is one answer a device: with
+ * several streams at work, wait for all of them and ask once. */
 int gbm_ops_status(void *stream, char *errbuf, int32_t errlen);
 
 /* Failure-detection self test: on the current device, the operators' bounded
@@ -494,6 +496,9 @@ int gbm_ops_status(void *stream, char *errbuf, int32_t errlen);
  * (1..10000) at 2 GHz, then gbm_ops_status: GBM_ERR_TIMEOUT when the wait ran
  * out and said so.  Nothing is left waiting. */
 int gbm_test_ops_wait(int32_t timeout_ms, void *stream, char *errbuf, int32_t errlen);
+
+/* The same wait without asking: what a caller who does not ask is left with. */
+int gbm_test_ops_expire(int32_t timeout_ms, void *stream, char *errbuf, int32_t errlen);
 
 /* Synchronise the context's stream; returns the first asynchronous error
  * (no reference counterpart). */

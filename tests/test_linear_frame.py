@@ -1,9 +1,11 @@
 """The tensor-core frame under the operators for leaf-wise linear models: what
 its roles wait for.  Its protocol is read from the source and run on the CPU;
 on the GPU the launches that follow one another run many times over."""
+import ctypes as C
 import os
 import random
 import re
+import time
 
 import pytest
 
@@ -189,3 +191,29 @@ def test_tiles_of_which_the_second_cta_has_nothing(classes, hidden):
         p[:, 0] -= 1.0
         for got, want in ((fx, p @ wide.double()), (fw, p.T @ rows.double())):
             assert float((got.double() - want).norm()) <= 2 * u * float(want.norm()) + 1e-5
+
+
+@gpu
+def test_launches_behind_a_wait_that_ran_out_do_nothing():
+    """Hundreds of calls after one that ran out: none waits for itself, none writes, and the first to ask is told once."""
+    from bsscl_gbm_b200 import lib, linear
+    t = torch.bfloat16
+    x, w = _rand((300, 64), t, 1), _rand((2, 128, 64), t, 2, 0.1)
+    off = torch.tensor([0, 100, 300], dtype=torch.int32, device="cuda")
+    want = linear.leaf_linear(x, w, off)
+    linear.status()
+    err = C.create_string_buffer(256)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib().gbm_test_ops_expire(20, stream, err, 256) == 0
+    torch.cuda.synchronize()
+    out = torch.full_like(want, 5.0)
+    began = time.monotonic()
+    for _ in range(300):
+        linear.leaf_linear(x, w, off, out=out)
+    torch.cuda.synchronize()
+    assert time.monotonic() - began < 1.0 and (out == 5).all()
+    with pytest.raises(RuntimeError, match="ran out"):
+        linear.status()
+    linear.status()
+    assert torch.equal(linear.leaf_linear(x, w, off, out=out), want)
+    assert lib().gbm_test_ops_expire(0, stream, err, 256) == 1 and b"expire" in err.value
