@@ -24,7 +24,8 @@
 // plain test of the lane the compiler does not know that one thread runs, and
 // the loops took up to 20 % more clocks than the products.
 //
-// Every wait for a barrier in shared memory is bounded: when one runs out, the
+// Every wait for a barrier in shared memory is bounded (2 s, and more where it
+// lasts for a whole k axis: wait_clocks): when one runs out, the
 // kernel notes it in g_ops_timeout, all roles leave their loops, the copies in
 // flight get time to land, tensor memory is freed and the kernel returns; the
 // launches behind it, whose inputs it did not make, do nothing until the host
@@ -57,6 +58,8 @@ constexpr int kBK = 64;                       // values of k a stage: 128 bytes
 constexpr int kABytes = 128 * kBK * 2;        // A of one CTA and stage
 constexpr int kStaging = kEpiWarps * 4096;    // 32 rows x 128 bytes a warp
 constexpr long long kWaitClocks = 4000000000ll;   // about 2 s
+// A wait that may last for whole k axes gets more: 16 times the 512 clocks of a stage's products for each stage.
+__device__ __forceinline__ long long wait_clocks(long long stages) { return kWaitClocks + stages * 8192; }
 
 static __device__ int g_ops_timeout;
 
@@ -133,8 +136,8 @@ template <bool DATA = false> __device__ __forceinline__ bool mbar_wait(uint32_t 
     }
 }
 // The same for a whole warp, whose lanes all get the same answer.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *dead) {
-    const bool ok = mbar_wait(bar, parity, dead);
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *dead, long long limit = kWaitClocks) {
+    const bool ok = mbar_wait(bar, parity, dead, limit);
     return __all_sync(~0u, ok);
 }
 // One thread of a converged warp, known as such to the compiler.
@@ -553,11 +556,12 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         uint32_t ph = 0;
         typename Op::Iter it(op, cid, ncl);
         Tile t, next{};
-        int n = 0;
+        int n = 0, longest = 0;     // stages of the longest tile so far: this warp is up to kTold tiles ahead of the products
         auto tell = [&](bool more) {
+            longest = max(longest, next.nkb);
             if (rank) return true;
             const int slot = n % kTold;
-            if (!mbar_wait_warp(heard + 8 * slot, (n / kTold & 1) ^ 1, dead)) return false;
+            if (!mbar_wait_warp(heard + 8 * slot, (n / kTold & 1) ^ 1, dead, wait_clocks(longest))) return false;
             if (lane == 0) {
                 tiles[slot] = make_int4(more ? next.nkb : -1, next.cols(), next.tail && next.nkb, next.kind);
                 mbar_arrive(told + 8 * slot);
@@ -576,7 +580,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
                 r.skip(t.nkb);
                 if (!t.tail || !t.nkb) continue;
                 const int s = r.s == 0 ? kStages - 1 : r.s - 1;
-                if (!mbar_wait_warp(tailbar + 8 * s, ph >> s & 1, dead)) break;
+                if (!mbar_wait_warp(tailbar + 8 * s, ph >> s & 1, dead, wait_clocks((kTold + 1ll) * longest))) break;
                 ph ^= 1u << s;
                 uint8_t *st = base + s * kStageBytes;
                 for (int box = 0; box < kStageBytes / 8192; box++)
@@ -605,7 +609,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         while (it.next(op, t)) {
             const int buf = n & 1;
             const auto rows = op.rows(t, p);     // the rows' scalars, on their way while the products run
-            if (!mbar_wait_warp(tfull + 8 * buf, (n >> 1) & 1, dead)) break;
+            if (!mbar_wait_warp(tfull + 8 * buf, (n >> 1) & 1, dead, wait_clocks(t.nkb))) break;
             n++;
             fence_after();
             p.wide = t.cols() / 2;

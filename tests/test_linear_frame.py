@@ -217,3 +217,17 @@ def test_launches_behind_a_wait_that_ran_out_do_nothing():
     linear.status()
     assert torch.equal(linear.leaf_linear(x, w, off, out=out), want)
     assert lib().gbm_test_ops_expire(0, stream, err, 256) == 1 and b"expire" in err.value
+
+
+@gpu
+def test_a_tile_that_takes_longer_than_the_shortest_limit():
+    """One row of 2^31 - 600 features: 33 million stages in one tile.  Ones in a few places, the last one among them: exact."""
+    from bsscl_gbm_b200 import linear
+    d = 2 ** 31 - 600
+    x, w = torch.zeros(1, d, dtype=torch.bfloat16, device="cuda"), torch.ones(1, d, dtype=torch.bfloat16, device="cuda")
+    x[0, [0, 77, 1 << 30, d - 1]] = 1.0
+    loss, lse = linear.softmax_xent(x, w, torch.zeros(1, dtype=torch.int64, device="cuda"))
+    linear.status()
+    assert float(lse) == 4.0 and float(loss) == 0.0
+    del x, w
+    torch.cuda.empty_cache()
