@@ -111,6 +111,7 @@ class LeafLinearClassifier:
         X, y = self._check(X), np.asarray(y)
         if len(y) != len(X):
             raise ValueError(f"X has {len(X)} rows but y has {len(y)}")
+        self.__dict__.pop('_w', None)      # not fitted until the operators' results are known to be valid
         self.classes_, index = np.unique(y, return_inverse=True)
         if len(self.classes_) < 2:
             raise ValueError("y holds a single class")
@@ -134,9 +135,9 @@ class LeafLinearClassifier:
         p = x.shape[1]
         # one start for all leaves: they part where their rows differ
         first = torch.randn(1, self.n_hidden, p, generator=g, device=dev) * p ** -0.5
-        self._w = first.expand(self.n_leaves_, -1, -1).contiguous()
-        self._head = torch.randn(K, self.n_hidden, generator=g, device=dev) * 0.1 * self.n_hidden ** -0.5
-        w, head = self._w.to(dt), self._head.to(dt)
+        w32 = first.expand(self.n_leaves_, -1, -1).contiguous()
+        head32 = torch.randn(K, self.n_hidden, generator=g, device=dev) * 0.1 * self.n_hidden ** -0.5
+        w, head = w32.to(dt), head32.to(dt)
         dw, dhead = torch.empty_like(w), torch.empty_like(head)
         clip = linear.GradClip([dw, dhead])
         self.loss_history_ = []
@@ -152,16 +153,19 @@ class LeafLinearClassifier:
                 dh, _ = linear.softmax_xent_grad(h, head, yb, lse, c / c.sum(), dw_out=dhead)
                 linear.leaf_linear_grad(xb, w, offsets, dh, want_dx=False, dw_out=dw)
                 clip.clip(self.max_norm)
-                for master, copy, grad in ((self._w, w, dw), (self._head, head, dhead)):
+                for master, copy, grad in ((w32, w, dw), (head32, head, dhead)):
                     master.add_(grad.float(), alpha=-self.learning_rate)
                     copy.copy_(master)
                 total += loss.sum(dtype=torch.float64)
+            linear.status(dev)
             self.loss_history_.append(float(total) / len(x))
+        self._w, self._head = w32, head32
         return self
 
     # -- answers ------------------------------------------------------------
     def _hidden(self, X):
-        """Blocks of (rows of X, their hidden rows)."""
+        """Blocks of (rows of X, their hidden rows).  Raises at the end when a
+        wait of the operators that the blocks went through ran out."""
         import torch
 
         from . import linear
@@ -177,6 +181,7 @@ class LeafLinearClassifier:
             leaf = torch.from_numpy(route[at:at + (1 << 16)].astype(np.int64)).to(x.device)
             rows, offsets = self._by_leaf(torch.arange(len(x), device=x.device), leaf)
             yield at + rows, linear.leaf_linear(x[rows], w, offsets)
+        linear.status(self._device())
 
     def predict_proba(self, X):
         """Class probabilities [n, classes] (float64)."""
