@@ -111,11 +111,11 @@ class LeafLinearClassifier:
         X, y = self._check(X), np.asarray(y)
         if len(y) != len(X):
             raise ValueError(f"X has {len(X)} rows but y has {len(y)}")
-        self.__dict__.pop('_w', None)      # not fitted until the operators' results are known to be valid
-        self.classes_, index = np.unique(y, return_inverse=True)
-        if len(self.classes_) < 2:
+        classes, index = np.unique(y, return_inverse=True)
+        if len(classes) < 2:
             raise ValueError("y holds a single class")
-        self.n_features_in_, K = X.shape[1], len(self.classes_)
+        self.__dict__.pop('_w', None)      # not fitted until the operators' results are known to be valid
+        self.classes_, self.n_features_in_, K = classes, X.shape[1], len(classes)
         finite = np.where(np.isfinite(X), X, np.nan).astype(np.float64)
         seen = np.isfinite(finite).sum(0) > 0
         self._mean, self._std = np.zeros(X.shape[1]), np.ones(X.shape[1])

@@ -92,3 +92,14 @@ def test_answers_ask_whether_a_wait_ran_out(on_cpu):
     assert not on_cpu
     with pytest.raises(ValueError, match="not fitted"):      # neither the weights of that fit nor the last one's
         m.predict(X)
+
+
+def test_a_refused_fit_leaves_the_model_as_it_was(on_cpu):
+    from bsscl_gbm_b200 import LeafLinearClassifier
+    X, y = _data()
+    m = LeafLinearClassifier(n_hidden=4, n_epochs=1, batch_size=128).fit(X, y)
+    P, best = m.predict_proba(X), m.predict(X)
+    for bad in ((X, np.zeros(len(X))), (X, y[:-1]), (X[0], y)):
+        with pytest.raises(ValueError):
+            m.fit(*bad)
+        assert np.array_equal(m.predict_proba(X), P) and np.array_equal(m.predict(X), best)
