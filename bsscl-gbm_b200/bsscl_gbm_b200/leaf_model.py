@@ -10,6 +10,8 @@ device operators of :mod:`bsscl_gbm_b200.linear`.
 
 from __future__ import annotations
 
+import math
+
 import numpy as np
 
 from .estimator import _device_index
@@ -53,8 +55,9 @@ class LeafLinearClassifier:
     regression) whose tree ``tree`` routes the rows; None = one leaf.  Trained
     by stochastic gradient descent on the class-weighted log-loss
     (class_weight as the estimator's), the gradients clipped to ``max_norm``.
-    Weights are kept in float32 and multiplied in ``dtype``.  Features are
-    standardised; a missing or infinite value counts as the mean.
+    Weights are kept in float32 and multiplied in ``dtype``; in float16 each
+    step's loss is scaled so that the gradients fill the type's range.  Features
+    are standardised; a missing or infinite value counts as the mean.
     """
 
     def __init__(self, router=None, tree=0, n_hidden=64, learning_rate=0.5, max_norm=1.0, n_epochs=10, batch_size=8192,
@@ -104,6 +107,18 @@ class LeafLinearClassifier:
         return X
 
     # -- training -----------------------------------------------------------
+    @staticmethod
+    def _loss_scale(h, head, x_top):
+        """The power of two that takes a float16 step's gradients to at most
+        2^15, on the device.  A row's share of the loss is about 1 / rows, so
+        that its dh would lie among the type's subnormals or below.  With the
+        rows' weights c summing to 1 and sum_v |G_iv| <= 2 c_i:
+        |dhead| <= max |h|, |dh| and |dw| <= 2 max |head| max |x| (x has a
+        column of ones)."""
+        import torch
+        top = torch.maximum(h.abs().amax().float(), 2.0 * head.abs().amax().float() * x_top)
+        return torch.exp2(torch.floor(15.0 - torch.log2(top.clamp(min=2.0 ** -14))))
+
     def fit(self, X, y):
         import torch
 
@@ -141,6 +156,8 @@ class LeafLinearClassifier:
         dw, dhead = torch.empty_like(w), torch.empty_like(head)
         clip = linear.GradClip([dw, dhead])
         self.loss_history_ = []
+        half = dt == torch.float16
+        x_top = x.abs().amax().float() if half else None
         for _ in range(self.n_epochs):
             total = torch.zeros((), dtype=torch.float64, device=dev)
             shuffled = torch.randperm(len(x), generator=g, device=dev)
@@ -148,13 +165,19 @@ class LeafLinearClassifier:
                 rows, offsets = self._by_leaf(shuffled[at:at + self.batch_size], leaf)
                 xb, yb = x[rows], target[rows]
                 c = weight[yb]
+                c = c / c.sum()
                 h = linear.leaf_linear(xb, w, offsets)
                 loss, lse = linear.softmax_xent(h, head, yb)
-                dh, _ = linear.softmax_xent_grad(h, head, yb, lse, c / c.sum(), dw_out=dhead)
+                if half:
+                    scale = self._loss_scale(h, head, x_top)
+                    c = c * scale
+                dh, _ = linear.softmax_xent_grad(h, head, yb, lse, c, dw_out=dhead)
                 linear.leaf_linear_grad(xb, w, offsets, dh, want_dx=False, dw_out=dw)
-                clip.clip(self.max_norm)
+                # scaled gradients are clipped where they are scaled back, in float32
+                norm = clip.clip(math.inf if half else self.max_norm)
+                step = torch.clamp(self.max_norm / (norm / scale + 1e-6), max=1.0) / scale if half else None
                 for master, copy, grad in ((w32, w, dw), (head32, head, dhead)):
-                    master.add_(grad.float(), alpha=-self.learning_rate)
+                    master.add_(grad.float() * step if half else grad.float(), alpha=-self.learning_rate)
                     copy.copy_(master)
                 total += loss.sum(dtype=torch.float64)
             linear.status(dev)

@@ -103,3 +103,56 @@ def test_a_refused_fit_leaves_the_model_as_it_was(on_cpu):
         with pytest.raises(ValueError):
             m.fit(*bad)
         assert np.array_equal(m.predict_proba(X), P) and np.array_equal(m.predict(X), best)
+
+
+def _check_step(n, classes, n_hidden, seed, max_norm, few_of_a_class=None):
+    """One full-batch float16 step moves the weights by -lr times the 64-bit gradient, clipped.  Features, weights and
+    hidden rows are rounded once (the first two in the formula too), dh and the gradients once more: 2^-11 of a value each,
+    and of the logits, whose shift is under 2^-11 |h| |head| < 2^-9.  Under 1 % norm-wise in all, for the leaf maps alone and
+    for the head alone."""
+    from bsscl_gbm_b200 import LeafLinearClassifier
+    X, y = _data(n, 5, classes, seed)
+    if few_of_a_class:
+        y[classes * few_of_a_class:] = 0
+        y[:classes * few_of_a_class] = np.arange(classes * few_of_a_class) % classes
+    kw = dict(n_hidden=n_hidden, n_epochs=1, batch_size=n, max_norm=max_norm, random_state=1, dtype="float16", class_weight="balanced")
+    start = LeafLinearClassifier(learning_rate=0.0, **kw).fit(X, y)
+    done = LeafLinearClassifier(learning_rate=1.0, **kw).fit(X, y)
+    dev = start._device()
+    x, index = start._features(X).double(), torch.from_numpy(np.searchsorted(start.classes_, y)).to(dev)
+    w, head = (a.to(torch.float16).double().requires_grad_() for a in (start._w, start._head))
+    c = n / (classes * torch.bincount(index, minlength=classes).double())
+    loss = torch.nn.functional.cross_entropy(x @ w[0].T @ head.T, index, reduction="none")
+    (loss * c[index] / c[index].sum()).sum().backward()
+    norm = float((w.grad.square().sum() + head.grad.square().sum()).sqrt())
+    clipped = min(1.0, max_norm / (norm + 1e-6))
+    for a, b, g in ((start._w, done._w, w.grad), (start._head, done._head, head.grad)):
+        moved = (a - b).double()
+        assert float((moved - clipped * g).norm() / (clipped * g).norm()) < 0.01
+    return norm
+
+
+STEPS = [(262_144, 30, 8, None), (65_536, 90, 64, None), (8192, 90, 64, 1), (300, 7, 16, None)]
+
+
+@pytest.mark.parametrize("n,classes,n_hidden,few", STEPS)
+def test_half_precision_step(on_cpu, n, classes, n_hidden, few):
+    """Many rows a step, and rows of a class that is 99 % of the table: dh of float16 without a scale was 0 for most."""
+    norm = _check_step(n, classes, n_hidden, 2, 1e9, few)
+    _check_step(n, classes, n_hidden, 2, norm / 3, few)
+
+
+@pytest.mark.parametrize("h,head,x_top", [(4.0, 0.05, 6.0), (300.0, 2.0, 50.0), (0.0, 0.0, 1.0), (60000.0, 3.0, 1e4), (1.0, 1e-7, 1.0)])
+def test_half_precision_scale_is_a_power_of_two_within_range(h, head, x_top):
+    from bsscl_gbm_b200 import LeafLinearClassifier
+    scale = float(LeafLinearClassifier._loss_scale(torch.tensor([[h, -h / 2]]), torch.tensor([[head / 3, -head]]), torch.tensor(x_top)))
+    most = max(h, 2 * head * x_top)
+    assert scale > 0 and np.log2(scale) == int(np.log2(scale)) and scale * most <= 2.0 ** 15
+    assert most < 2.0 ** -13 or scale * most > 2.0 ** 13
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,classes,n_hidden,few", STEPS)
+def test_half_precision_step_on_the_device(n, classes, n_hidden, few):
+    norm = _check_step(n, classes, n_hidden, 2, 1e9, few)
+    _check_step(n, classes, n_hidden, 2, norm / 3, few)
