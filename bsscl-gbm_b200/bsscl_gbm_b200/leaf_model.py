@@ -186,9 +186,10 @@ class LeafLinearClassifier:
         return self
 
     # -- answers ------------------------------------------------------------
-    def _hidden(self, X):
-        """Blocks of (rows of X, their hidden rows).  Raises at the end when a
-        wait of the operators that the blocks went through ran out."""
+    def _hidden(self, X, rows=1 << 16):
+        """Blocks of (rows of X, their hidden rows), `rows` at a time.  Raises
+        at the end when a wait of the operators that the blocks went through
+        ran out."""
         import torch
 
         from . import linear
@@ -199,24 +200,33 @@ class LeafLinearClassifier:
             raise ValueError(f"X has {X.shape[1]} features; the model has {self.n_features_in_}")
         route, _ = self._routes(X)
         w = self._w.to(getattr(torch, self.dtype))
-        for at in range(0, len(X), 1 << 16):
-            x = self._features(X[at:at + (1 << 16)])
-            leaf = torch.from_numpy(route[at:at + (1 << 16)].astype(np.int64)).to(x.device)
-            rows, offsets = self._by_leaf(torch.arange(len(x), device=x.device), leaf)
-            yield at + rows, linear.leaf_linear(x[rows], w, offsets)
+        for at in range(0, len(X), rows):
+            x = self._features(X[at:at + rows])
+            leaf = torch.from_numpy(route[at:at + rows].astype(np.int64)).to(x.device)
+            order, offsets = self._by_leaf(torch.arange(len(x), device=x.device), leaf)
+            yield at + order, linear.leaf_linear(x[order], w, offsets)
         linear.status(self._device())
+
+    def _probabilities(self, X):
+        """Blocks of (rows of X, their probabilities in float64 on the device),
+        of at most 2^26 values."""
+        import torch
+        classes = len(self.classes_) if hasattr(self, 'classes_') else 1
+        for rows, h in self._hidden(X, max(1, min(1 << 16, (1 << 26) // classes))):
+            yield rows, torch.softmax(h.double() @ self._head.to(h.dtype).double().T, 1)
 
     def predict_proba(self, X):
         """Class probabilities [n, classes] (float64)."""
-        import torch
         out = np.empty((len(X), len(self.classes_) if hasattr(self, 'classes_') else 0))
-        for rows, h in self._hidden(X):
-            head = self._head.to(h.dtype).double()
-            out[rows.cpu().numpy()] = torch.softmax(h.double() @ head.T, 1).cpu().numpy()
+        for rows, p in self._probabilities(X):
+            out[rows.cpu().numpy()] = p.cpu().numpy()
         return out
 
     def predict(self, X):
-        best = np.argmax(self.predict_proba(X), axis=1)
+        """The most probable class of each row, without the n x classes matrix."""
+        best = np.empty(len(X), np.int64)
+        for rows, p in self._probabilities(X):
+            best[rows.cpu().numpy()] = p.argmax(1).cpu().numpy()
         return self.classes_[best]
 
     def log_loss(self, X, y):

@@ -151,6 +151,42 @@ def test_half_precision_scale_is_a_power_of_two_within_range(h, head, x_top):
     assert most < 2.0 ** -13 or scale * most > 2.0 ** 13
 
 
+def test_answers_take_classes_in_blocks(on_cpu, monkeypatch):
+    """200,000 classes: probabilities of at most 2^26 values at a time, and none of the n x classes matrix for predict."""
+    from bsscl_gbm_b200 import LeafLinearClassifier
+    X, y = _data(900)
+    m = LeafLinearClassifier(n_hidden=4, n_epochs=1, batch_size=900).fit(X, y)
+    small = m.predict_proba(X)
+    assert np.array_equal(m.predict(X), m.classes_[small.argmax(1)])
+    m.classes_, m._head = np.arange(200_000) * 2, torch.randn(200_000, 4, generator=torch.Generator().manual_seed(0))
+    softmax, sizes = torch.softmax, []
+
+    def seen(a, dim):
+        sizes.append(a.numel())
+        return softmax(a, dim)
+
+    monkeypatch.setattr(torch, "softmax", seen)
+    monkeypatch.setattr(LeafLinearClassifier, "predict_proba", None)
+    best = m.predict(X)
+    assert len(sizes) > 1 and max(sizes) <= 1 << 26 and sum(sizes) == 900 * 200_000
+    h = torch.cat([h[torch.argsort(rows)] for rows, h in m._hidden(X)]).double()
+    at = (h @ m._head.to(torch.bfloat16).double().T).argmax(1).numpy()
+    assert np.array_equal(best, m.classes_[at])
+
+
+@pytest.mark.gpu
+def test_predict_of_many_classes_keeps_its_memory():
+    from bsscl_gbm_b200 import LeafLinearClassifier
+    X, y = _data(20_000, 5, 15_000)
+    m = LeafLinearClassifier(n_hidden=16, n_epochs=1).fit(X, y)
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    best = m.predict(X)
+    assert torch.cuda.max_memory_allocated() - before < 3 * 8 * 2 ** 26       # a block's logits and probabilities, and the head
+    assert np.array_equal(best[:700], m.classes_[m.predict_proba(X[:700]).argmax(1)])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,classes,n_hidden,few", STEPS)
 def test_half_precision_step_on_the_device(n, classes, n_hidden, few):
