@@ -11,10 +11,11 @@ device operators of :mod:`bsscl_gbm_b200.linear`.
 from __future__ import annotations
 
 import math
+import os
 
 import numpy as np
 
-from .estimator import _device_index
+from .estimator import _device_index, _dist
 
 
 def leaf_of_rows(model, X, tree=0, class_index=0):
@@ -76,7 +77,10 @@ class LeafLinearClassifier:
     # -- data ---------------------------------------------------------------
     def _device(self):
         import torch
-        return torch.device("cuda", _device_index(self.device) or 0)
+        index = _device_index(self.device)
+        if index is None:      # the GPU that the routing estimator takes
+            index = int(os.environ.get("LOCAL_RANK", 0)) if _dist() is not None else 0
+        return torch.device("cuda", index)
 
     def _routes(self, X):
         if self.router is None:

@@ -151,6 +151,16 @@ def test_half_precision_scale_is_a_power_of_two_within_range(h, head, x_top):
     assert most < 2.0 ** -13 or scale * most > 2.0 ** 13
 
 
+def test_each_rank_takes_its_own_gpu(monkeypatch):
+    """As the routing estimator does: LOCAL_RANK's in a process group, the first one elsewhere, a named one always."""
+    from bsscl_gbm_b200 import LeafLinearClassifier, leaf_model
+    monkeypatch.setenv("LOCAL_RANK", "3")
+    assert LeafLinearClassifier()._device() == torch.device("cuda", 0)
+    monkeypatch.setattr(leaf_model, "_dist", lambda: object())
+    assert LeafLinearClassifier()._device() == torch.device("cuda", 3)
+    assert LeafLinearClassifier(device="cuda:1")._device() == torch.device("cuda", 1)
+
+
 def test_answers_take_classes_in_blocks(on_cpu, monkeypatch):
     """200,000 classes: probabilities of at most 2^26 values at a time, and none of the n x classes matrix for predict."""
     from bsscl_gbm_b200 import LeafLinearClassifier
