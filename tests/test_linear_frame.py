@@ -5,6 +5,7 @@ import ctypes as C
 import os
 import random
 import re
+import subprocess
 import time
 
 import pytest
@@ -106,6 +107,19 @@ def test_a_cta_that_fetches_nothing_is_held_in_step():
     # the model tells: without the second CTA's arrival it is lapped where it fetches nothing
     assert any(_run_ring(1, False, 0, 8, rng) for _ in range(300))
     assert not any(_run_ring(1, False, 1, 8, rng) for _ in range(300))
+
+
+def test_build_needs_no_torch_with_cuda(tmp_path):
+    """The engine's library is built beside a torch that has no CUDA, without the torch binding."""
+    csrc = os.path.join(ROOT, "bsscl-gbm_b200", "csrc")
+
+    def plan():
+        return subprocess.run(["make", "-n", "-B", "-C", csrc, f"TORCH={tmp_path}"], check=True, capture_output=True, text=True).stdout
+
+    (tmp_path / "lib").mkdir()
+    assert "libgbm_b200.so" in plan() and "torch_ops.cpp" not in plan()
+    (tmp_path / "lib" / "libc10_cuda.so").touch()
+    assert "torch_ops.cpp" in plan()
 
 
 def _rand(shape, t, seed, scale=1.0):
