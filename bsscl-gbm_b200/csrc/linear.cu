@@ -1651,10 +1651,12 @@ template <class F> void clip_items(const int64_t *sizes, int32_t n, F item) {
         }
 }
 
-int finish(const char *what, char *errbuf, int32_t errlen) {
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fail(errbuf, errlen, GBM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    return GBM_OK;
+// A call's answer: each launch has told its own error.  (The thread's last
+// error may be that of an earlier call, which has told it.)
+int finish(const char *what, const Err &e, char *errbuf, int32_t errlen) {
+    if (!e.bad()) return GBM_OK;
+    cudaGetLastError();
+    return fail(errbuf, errlen, e.code, "%s: %s", what, e.what);
 }
 
 int type_size(int32_t t) { return t == GBM_TYPE_F32 ? 4 : t == GBM_TYPE_BF16 || t == GBM_TYPE_F16 ? 2 : 0; }
@@ -1698,8 +1700,7 @@ int gbm_softmax_xent(const void *x, int64_t ldx, const void *w, int64_t ldw, int
         return fail(errbuf, errlen, GBM_ERR_ARG, "gbm_softmax_xent: loss or lse is null or not aligned");
     if (!n) return GBM_OK;
     Err e = xent_forward(x, ldx, w, ldw, dtype == GBM_TYPE_BF16, n, d, v, target, loss, lse, ws, static_cast<cudaStream_t>(stream));
-    if (e.bad()) return fail(errbuf, errlen, e.code, "gbm_softmax_xent: %s", e.what);
-    return finish("gbm_softmax_xent", errbuf, errlen);
+    return finish("gbm_softmax_xent", e, errbuf, errlen);
 }
 
 int gbm_softmax_xent_grad(const void *x, int64_t ldx, const void *w, int64_t ldw, int32_t dtype, int64_t n, int64_t d,
@@ -1716,14 +1717,13 @@ int gbm_softmax_xent_grad(const void *x, int64_t ldx, const void *w, int64_t ldw
         return fail(errbuf, errlen, GBM_ERR_ARG, "%s: row stride of an output below its row", what);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (!n) {
-        if (dw && cudaMemset2DAsync(dw, lddw * 2, 0, d * 2, v, st) != cudaSuccess) return finish(what, errbuf, errlen);
-        return GBM_OK;
+        const bool ok = !dw || cudaMemset2DAsync(dw, lddw * 2, 0, d * 2, v, st) == cudaSuccess;
+        return finish(what, ok ? Err{} : Err{GBM_ERR_CUDA, "cudaMemset2DAsync"}, errbuf, errlen);
     }
     Err e = dtype == GBM_TYPE_BF16
                 ? xent_backward(x, ldx, w, ldw, n, d, v, target, lse, grad_loss, (__nv_bfloat16 *)dx, lddx, (__nv_bfloat16 *)dw, lddw, ws, st)
                 : xent_backward(x, ldx, w, ldw, n, d, v, target, lse, grad_loss, (__half *)dx, lddx, (__half *)dw, lddw, ws, st);
-    if (e.bad()) return fail(errbuf, errlen, e.code, "%s: %s", what, e.what);
-    return finish(what, errbuf, errlen);
+    return finish(what, e, errbuf, errlen);
 }
 
 static bool leaf_ok(int64_t t, int32_t groups, int64_t din, int64_t dout) {
@@ -1764,8 +1764,7 @@ int gbm_leaf_linear(const void *x, int64_t ldx, const void *w, const int32_t *of
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Err e = dtype == GBM_TYPE_BF16 ? leaf_forward(x, ldx, w, offsets, t, groups, din, dout, (__nv_bfloat16 *)y, ldy, zero_rest != 0, ws, st)
                                    : leaf_forward(x, ldx, w, offsets, t, groups, din, dout, (__half *)y, ldy, zero_rest != 0, ws, st);
-    if (e.bad()) return fail(errbuf, errlen, e.code, "%s: %s", what, e.what);
-    return finish(what, errbuf, errlen);
+    return finish(what, e, errbuf, errlen);
 }
 
 int gbm_leaf_linear_grad(const void *x, int64_t ldx, const void *w, const int32_t *offsets, const void *dy,
@@ -1786,8 +1785,7 @@ int gbm_leaf_linear_grad(const void *x, int64_t ldx, const void *w, const int32_
     Err e = dtype == GBM_TYPE_BF16 ? leaf_backward(x, ldx, w, offsets, dy, lddy, t, groups, din, dout, (__nv_bfloat16 *)dx, lddx, zero_rest != 0,
                                                    (__nv_bfloat16 *)dw, ws, st)
                                    : leaf_backward(x, ldx, w, offsets, dy, lddy, t, groups, din, dout, (__half *)dx, lddx, zero_rest != 0, (__half *)dw, ws, st);
-    if (e.bad()) return fail(errbuf, errlen, e.code, "%s: %s", what, e.what);
-    return finish(what, errbuf, errlen);
+    return finish(what, e, errbuf, errlen);
 }
 
 int64_t gbm_grad_clip_plan_bytes(const int64_t *sizes, int32_t n) {
@@ -1883,14 +1881,13 @@ int gbm_grad_clip(const void *plan_host, const void *plan_dev, double max_norm, 
     const int blocks = std::max(1, std::min(shares, sm_count() * kClipBlocks));
     void *args[] = {&plan, &max_norm, &norm, &part};
     cudaError_t e = cudaLaunchCooperativeKernel((const void *)k_clip, dim3((unsigned)blocks), dim3(256), args, 0, static_cast<cudaStream_t>(stream));
-    if (e != cudaSuccess) return fail(errbuf, errlen, GBM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    return GBM_OK;
+    return finish(what, e == cudaSuccess ? Err{} : Err{GBM_ERR_CUDA, cudaGetErrorString(e)}, errbuf, errlen);
 }
 
 int gbm_test_ops_expire(int32_t timeout_ms, void *stream, char *errbuf, int32_t errlen) {
     if (timeout_ms < 1 || timeout_ms > 10000) return fail(errbuf, errlen, GBM_ERR_ARG, "gbm_test_ops_expire: %d ms", timeout_ms);
     Err e = start(tc::k_wait, 1, 32, 0, static_cast<cudaStream_t>(stream), timeout_ms * 2000000ll);
-    return e.bad() ? fail(errbuf, errlen, e.code, "gbm_test_ops_expire: %s", e.what) : GBM_OK;
+    return finish("gbm_test_ops_expire", e, errbuf, errlen);
 }
 
 int gbm_test_ops_wait(int32_t timeout_ms, void *stream, char *errbuf, int32_t errlen) {

@@ -245,3 +245,24 @@ def test_a_tile_that_takes_longer_than_the_shortest_limit():
     assert float(lse) == 4.0 and float(loss) == 0.0
     del x, w
     torch.cuda.empty_cache()
+
+
+@gpu
+def test_another_calls_error_is_not_the_operators():
+    """An engine call that found too little memory has told so; the operators behind it succeed."""
+    from bsscl_gbm_b200 import Engine, lib, linear
+    x, w = _rand((40, 64), torch.bfloat16, 1), _rand((30, 64), torch.bfloat16, 2)
+    y = torch.zeros(40, dtype=torch.int64, device="cuda")
+    want = linear.softmax_xent(x, w, y)
+    eng = Engine(0)
+    try:
+        one = C.create_string_buffer(64)
+        assert lib().gbm_predict_upload(eng._h, one, 1 << 40, 1000) == 2         # 2^50 bytes: nothing is read
+        assert "cudaMalloc" in eng.last_error()
+        got = linear.softmax_xent(x, w, y)
+        dx, dw = linear.softmax_xent_grad(x, w, y, got[1], torch.ones(40, device="cuda"))
+        assert lib().gbm_predict_upload(eng._h, one, 1 << 40, 1000) == 2
+        linear.leaf_linear(x, w[None], torch.tensor([0, 40], dtype=torch.int32, device="cuda"))
+    finally:
+        eng.close()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
