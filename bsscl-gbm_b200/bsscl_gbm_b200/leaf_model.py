@@ -224,6 +224,7 @@ class LeafLinearClassifier:
         out = np.empty((len(X), len(self.classes_) if hasattr(self, 'classes_') else 0))
         for rows, p in self._probabilities(X):
             out[rows.cpu().numpy()] = p.cpu().numpy()
+            del p      # before the next block is computed
         return out
 
     def predict(self, X):
@@ -231,6 +232,7 @@ class LeafLinearClassifier:
         best = np.empty(len(X), np.int64)
         for rows, p in self._probabilities(X):
             best[rows.cpu().numpy()] = p.argmax(1).cpu().numpy()
+            del p
         return self.classes_[best]
 
     def log_loss(self, X, y):
