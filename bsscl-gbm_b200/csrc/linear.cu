@@ -389,18 +389,20 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// A row's loss and lse from its sum of exponentials and its target's logit.
-__device__ __forceinline__ void xent_row(float2 a, float ly, int64_t y, int64_t v, float &loss, float &lse) {
-    const float z = a.x == -INFINITY ? logf(a.y) : a.x + logf(a.y);
-    lse = z;
-    loss = y >= 0 && y < v ? z - ly : 0.f;
+// (m, s) stands for the sum s exp(m) of exponentials, and s alone where m is
+// infinite: with no finite m yet s stays 0 (or NaN, if a NaN is among them), a
+// logit of +inf makes it +inf.
+__device__ __forceinline__ float shift_of(float m) { return fabsf(m) == INFINITY ? 0.f : m; }
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x), shift = shift_of(m);
+    return make_float2(m, a.y * ex2((a.x - shift) * kLog2e) + b.y * ex2((b.x - shift) * kLog2e));
 }
 
-// (m, s) stands for the sum s exp(m) of exponentials.  With no finite m yet
-// the shift is 0, so that s stays 0 (or NaN, if a NaN is among them).
-__device__ __forceinline__ float2 join(float2 a, float2 b) {
-    const float m = fmaxf(a.x, b.x), shift = m == -INFINITY ? 0.f : m;
-    return make_float2(m, a.y * ex2((a.x - shift) * kLog2e) + b.y * ex2((b.x - shift) * kLog2e));
+// A row's loss and lse from its sum of exponentials and its target's logit.
+__device__ __forceinline__ void xent_row(float2 a, float ly, int64_t y, int64_t v, float &loss, float &lse) {
+    const float z = shift_of(a.x) + logf(a.y);
+    lse = z;
+    loss = y >= 0 && y < v ? z - ly : 0.f;
 }
 
 // x w^T, of which each tile leaves the maximum and the sum of exponentials of
@@ -472,7 +474,7 @@ struct XentStats {
 #pragma unroll
             for (int i = 0; i < 28; i += 2) top[i / 2 % 4] = tc::max3(top[i / 2 % 4], v[i], v[i + 1]);
             const float mc = fmaxf(tc::max3(top[0], top[1], top[2]), fmaxf(top[3], v[28]));
-            const float shift = mc == -INFINITY ? 0.f : mc, zs = shift * kLog2e;
+            const float shift = shift_of(mc), zs = shift * kLog2e;
             const tc::F2 minus = tc::f2(-zs, -zs);
             tc::F2 e[4] = {tc::f2(s * ex2((m - shift) * kLog2e), 0.f), tc::f2(0.f, 0.f), tc::f2(0.f, 0.f), tc::f2(0.f, 0.f)};
 #pragma unroll

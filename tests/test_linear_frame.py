@@ -266,3 +266,38 @@ def test_another_calls_error_is_not_the_operators():
     finally:
         eng.close()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,d,v", [(8, 64, 9000), (13, 72, 20_000), (70, 64, 300), (300, 100, 5000), (2000, 64, 16_000)])
+def test_infinite_logits(n, d, v, kind):
+    """log sum exp of a row with a logit of +inf is +inf, of -inf beside finite ones finite; its loss follows, and its neighbours
+    are as they are without it."""
+    from bsscl_gbm_b200 import linear
+    x, w = _rand((n, d), kind, 1), _rand((v, d), kind, 2, 0.1)
+    w[:, 0] = 0.0
+    y = torch.arange(n, device="cuda") % v
+    want, lse = linear.softmax_xent(x, w, y)
+    x[3], x[5] = 0.0, 0.0
+    x[3, 0], x[5, 0] = float("inf"), 1.0
+    w[:, 0], w[v // 2, 0] = -1.0, 1.0            # one class of +inf in row 3
+    x[:3, 0], x[4, 0], x[6:, 0] = 0.0, 0.0, 0.0
+    y[3] = 7
+    loss, got = linear.softmax_xent(x, w, y)
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[[3, 5]] = False
+    assert torch.equal(loss[keep], want[keep]) and torch.equal(got[keep], lse[keep])
+    assert float(got[3]) == float("inf") and float(loss[3]) == float("inf")
+    e = (v - 1) * 2.718281828459045 ** -1 + 2.718281828459045
+    assert abs(float(got[5]) - float(torch.log(torch.tensor(e, dtype=torch.float64)))) < 1e-5
+    y[3] = v // 2                                # inf - inf
+    loss, got = linear.softmax_xent(x, w, y)
+    assert torch.isnan(loss[3]) and float(got[3]) == float("inf")
+    w[:, 0] = -1.0                               # every logit -inf
+    assert float(linear.softmax_xent(x, w, y)[1][3]) == float("-inf")
+    w[::2, 0] = 1.0                              # half of them +inf
+    assert float(linear.softmax_xent(x, w, y)[1][3]) == float("inf")
+    w[1] = float("nan")                          # and a NaN among them
+    assert torch.isnan(linear.softmax_xent(x, w, y)[1]).all()
+    linear.status()
