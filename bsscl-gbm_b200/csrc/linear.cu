@@ -185,13 +185,14 @@ __device__ __forceinline__ void pack_chunk(const PackJob &j, int64_t r, int64_t 
     *(uint4 *)(j.dst + r * j.ldp + c) = q;
 }
 
-// The power of two that takes m to at most 2^14.
-__device__ __forceinline__ int scale_exponent(float m) { return m > 0.f && m < INFINITY ? min(max(14 - (ilogbf(m) + 1), -100), 100) : 0; }
+// The power of two that takes m to 2^14 .. 2^15: |G| <= |c| (1 + the error of
+// p) stays within half precision's 65504, and what its subnormals round away is
+// at most 2^-25 / 2^14 = 2^-39 of m.
+__device__ __forceinline__ int scale_exponent(float m) { return m > 0.f && m < INFINITY ? min(max(14 - ilogbf(m), -100), 100) : 0; }
 
 // What a call's other launches need first: copies of operands, and the power
-// of two that takes the largest |grad_loss| of the rows that count to at most
-// 2^14, half precision's range (scale[0], its inverse in scale[1]; by the last
-// block).
+// of two that takes the largest |grad_loss| of the rows that count into half
+// precision's range (scale[0], its inverse in scale[1]; by the last block).
 struct Prep {
     PackJob job[3];
     int jobs = 0;

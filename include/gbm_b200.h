@@ -416,8 +416,8 @@ int gbm_softmax_xent(const void *x, int64_t ldx, const void *w, int64_t ldw, int
  * its dx is 0.  lse is gbm_softmax_xent's; grad_loss [n] f32.  G is made a piece of
  * classes at a time and rounded to `dtype` for the products (to half
  * precision times a power of two that follows the largest |grad_loss|, so
- * that small probabilities keep their bits); the products are summed in 32
- * bits.  ws: gbm_softmax_xent_workspace(n, d, v, 1, in_place) bytes, 256-byte aligned. */
+ * that small probabilities keep their bits down to 2^-39 of it); the products
+ * are summed in 32 bits.  ws: gbm_softmax_xent_workspace(n, d, v, 1, in_place) bytes, 256-byte aligned. */
 int gbm_softmax_xent_grad(const void *x, int64_t ldx, const void *w, int64_t ldw, int32_t dtype, int64_t n,
                           int64_t d, int64_t v, const int64_t *target, const float *lse,
                           const float *grad_loss, void *dx, int64_t lddx, void *dw, int64_t lddw, void *ws,

@@ -301,3 +301,27 @@ def test_infinite_logits(n, d, v, kind):
     w[1] = float("nan")                          # and a NaN among them
     assert torch.isnan(linear.softmax_xent(x, w, y)[1]).all()
     linear.status()
+
+
+@gpu
+@pytest.mark.parametrize("n", [400, 2000])
+@pytest.mark.parametrize("top", [2.0 ** 14, 1.9 * 2.0 ** 14])
+def test_half_gradients_of_rows_of_very_different_weights(n, top):
+    """Two classes and upstream gradients over ten decades (the largest one's row is near its target, so that its dx fits): what half precision's subnormals round away of G is at most
+    2^-39 of the largest upstream gradient (a power of two takes that to 2^14 at least, half a subnormal step is 2^-25),
+    beside one rounding of G and one of dx, and |c| p 2^-19 for p's own error (16 products, exp and log in 32 bits)."""
+    from bsscl_gbm_b200 import linear
+    x, w = _rand((n, 16), torch.float16, 1, 2.0 ** -12), _rand((2, 16), torch.float16, 2, 400.0)
+    y = torch.arange(n, device="cuda") % 2
+    apart = w[0].double() - w[1].double()
+    x[0] = (20.0 * apart / apart.square().sum()).half()
+    c = torch.exp2(-14.0 - (torch.arange(n, device="cuda") % 11)).float() * 1.37
+    c[0] = top
+    loss, lse = linear.softmax_xent(x, w, y)
+    dx, _ = linear.softmax_xent_grad(x, w, y, lse, c, want_dw=False)
+    linear.status()
+    p = torch.softmax(x.double() @ w.double().T, 1)
+    g = c.double()[:, None] * (p - torch.nn.functional.one_hot(y, 2))
+    want, u = g @ w.double(), 2.0 ** -11
+    tol = (u * g.abs() + c.double()[:, None] * 2.0 ** -19 + top * 2.0 ** -39) @ w.double().abs() + u * want.abs() + 2.0 ** -25
+    assert ((dx.double() - want).abs() <= tol).all(), float(((dx.double() - want).abs() / tol).max())
