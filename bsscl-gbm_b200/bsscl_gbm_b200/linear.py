@@ -78,7 +78,8 @@ class GradClip:
     device; float32, bfloat16 or float16, each dense), whose buffers it keeps;
     ``out`` (default: the gradients themselves) takes the clipped values.  No
     two buffers may overlap, but out[i] may be grads[i], and calls on two
-    streams at once would write the same outputs: wait between them.
+    streams at once would write the same outputs: wait between them.  A CUDA
+    graph that holds its calls needs the object as long as it is replayed.
     """
 
     def __init__(self, grads, out=None):

@@ -5,6 +5,7 @@
 // same checks and allocations took 8 us of a call whose kernel takes 5.
 #include <ATen/ATen.h>
 #include <Python.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -298,6 +299,8 @@ PyObject *grad_clip(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         const double most = PyFloat_AsDouble(args[2]);
         if (PyErr_Occurred()) return nullptr;
         Call c(dev, gbm_grad_clip_workspace(plan));
+        // the plan's owner may let go of it while this stream still reads it
+        c10::cuda::CUDACachingAllocator::recordStream(dev.storage().data_ptr(), c10::cuda::getCurrentCUDAStream(dev.get_device()));
         Tensor norm = fresh({}, dev, at::kFloat);
         c.done(gbm_grad_clip(plan, dev.data_ptr(), most, static_cast<float *>(norm.data_ptr()), c.ws, c.bytes, c.stream, c.err, sizeof c.err));
         return wrap(norm);

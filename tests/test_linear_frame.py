@@ -325,3 +325,27 @@ def test_half_gradients_of_rows_of_very_different_weights(n, top):
     want, u = g @ w.double(), 2.0 ** -11
     tol = (u * g.abs() + c.double()[:, None] * 2.0 ** -19 + top * 2.0 ** -39) @ w.double().abs() + u * want.abs() + 2.0 ** -25
     assert ((dx.double() - want).abs() <= tol).all(), float(((dx.double() - want).abs() / tol).max())
+
+
+@gpu
+def test_a_clip_that_is_let_go_while_another_stream_runs_it():
+    """The plan, made on one stream, is not handed to that stream's next tensors before the other stream has read it."""
+    from bsscl_gbm_b200 import linear
+    for size in (5, 70_000):
+        grads = [_rand((size + k,), torch.float32, k) for k in range(40)]
+        outs = [torch.zeros_like(g) for g in grads]
+        want = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
+        clip, side = linear.GradClip(grads, out=outs), torch.cuda.Stream()
+        room = clip._plan_dev.numel()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(50_000_000)          # some 30 ms
+            norm = clip.clip(1.0)
+        del clip
+        over = [torch.full((room,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        torch.cuda.synchronize()
+        assert abs(float(norm) - float(want)) <= 1e-6 * float(want)
+        c = float(torch.clamp(1.0 / (want + 1e-6), max=1.0))
+        for g, o in zip(grads, outs):
+            assert torch.allclose(o.double(), g.double() * c, rtol=1e-6, atol=0)
+        del over
