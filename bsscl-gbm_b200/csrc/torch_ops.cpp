@@ -156,7 +156,11 @@ PyObject *pair(const Tensor &a, const Tensor &b) {
     return t;
 }
 
-bool truth(PyObject *o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject *o) {
+    const int is = PyObject_IsTrue(o);
+    if (is < 0) throw python_error();      // an array of several values: Python's own error
+    return is == 1;
+}
 
 // C++ exceptions end here; torch's own become what torch makes of them.
 template <class F> PyObject *guarded(Py_ssize_t have, Py_ssize_t want, F f) {

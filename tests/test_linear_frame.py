@@ -8,6 +8,7 @@ import re
 import subprocess
 import time
 
+import numpy as np
 import pytest
 
 pytest.importorskip("torch")
@@ -349,3 +350,73 @@ def test_a_clip_that_is_let_go_while_another_stream_runs_it():
         for g, o in zip(grads, outs):
             assert torch.allclose(o.double(), g.double() * c, rtol=1e-6, atol=0)
         del over
+
+
+@gpu
+def test_a_wish_that_is_neither_true_nor_false():
+    from bsscl_gbm_b200 import linear
+    x, w, off = _rand((6, 16), torch.bfloat16, 1), _rand((1, 9, 16), torch.bfloat16, 2), torch.tensor([0, 6], dtype=torch.int32, device="cuda")
+    y, f = torch.zeros(6, dtype=torch.int64, device="cuda"), torch.zeros(6, device="cuda")
+    many = np.zeros(2)
+    for call in (lambda: linear.softmax_xent_grad(x, w[0], y, f, f, want_dx=many), lambda: linear.softmax_xent_grad(x, w[0], y, f, f, want_dw=many),
+                 lambda: linear.leaf_linear_grad(x, w, off, x[:, :9], want_dx=many), lambda: linear.leaf_linear_grad(x, w, off, x[:, :9], want_dw=many)):
+        with pytest.raises(ValueError, match="ambiguous"):
+            call()
+
+
+@gpu
+def test_calls_behind_copies_fills_and_other_streams():
+    """In order behind what another stream, a copy or a fill made: eagerly and captured with a fork and a join."""
+    from bsscl_gbm_b200 import linear
+    t, n, d, v = torch.bfloat16, 3000, 64, 5000
+    src = [_rand((n, d), t, k) for k in range(4)]
+    w, y, c = _rand((v, d), t, 9, 0.2), torch.arange(n, device="cuda") % v, torch.ones(n, device="cuda")
+    off, lw = torch.tensor([0, 1000, n], dtype=torch.int32, device="cuda"), _rand((2, 48, d), t, 10, 0.1)
+    x, side = torch.empty_like(src[0]), torch.cuda.Stream()
+
+    def work():
+        loss, lse = linear.softmax_xent(x, w, y)
+        return (loss, lse) + linear.softmax_xent_grad(x, w, y, lse, c) + (linear.leaf_linear(x, lw, off),)
+
+    def forked(a):
+        """x filled on this stream, then copied over on the side stream, worked on there and here after the join."""
+        main = torch.cuda.current_stream()
+        x.zero_()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            x.copy_(a)
+            there = work()
+            for o in there:
+                o.record_stream(main)
+        main.wait_stream(side)
+        here = work()
+        x.fill_(1.0)
+        return there, here, work()
+
+    want = []
+    for a in src:
+        x.copy_(a)
+        torch.cuda.synchronize()
+        want.append(work())
+        torch.cuda.synchronize()
+    x.fill_(1.0)
+    torch.cuda.synchronize()
+    ones = work()
+    torch.cuda.synchronize()
+
+    def check(got, k):
+        torch.cuda.synchronize()
+        for g, e in zip(got, (want[k], want[k], ones)):
+            for p, q in zip(g, e):
+                assert torch.equal(p, q)
+
+    for k, a in enumerate(src):
+        check(forked(a), k)
+    a, graph = src[0].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = forked(a)
+    for k in (2, 3, 1):
+        a.copy_(src[k])
+        graph.replay()
+        check(got, k)
+    linear.status()
