@@ -83,9 +83,11 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// A word of the cluster's CTA `rank`, at this address in its shared memory.
-__device__ __forceinline__ void store_at(uint32_t addr, uint32_t rank, int v) {
-    asm volatile("{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n st.shared::cluster.b32 [r], %2;\n}" ::"r"(addr), "r"(rank), "r"(v) : "memory");
+// The word at this address in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ int load_at(uint32_t addr, uint32_t rank) {
+    int v;
+    asm volatile("{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %1, %2;\n ld.shared::cluster.b32 %0, [r];\n}" : "=r"(v) : "r"(addr), "r"(rank) : "memory");
+    return v;
 }
 // Arrive on the same barrier of the cluster's CTA `rank`.  DATA: with writes
 // to shared memory that the other side is to see; tensor memory has its own fences.
@@ -151,9 +153,17 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void cluster_sync() {
+__device__ __forceinline__ void cluster_arrive() {
     __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    cluster_arrive();
+    cluster_wait();
 }
 
 // ---- TMA --------------------------------------------------------------------
@@ -465,29 +475,32 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         }
         if (lane < 16) mbar_init(swap + 8 * lane, 1);
         if (lane < 2 * kTold) mbar_init(told + 8 * lane, 1);
-        if (lane == 0) *dead = 0;
+        // whether a launch before this one has run out; the one directly in front may not have ended yet
+        if (lane == 0) *dead = *(volatile int *)&g_ops_timeout;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // whether a launch before this one has run out; the one directly in front may not have ended yet
-    const bool late = threadIdx.x == kThreads - 1 && *(volatile int *)&g_ops_timeout;
     cluster_sync();     // both CTAs run, their barriers stand
+    const bool none = load_at(smem_u32((const void *)dead), 0) | load_at(smem_u32((const void *)dead), 1);
     depend();
-    if (late) {
-        store_at(smem_u32((const void *)dead), 0, 1);
-        store_at(smem_u32((const void *)dead), 1, 1);
+    if (none) {
+        cluster_sync();
+        return;
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
         fence_before();
     }
-    cluster_sync();     // both have their tensor memory
-    fence_after();
-    const uint32_t tmem = *(volatile uint32_t *)tmem_slot;
-    const bool none = *dead;      // the same in both CTAs
+    // both have their tensor memory; the fetching warp, which does not touch it, goes ahead
+    cluster_arrive();
+    uint32_t tmem = 0;
+    if (warp) {
+        cluster_wait();
+        fence_after();
+        tmem = *(volatile uint32_t *)tmem_slot;
+    }
 
-    if (none) {
-    } else if (warp == 0) {
+    if (warp == 0) {
         // ---- fetch: one thread runs a tile's stages (a stage has 512 clocks)
         Ring r;
         typename Op::Iter it(op, cid, ncl);
@@ -518,6 +531,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         }
         // every product's end has reached this CTA's barriers before it leaves
         for (int i = 0; i < kStages && mbar_wait_warp(empty + 8 * r.s, r.ph ^ 1, dead); i++) r.step();
+        cluster_wait();
     } else if (warp == 1) {
         // ---- products, issued by one thread too
         if (rank == 0 && elect_one()) {
@@ -621,7 +635,7 @@ k_tc(const __grid_constant__ Maps maps, const __grid_constant__ Op op, const uin
         }
     }
     __syncwarp();
-    if (*dead && !none)
+    if (*dead)
         for (int i = 0; i < 1000; i++) __nanosleep(1000);    // copies in flight land meanwhile
     cluster_sync();     // nobody reads tensor memory any more
     fence_after();

@@ -30,11 +30,12 @@ def _frame():
 
 
 def test_tensor_memory_is_taken_and_freed_while_both_ctas_are_there():
-    """The cluster meets, the launch in front is over, tensor memory is allocated, the cluster meets; at the end it meets,
-    frees, and meets again before either CTA leaves."""
-    order = re.findall(r"cluster_sync\(\)|depend\(\)|tcgen05\.alloc|tcgen05\.dealloc|op\.epilogue", _frame())
-    assert order == ["cluster_sync()", "depend()", "tcgen05.alloc", "cluster_sync()", "op.epilogue",
-                     "cluster_sync()", "tcgen05.dealloc", "cluster_sync()"]
+    """The cluster meets, the launch in front is over, tensor memory is allocated, the cluster meets (the fetching warp, which
+    does not touch it, at the end of its role); at the end it meets, frees, and meets again before either CTA leaves.  A
+    launch that does nothing meets once more and leaves before it allocates."""
+    order = re.findall(r"cluster_(?:sync|arrive|wait)\(\)|depend\(\)|return;|tcgen05\.alloc|tcgen05\.dealloc|op\.epilogue|if \(warp\) ", _frame())
+    assert order == ["cluster_sync()", "depend()", "cluster_sync()", "return;", "tcgen05.alloc", "cluster_arrive()", "if (warp) ", "cluster_wait()",
+                     "cluster_wait()", "op.epilogue", "cluster_sync()", "tcgen05.dealloc", "cluster_sync()"]
 
 
 class _Bar:
