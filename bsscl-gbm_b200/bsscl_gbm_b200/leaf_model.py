@@ -113,15 +113,14 @@ class LeafLinearClassifier:
     # -- training -----------------------------------------------------------
     @staticmethod
     def _loss_scale(h, head, x_top):
-        """The power of two that takes a float16 step's gradients to at most
-        2^15, on the device.  A row's share of the loss is about 1 / rows, so
-        that its dh would lie among the type's subnormals or below.  With the
-        rows' weights c summing to 1 and sum_v |G_iv| <= 2 c_i:
-        |dhead| <= max |h|, |dh| and |dw| <= 2 max |head| max |x| (x has a
-        column of ones)."""
+        """The factor that takes a float16 step's gradients to at most 2^15, on
+        the device.  A row's share of the loss is about 1 / rows, so that its
+        dh would lie among the type's subnormals or below.  With the rows'
+        weights c summing to 1 and sum_v |G_iv| <= 2 c_i: |dhead| <= max |h|,
+        |dh| and |dw| <= 2 max |head| max |x| (x has a column of ones)."""
         import torch
-        top = torch.maximum(h.abs().amax().float(), 2.0 * head.abs().amax().float() * x_top)
-        return torch.exp2(torch.floor(15.0 - torch.log2(top.clamp(min=2.0 ** -14))))
+        h_top, head_top = (torch.linalg.vector_norm(a, math.inf, dtype=torch.float32) for a in (h, head))
+        return 2.0 ** 15 / torch.maximum(h_top, head_top * (2.0 * x_top)).add_(2.0 ** -14)
 
     def fit(self, X, y):
         import torch
@@ -161,7 +160,7 @@ class LeafLinearClassifier:
         clip = linear.GradClip([dw, dhead])
         self.loss_history_ = []
         half = dt == torch.float16
-        x_top = x.abs().amax().float() if half else None
+        x_top = float(x.abs().amax()) if half else None
         for _ in range(self.n_epochs):
             total = torch.zeros((), dtype=torch.float64, device=dev)
             shuffled = torch.randperm(len(x), generator=g, device=dev)
@@ -177,11 +176,14 @@ class LeafLinearClassifier:
                     c = c * scale
                 dh, _ = linear.softmax_xent_grad(h, head, yb, lse, c, dw_out=dhead)
                 linear.leaf_linear_grad(xb, w, offsets, dh, want_dx=False, dw_out=dw)
-                # scaled gradients are clipped where they are scaled back, in float32
                 norm = clip.clip(math.inf if half else self.max_norm)
-                step = torch.clamp(self.max_norm / (norm / scale + 1e-6), max=1.0) / scale if half else None
+                if half:      # clipped where they are scaled back, in float32
+                    step = torch.minimum(self.max_norm / torch.add(norm, scale, alpha=1e-6), 1.0 / scale)
                 for master, copy, grad in ((w32, w, dw), (head32, head, dhead)):
-                    master.add_(grad.float() * step if half else grad.float(), alpha=-self.learning_rate)
+                    if half:
+                        master.addcmul_(grad.float(), step, value=-self.learning_rate)
+                    else:
+                        master.add_(grad.float(), alpha=-self.learning_rate)
                     copy.copy_(master)
                 total += loss.sum(dtype=torch.float64)
             linear.status(dev)

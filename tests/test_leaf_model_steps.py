@@ -143,12 +143,13 @@ def test_half_precision_step(on_cpu, n, classes, n_hidden, few):
 
 
 @pytest.mark.parametrize("h,head,x_top", [(4.0, 0.05, 6.0), (300.0, 2.0, 50.0), (0.0, 0.0, 1.0), (60000.0, 3.0, 1e4), (1.0, 1e-7, 1.0)])
-def test_half_precision_scale_is_a_power_of_two_within_range(h, head, x_top):
+@pytest.mark.parametrize("kind", [torch.float16, torch.float32])
+def test_half_precision_scale_fills_the_range(h, head, x_top, kind):
     from bsscl_gbm_b200 import LeafLinearClassifier
-    scale = float(LeafLinearClassifier._loss_scale(torch.tensor([[h, -h / 2]]), torch.tensor([[head / 3, -head]]), torch.tensor(x_top)))
+    scale = float(LeafLinearClassifier._loss_scale(torch.tensor([[h, -h / 2]], dtype=kind), torch.tensor([[head / 3, -head]], dtype=kind), x_top))
     most = max(h, 2 * head * x_top)
-    assert scale > 0 and np.log2(scale) == int(np.log2(scale)) and scale * most <= 2.0 ** 15
-    assert most < 2.0 ** -13 or scale * most > 2.0 ** 13
+    assert 0 < scale <= 2.0 ** 29 and scale * most <= 2.0 ** 15 * 1.001
+    assert most < 2.0 ** -13 or scale * most > 2.0 ** 14
 
 
 def test_each_rank_takes_its_own_gpu(monkeypatch):
