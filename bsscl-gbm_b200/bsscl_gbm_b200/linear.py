@@ -13,9 +13,11 @@ model whose leaves hold linear maps under a softmax head of many classes:
 
 Every call runs on the current stream of its tensors' device, whatever the
 current device is, waits for nothing, and may be captured into a CUDA graph.
-There is no CPU path.  Wrong types, shapes, strides and devices, and a given
-output that overlaps what its call reads, raise ValueError before anything is
-launched.
+There is no CPU path.  The operators know no autograd: tensors that require
+gradients are taken as they are, results require none, and the gradients are
+what the ``_grad`` calls return (``backward()`` finds nothing behind a
+result).  Wrong types, shapes, strides and devices, and a given output that
+overlaps what its call reads, raise ValueError before anything is launched.
 """
 
 from __future__ import annotations
@@ -37,16 +39,20 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}     # GBM_TYPE_
 
 def softmax_xent(x, w, target):
     """Softmax cross entropy of the linear head ``x @ w.T`` without keeping
-    the logits: ``(loss, lse)``, float32 [n].  x [n, d] and w [v, d] bfloat16
-    or float16 (rows contiguous, any row stride), target int64 [n].  A row
-    whose target is outside 0..v-1 is ignored: its loss is 0."""
+    the logits: ``(loss, lse)``, float32 [n] and computed in 32 bits.  x [n, d]
+    and w [v, d] bfloat16 or float16 (rows contiguous, any row stride that keeps
+    them apart), target int64 [n].  A row whose target is outside 0..v-1 is
+    ignored: its loss is 0."""
     return _ops.softmax_xent(x, w, target)
 
 
 def softmax_xent_grad(x, w, target, lse, grad_loss, want_dx=True, want_dw=True, dw_out=None):
     """Gradients ``(dx, dw)`` of ``sum(grad_loss * loss)`` in the operands'
     type; lse as :func:`softmax_xent` returned it, grad_loss float32 [n].
-    Ignored rows get dx = 0 and add nothing to dw.  ``want_dx=False`` /
+    Ignored rows get dx = 0 and add nothing to dw.  The rows x classes matrix
+    between them is rounded to the operands' type once (up to 256 rows it is
+    kept in two parts), in float16 relative to the largest ``|grad_loss|`` (down
+    to 2^-39 of it); products are summed in 32 bits.  ``want_dx=False`` /
     ``want_dw=False`` give None in that place and save its product;
     ``dw_out`` (of w's shape and type, rows contiguous) takes dw, so that a
     :class:`GradClip` made once for it stays good."""
@@ -55,8 +61,8 @@ def softmax_xent_grad(x, w, target, lse, grad_loss, want_dx=True, want_dw=True, 
 
 def leaf_linear(x, w, offsets, out=None):
     """Products grouped by leaf: row r of leaf g, offsets[g] <= r <
-    offsets[g+1], gives ``y[r] = w[g] @ x[r]``.  x [t, din] (rows contiguous,
-    any row stride), w [leaves, dout, din] contiguous, both bfloat16 or
+    offsets[g+1], gives ``y[r] = w[g] @ x[r]``.  x [t, din] (rows as
+    :func:`softmax_xent`'s), w [leaves, dout, din] contiguous, both bfloat16 or
     float16; offsets int32 [leaves + 1] on the device, non-decreasing within
     0..t.  Rows that no leaf has (before offsets[0], from offsets[-1] on) are
     0 in a new y and left as they were in ``out``."""
@@ -76,7 +82,9 @@ class GradClip:
 
     Made once for the gradients of a model (a list of CUDA tensors of one
     device; float32, bfloat16 or float16, each dense), whose buffers it keeps;
-    ``out`` (default: the gradients themselves) takes the clipped values.  No
+    ``out`` (default: the gradients themselves) takes the clipped values.  Making
+    it takes some 40 us for 5 gradients and 0.9 ms for 300 (checks, and a copy
+    that waits): keep it, and the gradients in their buffers, from step to step.  No
     two buffers may overlap, but out[i] may be grads[i], and calls on two
     streams at once would write the same outputs: wait between them.  A CUDA
     graph that holds its calls needs the object as long as it is replayed.

@@ -325,9 +325,11 @@ struct DenseIter {
 // 512 bytes of each at a time, straight into the operand's registers: a lane's
 // 16 bytes are 8 values of k of one row, and as both operands are read alike,
 // it does not matter that the instruction counts these k's in another order.
-// 1 row x 1024 against 32768 classes: 10.9 us on the device (67 MB, 6.2 TB/s
-// with the joining launch), 64 rows through 63 leaves of 1024 x 1024 23.6 us
-// (132 MB, 5.6 TB/s).
+// 1 row x 1024 against 32768 classes: 16 us with the joining launch (67 MB, 4.2
+// TB/s; 256 blocks on 148 SMs, so that some have two and some one), 64 rows
+// through 63 leaves of 1024 x 1024 23.2 us (132 MB, 5.7 TB/s).  Two blocks an SM
+// leave a thread 128 registers: k_leaf_few spills 24 bytes, k_xent_few with up
+// to 8 rows 8.
 
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __nv_bfloat16) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -851,6 +853,12 @@ struct XentPlan {
         // One tile of rows: the products are bound by memory and launches,
         // and few rounded values of G weigh in a result (with one row a
         // single one), whose rounding does not average out: keep G in two parts.
+        // With more rows G is rounded once, as the results are: dx and dw are
+        // 1.43 times as far from 64 bits as with two parts (norm-wise 2.4e-3
+        // against 1.66e-3 in bf16, 3.0e-4 against 2.1e-4 in half precision).
+        // Two parts double the products: one / two parts, us, 999 x 100 x 1501
+        // 24 / 30, 8192 x 64 x 1000 28 / 36, 2048 x 256 x 8192 47 / 67,
+        // 4096 x 512 x 16384 189 / 343.
         parts = n <= 256 ? 2 : 1;
         constexpr int64_t kMost = 512 << 20;
         pieces = (int)std::min<int64_t>((n * v * 2 * parts + kMost - 1) / kMost, (v + 255) / 256);
