@@ -129,6 +129,8 @@ class LeafLinearClassifier:
         X, y = self._check(X), np.asarray(y)
         if len(y) != len(X):
             raise ValueError(f"X has {len(X)} rows but y has {len(y)}")
+        if not self.max_norm >= 0:
+            raise ValueError(f"max_norm must not be negative, got {self.max_norm}")
         classes, index = np.unique(y, return_inverse=True)
         if len(classes) < 2:
             raise ValueError("y holds a single class")

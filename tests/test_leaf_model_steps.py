@@ -152,6 +152,21 @@ def test_half_precision_scale_fills_the_range(h, head, x_top, kind):
     assert most < 2.0 ** -13 or scale * most > 2.0 ** 14
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("max_norm", [-1.0, float("nan")])
+def test_a_negative_norm_is_refused(on_cpu, dtype, max_norm):
+    """In either type, before anything is learnt; 0 and infinity are limits like others."""
+    from bsscl_gbm_b200 import LeafLinearClassifier
+    X, y = _data()
+    kw = dict(n_hidden=4, n_epochs=1, batch_size=128, dtype=dtype)
+    with pytest.raises(ValueError, match="max_norm"):
+        LeafLinearClassifier(max_norm=max_norm, **kw).fit(X, y)
+    still, free = (LeafLinearClassifier(max_norm=m, **kw).fit(X, y) for m in (0.0, float("inf")))
+    start = LeafLinearClassifier(learning_rate=0.0, **kw).fit(X, y)
+    assert torch.equal(still._w, start._w) and torch.equal(still._head, start._head)
+    assert torch.isfinite(free._w).all() and not torch.equal(free._w, start._w)
+
+
 def test_each_rank_takes_its_own_gpu(monkeypatch):
     """As the routing estimator does: LOCAL_RANK's in a process group, the first one elsewhere, a named one always."""
     from bsscl_gbm_b200 import LeafLinearClassifier, leaf_model
