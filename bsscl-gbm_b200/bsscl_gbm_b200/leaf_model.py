@@ -59,6 +59,7 @@ class LeafLinearClassifier:
     Weights are kept in float32 and multiplied in ``dtype``; in float16 each
     step's loss is scaled so that the gradients fill the type's range.  Features
     are standardised; a missing or infinite value counts as the mean.
+    random_state None starts from another state at each fit.
     """
 
     def __init__(self, router=None, tree=0, n_hidden=64, learning_rate=0.5, max_norm=1.0, n_epochs=10, batch_size=8192,
@@ -151,7 +152,8 @@ class LeafLinearClassifier:
         x, leaf = self._features(X), torch.from_numpy(route.astype(np.int64)).to(dev)
         target = torch.from_numpy(index.astype(np.int64).reshape(-1)).to(dev)
         weight = torch.from_numpy(weight).to(dev, torch.float32)
-        g = torch.Generator(device=dev).manual_seed(int(self.random_state))
+        g = torch.Generator(device=dev).manual_seed(
+            int.from_bytes(os.urandom(7), 'little') if self.random_state is None else int(self.random_state))
         p = x.shape[1]
         # one start for all leaves: they part where their rows differ
         first = torch.randn(1, self.n_hidden, p, generator=g, device=dev) * p ** -0.5

@@ -167,6 +167,13 @@ def test_a_negative_norm_is_refused(on_cpu, dtype, max_norm):
     assert torch.isfinite(free._w).all() and not torch.equal(free._w, start._w)
 
 
+def test_a_fit_without_a_random_state(on_cpu):
+    from bsscl_gbm_b200 import LeafLinearClassifier
+    X, y = _data()
+    a, b = (LeafLinearClassifier(n_hidden=4, n_epochs=1, batch_size=128, random_state=None).fit(X, y) for _ in range(2))
+    assert torch.isfinite(a._w).all() and not torch.equal(a._w, b._w)
+
+
 def test_each_rank_takes_its_own_gpu(monkeypatch):
     """As the routing estimator does: LOCAL_RANK's in a process group, the first one elsewhere, a named one always."""
     from bsscl_gbm_b200 import LeafLinearClassifier, leaf_model
